@@ -318,6 +318,138 @@ void q3vl_checkpoint_free(q3vl_checkpoint *ck);
 int q3vl_quantize_groupwise(const float *x, size_t count, size_t group, int8_t *q,
                             float *scales, q3vl_stream stream);
 
+/* ---- rows of tokens over the caches: a prompt, one token of each sequence of
+ * a batch, or trees of drafted tokens checked in one pass. No counterpart in
+ * the reference, which runs one token of one sequence at a time. Around the
+ * linears one layer is q3vl_qk_norm_rope, then q3vl_tree_attention;
+ * q3vl_draft_plan runs once a step ahead of the layers, q3vl_token_logprobs
+ * scores the step's logits.
+ *
+ * A batch: `rows` rows of tokens, those of sequence b at row_start[b] ..
+ * row_start[b+1] - 1 (row_start [batch + 1] int32, ascending from 0; a
+ * sequence may have none). row_start and cache_len [batch] int32 (positions
+ * cached before this step) live in device memory, so that a captured call
+ * replays with other lengths. Rows behind the last sequence hold no token.
+ * Values there are clamped to the arrays: no row_start or cache_len makes a
+ * call read or write outside of its buffers. */
+
+/* One layer's caches of a batch, fp16. Row r of kv head h of sequence b is the
+ * head_dim values at b * seq_stride + h * head_stride + r * row_stride
+ * (elements, the same for k and v; multiples of 8, pointers 16-byte aligned).
+ * The decode step's caches are batch 1, head_stride max_seq * head_dim,
+ * row_stride head_dim, from a layer's first element on. */
+typedef struct q3vl_kv_cache {
+    uint16_t *k, *v;
+    int batch, kv_heads, max_seq, head_dim;
+    size_t seq_stride, head_stride, row_stride;
+} q3vl_kv_cache;
+
+/* One layer's head norms: int8 weights [head_dim] under fp32 scales
+ * [head_dim / group_size], as q3vl_text_model holds them. */
+typedef struct q3vl_head_norm {
+    const int8_t *q_w;
+    const float *q_s;
+    const int8_t *k_w;
+    const float *k_s;
+    int group_size;
+    float eps;
+} q3vl_head_norm;
+
+/* Rotary tables [rows, head_dim/2] (q3vl_rope_tables) and which position turns
+ * which frequency. axes 1: the row's one position. axes 3 (time, height,
+ * width; images and video): sections[a] frequencies turn by axis a, adding up
+ * to head_dim/2; interleaved 0: axis by axis in that order, 1: frequency
+ * 3 n + a by axis a = 1, 2 for n < sections[a] (at most head_dim/6), the rest
+ * by time. */
+typedef struct q3vl_rope {
+    const float *cos, *sin;
+    int rows;
+    int axes;
+    int sections[3];
+    int interleaved;
+} q3vl_rope;
+
+/* Plans one step over drafts. parents [rows]: the row's parent among its
+ * sequence's own rows, or -1 where it follows the last cached token; a parent
+ * comes before its children. For row t of sequence b:
+ *   mask  [rows, mask_words] uint64: bit j of the row's words (bit j % 64 of
+ *         word j / 64) for j = t and each of its ancestors j;
+ *   pos   [rows] int32: cache_len[b] + pos_delta[b] + number of ancestors
+ *         (pos_delta NULL: 0);
+ *   slots [rows] int64: b * max_seq + cache_len[b] + t.
+ * A row behind the last sequence gets an empty mask, position -1 and slot -1
+ * (no token: q3vl_qk_norm_rope leaves it alone). A row that cannot be planned
+ * gets an empty mask, position -2 and slot -1 (its query becomes NaN): one
+ * whose chain of parents leaves [-1, its own index), one past max_rows or past
+ * the cache, and every row of a sequence whose cache_len is negative.
+ * max_rows: the most rows of one sequence (at most 1024); mask_words at least
+ * ceil(max_rows / 64). */
+int q3vl_draft_plan(const int32_t *parents, const int32_t *row_start, const int32_t *cache_len,
+                    const int32_t *pos_delta, int batch, size_t rows, int max_rows, int max_seq,
+                    uint64_t *mask, int mask_words, int32_t *pos, int64_t *slots,
+                    q3vl_stream stream);
+
+/* Head norms, rotation and cache stores of one layer's q, k and v rows. For
+ * each head x of q and k: y = w * ((s_g * inv) * x), inv = 1 / sqrt(mean(x^2) +
+ * eps), then (y_i, y_{i + head_dim/2}) turned by the table's row of the
+ * position that frequency i belongs to (rope->axes positions a row in pos).
+ * q_out [rows, heads * head_dim] fp32 or fp16 (q_dtype; fp32: q_out may be q
+ * itself, with its stride); k and v go to the cache as fp16, to the row that
+ * slots[r] = b * max_seq + row names. With one axis and head_dim 128 every
+ * value stored is the decode step's, bit for bit.
+ * q, k, v: fp32, row strides ldq, ldk, ldv in elements (views of one
+ * projection's output are fine). A row whose first position is -1 holds no
+ * token: nothing is read or written for it. Another position outside of
+ * [0, rope->rows) makes the row's q_out NaN and stores nothing in the cache; a
+ * slot outside of [0, batch * max_seq) stores nothing in the cache. Two rows
+ * with one slot: each element kept is either's. head_dim 64 or 128. */
+int q3vl_qk_norm_rope(const float *q, size_t ldq, const float *k, size_t ldk, const float *v,
+                      size_t ldv, void *q_out, size_t ldo, int q_dtype, size_t rows, int heads,
+                      const q3vl_kv_cache *cache, const int64_t *slots, const int32_t *pos,
+                      const q3vl_head_norm *norm, const q3vl_rope *rope, q3vl_stream stream);
+
+/* Attention of each row over its sequence's cache: out = sum_j p_j v_j, p the
+ * softmax of scale * q.k_j over the rows j of the cache that the row sees:
+ * j < cache_len[b], and of the step's own rows (cached at cache_len[b] + i for
+ * row i of the sequence) those whose bit i is set in the row's mask. mask
+ * [rows, mask_words] as q3vl_draft_plan writes it (bits of rows the sequence
+ * does not have count for nothing, rows past 64 * mask_words are not seen), or
+ * NULL: row t sees rows 0 .. t, a prompt's chunk or a single new token. A row
+ * that sees nothing gives 0. What a row does not see does not touch its
+ * result, infinities and NaN included.
+ * q, out: [rows, heads * head_dim] fp32 or fp16 (`dtype`, both the same), row
+ * strides ldq and ldo; heads a multiple of cache->kv_heads, query head h reads
+ * kv head h / (heads / kv_heads). Products in fp16 matrix instructions with
+ * fp32 sums: fp32 queries and their probabilities as two fp16 terms each
+ * (relative 2^-21), fp16 ones as one. The rows of a sequence with cache_len[b]
+ * < 0 or cache_len[b] + its rows > max_seq give NaN, reading nothing. Rows
+ * behind the last sequence, and rows of a sequence past max_rows, are left as
+ * they were in `out`. max_rows: the most rows of one sequence. max_len: the
+ * most cached positions of one sequence with its rows, used only to choose how
+ * far the work is split (0: max_seq). head_dim 64 or 128. */
+size_t q3vl_tree_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
+                                           const q3vl_kv_cache *cache);
+int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,
+                        int heads, const q3vl_kv_cache *cache, const int32_t *row_start,
+                        const int32_t *cache_len, const uint64_t *mask, int mask_words,
+                        int max_rows, int max_len, float scale, void *workspace,
+                        size_t workspace_bytes, q3vl_stream stream);
+
+/* What each row of logits [M, V] (fp32 or fp16, row stride ld in elements)
+ * says: logprob[m] of tokens[m] (log softmax), rank[m] = how many values stand
+ * ahead of it, entropy[m] = -sum p log p, and the top_k (at most 64 and V)
+ * best values, top_ids and top_logprobs [M, top_k]. Order: larger values
+ * first, equal ones (-0 and 0 among them) by their index; NaN stands with
+ * -inf. rank, entropy and, for top_k 0, the top arrays may be NULL. A logit of
+ * -inf has probability 0. A row with a NaN or +inf, or with nothing but -inf,
+ * has NaN log probabilities and entropy; its ids and rank stand. A token
+ * outside of [0, V) gives NaN and rank -1. */
+size_t q3vl_token_logprobs_workspace_bytes(size_t M, size_t V);
+int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t *tokens,
+                        size_t M, size_t V, int top_k, float *logprob, int32_t *rank,
+                        float *entropy, int32_t *top_ids, float *top_logprobs, void *workspace,
+                        size_t workspace_bytes, q3vl_stream stream);
+
 /* ---- weight registry for host-pointer callers (the drop-in linear()).
  * The reference hands linear() mmapped host pointers to weights and scales
  * (model/src/load_model.cpp:146-181); the registry uploads a weight once and

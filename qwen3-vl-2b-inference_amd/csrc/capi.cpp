@@ -1416,4 +1416,231 @@ int q3vl_quantize_groupwise(const float *x, size_t count, size_t group, int8_t *
     return Q3VL_OK;
 }
 
+// ---- rows of tokens over the caches
+
+static int check_cache(const q3vl_kv_cache *c) {
+    if (!c || !c->k || !c->v) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null cache");
+    if (c->batch < 1 || c->kv_heads < 1 || c->max_seq < 1)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad cache: batch=%d kv_heads=%d max_seq=%d", c->batch, c->kv_heads, c->max_seq);
+    if (c->head_dim != 64 && c->head_dim != 128)
+        return fail(Q3VL_ERR_UNSUPPORTED, "head_dim=%d: 64 or 128 are served", c->head_dim);
+    if (!aligned16(c->k) || !aligned16(c->v) || c->seq_stride % 8 || c->head_stride % 8 || c->row_stride % 8)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "cache rows must be 16-byte aligned");
+    const size_t d = (size_t)c->head_dim;
+    // (a tile of the attention addresses its rows by 32-bit byte offsets)
+    if (c->row_stride < d || c->row_stride > (1u << 23) || c->seq_stride > (SIZE_MAX >> 20) || c->head_stride > (SIZE_MAX >> 20))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad cache strides (row_stride=%zu)", c->row_stride);
+    return Q3VL_OK;
+}
+
+int q3vl_draft_plan(const int32_t *parents, const int32_t *row_start, const int32_t *cache_len,
+                    const int32_t *pos_delta, int batch, size_t rows, int max_rows, int max_seq,
+                    uint64_t *mask, int mask_words, int32_t *pos, int64_t *slots, q3vl_stream stream) {
+    if (batch < 0 || max_rows < 0 || max_seq < 1)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape batch=%d max_rows=%d max_seq=%d", batch, max_rows, max_seq);
+    if (max_rows > kDraftRows)
+        return fail(Q3VL_ERR_UNSUPPORTED, "max_rows=%d: at most %d rows a sequence", max_rows, kDraftRows);
+    if (rows > 0x7fffffff || batch > 0x7ffffffe)
+        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu batch=%d)", rows, batch);
+    if (mask_words < (max_rows + 63) / 64)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "mask_words=%d do not hold %d rows", mask_words, max_rows);
+    if (rows == 0) return Q3VL_OK;
+    if (!parents || !row_start || !cache_len || !pos || !slots || (mask_words && !mask))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    Q3VL_HIP(launch_draft_plan(parents, row_start, cache_len, pos_delta, batch, (int)rows, max_rows, max_seq, mask,
+                               mask_words, pos, slots, (hipStream_t)stream),
+             "draft plan launch");
+    return Q3VL_OK;
+}
+
+int q3vl_qk_norm_rope(const float *q, size_t ldq, const float *k, size_t ldk, const float *v,
+                      size_t ldv, void *q_out, size_t ldo, int q_dtype, size_t rows, int heads,
+                      const q3vl_kv_cache *cache, const int64_t *slots, const int32_t *pos,
+                      const q3vl_head_norm *norm, const q3vl_rope *rope, q3vl_stream stream) {
+    const int rc = check_cache(cache);
+    if (rc) return rc;
+    if (!norm || !rope) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null norm / rope");
+    if (q_dtype != Q3VL_DTYPE_FP32 && q_dtype != Q3VL_DTYPE_FP16)
+        return fail(Q3VL_ERR_UNSUPPORTED, "q_dtype=%d: fp32 or fp16 are served", q_dtype);
+    if (heads < 1) return fail(Q3VL_ERR_INVALID_ARGUMENT, "heads=%d", heads);
+    const int D = cache->head_dim;
+    const size_t qn = (size_t)heads * D, kn = (size_t)cache->kv_heads * D;
+    if (ldq < qn || ldo < qn || ldk < kn || ldv < kn)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "a row stride is shorter than its row");
+    if (q_out == q && (q_dtype != Q3VL_DTYPE_FP32 || ldo != ldq) && rows > 0)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "q_out over q needs fp32 and q's stride");
+    if (norm->group_size < 1 || D % norm->group_size)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "group_size=%d does not divide head_dim=%d", norm->group_size, D);
+    if (rope->rows < 1) return fail(Q3VL_ERR_INVALID_ARGUMENT, "empty rotary tables");
+    if (rope->axes != 1 && rope->axes != 3) return fail(Q3VL_ERR_UNSUPPORTED, "axes=%d: 1 or 3 are served", rope->axes);
+    if (rope->axes == 3) {
+        const int *s = rope->sections;
+        for (int i = 0; i < 3; ++i)
+            if (s[i] < 0 || s[i] > D / 2) return fail(Q3VL_ERR_INVALID_ARGUMENT, "section %d of %d frequencies", i, s[i]);
+        if (s[0] + s[1] + s[2] != D / 2)
+            return fail(Q3VL_ERR_INVALID_ARGUMENT, "sections %d + %d + %d are not %d frequencies", s[0], s[1], s[2], D / 2);
+        if (rope->interleaved && (3 * s[1] > D / 2 || 3 * s[2] > D / 2))
+            return fail(Q3VL_ERR_INVALID_ARGUMENT, "interleaved sections %d, %d exceed a third of %d", s[1], s[2], D / 2);
+    }
+    if (rows > 0x7fffffff || heads > (1 << 20) || cache->kv_heads > (1 << 20) ||
+        rows * (((size_t)heads + 2 * (size_t)cache->kv_heads + 15) / 16) > 0x7fffffff)
+        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu heads=%d)", rows, heads);
+    if (rows == 0) return Q3VL_OK;
+    if (!q || !k || !v || !q_out || !slots || !pos || !norm->q_w || !norm->q_s || !norm->k_w || !norm->k_s || !rope->cos || !rope->sin)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    QkRopeArgs a{};
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.ldq = (int64_t)ldq;
+    a.ldk = (int64_t)ldk;
+    a.ldv = (int64_t)ldv;
+    a.q_out = q_out;
+    a.ldo = (int64_t)ldo;
+    a.rows = (int64_t)rows;
+    a.slots = slots;
+    a.pos = pos;
+    a.q_w = norm->q_w;
+    a.q_s = norm->q_s;
+    a.k_w = norm->k_w;
+    a.k_s = norm->k_s;
+    a.cos = rope->cos;
+    a.sin = rope->sin;
+    a.k_cache = cache->k;
+    a.v_cache = cache->v;
+    a.seq_stride = cache->seq_stride;
+    a.head_stride = cache->head_stride;
+    a.row_stride = cache->row_stride;
+    a.heads = heads;
+    a.kv_heads = cache->kv_heads;
+    a.batch = cache->batch;
+    a.max_seq = cache->max_seq;
+    a.gs = norm->group_size;
+    a.table_rows = rope->rows;
+    a.sec0 = rope->sections[0];
+    a.sec1 = rope->sections[1];
+    a.sec2 = rope->sections[2];
+    a.interleaved = rope->interleaved;
+    a.eps = norm->eps;
+    Q3VL_HIP(launch_qk_norm_rope(a, D, q_dtype == Q3VL_DTYPE_FP16, rope->axes, (hipStream_t)stream), "head norm launch");
+    return Q3VL_OK;
+}
+
+// Sizes of a call, checked; its splits and workspace bytes.
+static int tree_attention_plan(size_t rows, int heads, int max_rows, int max_len, const q3vl_kv_cache *c, int *splits,
+                               size_t *bytes) {
+    const int rc = check_cache(c);
+    if (rc) return rc;
+    if (heads < 1 || heads % c->kv_heads)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "heads=%d is not a multiple of kv_heads=%d", heads, c->kv_heads);
+    if (max_rows < 0 || max_len < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "max_rows=%d max_len=%d", max_rows, max_len);
+    if (rows > 0x7fffffff / (size_t)heads || (int64_t)max_rows * (heads / c->kv_heads) > 0x7fffff00)
+        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu heads=%d)", rows, heads);
+    if ((size_t)max_rows > rows) max_rows = (int)rows;
+    if (max_len == 0 || max_len > c->max_seq) max_len = c->max_seq;
+    *splits = tree_attention_splits((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, max_len);
+    if (*splits < 0) return fail(Q3VL_ERR_UNSUPPORTED, "too many blocks (batch=%d max_rows=%d)", c->batch, max_rows);
+    const size_t parts = rows * (size_t)heads * (size_t)*splits;
+    *bytes = *splits > 1 ? align256(parts * (size_t)c->head_dim * 4) + align256(parts * 8) : 0;
+    return Q3VL_OK;
+}
+
+size_t q3vl_tree_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
+                                           const q3vl_kv_cache *cache) {
+    int splits = 0;
+    size_t bytes = 0;
+    return tree_attention_plan(rows, heads, max_rows, max_len, cache, &splits, &bytes) ? 0 : bytes;
+}
+
+int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,
+                        int heads, const q3vl_kv_cache *cache, const int32_t *row_start,
+                        const int32_t *cache_len, const uint64_t *mask, int mask_words,
+                        int max_rows, int max_len, float scale, void *workspace,
+                        size_t workspace_bytes, q3vl_stream stream) {
+    int splits = 0;
+    size_t need = 0;
+    int rc = tree_attention_plan(rows, heads, max_rows, max_len, cache, &splits, &need);
+    if (rc) return rc;
+    if (dtype != Q3VL_DTYPE_FP32 && dtype != Q3VL_DTYPE_FP16)
+        return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
+    const size_t qn = (size_t)heads * cache->head_dim;
+    if (ldq < qn || ldo < qn) return fail(Q3VL_ERR_INVALID_ARGUMENT, "a row stride is shorter than its row");
+    if (mask_words < 0 || (mask && mask_words < 1) || mask_words > (1 << 24))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "mask_words=%d", mask_words);
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "scale is not finite");
+    if (rows == 0 || max_rows == 0) return Q3VL_OK;
+    if (!q || !out || !row_start || !cache_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    char *w = nullptr;
+    if (need && (rc = resolve_ws(workspace, workspace_bytes, need, &w))) return rc;
+    TreeAttnArgs a{};
+    a.q = q;
+    a.out = out;
+    a.ldq = (int64_t)ldq;
+    a.ldo = (int64_t)ldo;
+    a.k_cache = cache->k;
+    a.v_cache = cache->v;
+    a.seq_stride = cache->seq_stride;
+    a.head_stride = cache->head_stride;
+    a.row_stride = cache->row_stride;
+    a.row_start = row_start;
+    a.cache_len = cache_len;
+    a.mask = mask;
+    a.part_o = reinterpret_cast<float *>(w);
+    a.part_ml = need ? reinterpret_cast<float *>(w + align256(rows * (size_t)heads * splits * cache->head_dim * 4)) : nullptr;
+    a.rows = (int)rows;
+    a.heads = heads;
+    a.kv_heads = cache->kv_heads;
+    a.batch = cache->batch;
+    a.max_seq = cache->max_seq;
+    a.max_rows = (size_t)max_rows > rows ? (int)rows : max_rows;
+    a.words = mask_words;
+    a.splits = splits;
+    a.scale_log2e = (float)((double)scale * 1.4426950408889634);
+    Q3VL_HIP(launch_tree_attention(a, cache->head_dim, dtype == Q3VL_DTYPE_FP16, (hipStream_t)stream), "attention launch");
+    return Q3VL_OK;
+}
+
+size_t q3vl_token_logprobs_workspace_bytes(size_t M, size_t V) {
+    if (M == 0 || V == 0 || V > 0x7fffff00 || M > 0x7fffffff) return 0;
+    return align256(M * (size_t)logprob_parts((int)M, (int)V) * 16) + align256(M * (size_t)logprob_subs((int)V) * 4);
+}
+
+int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t *tokens, size_t M,
+                        size_t V, int top_k, float *logprob, int32_t *rank, float *entropy,
+                        int32_t *top_ids, float *top_logprobs, void *workspace,
+                        size_t workspace_bytes, q3vl_stream stream) {
+    if (dtype != Q3VL_DTYPE_FP32 && dtype != Q3VL_DTYPE_FP16)
+        return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
+    if (V == 0 || V > 0x7fffff00 || ld < V || ld > (SIZE_MAX >> 24))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape V=%zu ld=%zu", V, ld);
+    if (top_k < 0 || top_k > kLogprobTop || (size_t)top_k > V)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "top_k=%d: 0 to %d, at most V=%zu", top_k, kLogprobTop, V);
+    if (M == 0) return Q3VL_OK;
+    if (M > 0x7fffffff || M * (size_t)logprob_parts((int)M, (int)V) > 0x7fffffff)
+        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (M=%zu V=%zu)", M, V);
+    if (!logits || !tokens || !logprob || (top_k && (!top_ids || !top_logprobs)))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((uintptr_t)logits % (dtype == Q3VL_DTYPE_FP16 ? 2 : 4)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned logits");
+    char *w = nullptr;
+    const int rc = resolve_ws(workspace, workspace_bytes, q3vl_token_logprobs_workspace_bytes(M, V), &w);
+    if (rc) return rc;
+    LogprobArgs a{};
+    a.logits = logits;
+    a.ld = (int64_t)ld;
+    a.tokens = tokens;
+    a.M = (int)M;
+    a.V = (int)V;
+    a.k = top_k;
+    a.parts = logprob_parts((int)M, (int)V);
+    a.part = reinterpret_cast<float *>(w);
+    a.sub_max = reinterpret_cast<float *>(w + align256(M * (size_t)a.parts * 16));
+    a.logprob = logprob;
+    a.rank = rank;
+    a.entropy = entropy;
+    a.top_ids = top_ids;
+    a.top_logprobs = top_logprobs;
+    Q3VL_HIP(launch_token_logprobs(a, dtype == Q3VL_DTYPE_FP16, (hipStream_t)stream), "log probability launch");
+    return Q3VL_OK;
+}
+
 }  // extern "C"

@@ -39,22 +39,6 @@ __device__ __forceinline__ float exp256(float x) {
     return y * __uint_as_float((uint32_t)(n + 127) << 23);
 }
 
-__device__ __forceinline__ float h2f(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
-// fp32 -> fp16 bits, round to nearest even (NaN -> sign | 0x7E00), as one
-// v_cvt_f16_f32 on the fp32 value. A plain (_Float16) conversion lets the
-// compiler fuse it with the fmaf that produced the value (v_fma_mixlo_f16
-// rounds the exact result once, straight to fp16), which differs from the
-// reference's fp32 result rounded to fp16 whenever that result lies exactly
-// halfway between two fp16 values; the asm keeps the conversion on its own.
-// It equals the integer rounding (sign, rebiased exponent, 13 dropped
-// mantissa bits rounded half to even, subnormals below 2^-14, overflow from
-// 65520 on) for all 2^32 inputs, checked exhaustively on the device.
-__device__ __forceinline__ uint16_t f2h(float f) {
-    uint32_t h;
-    asm("v_cvt_f16_f32 %0, %1" : "=v"(h) : "v"(f));
-    return (uint16_t)h;
-}
-
 // s_waitcnt lgkmcnt(0) alone. A batch of 16 LDS reads issued behind another
 // 16 exceeds what the 4-bit lgkm counter can tell apart, so the compiler's
 // own wait before the first batch's use would also wait for most of the

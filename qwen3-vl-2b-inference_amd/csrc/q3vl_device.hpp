@@ -17,6 +17,26 @@
 
 namespace q3vl {
 
+Q3VL_INLINE float h2f(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+// fp32 -> fp16 bits, round to nearest even (NaN -> sign | 0x7E00), as one
+// v_cvt_f16_f32 on the fp32 value. A plain (_Float16) conversion lets the
+// compiler fuse it with the fmaf that produced the value (v_fma_mixlo_f16
+// rounds the exact result once, straight to fp16), which differs from the
+// reference's fp32 result rounded to fp16 whenever that result lies exactly
+// halfway between two fp16 values; the asm keeps the conversion on its own.
+// It equals the integer rounding (sign, rebiased exponent, 13 dropped
+// mantissa bits rounded half to even, subnormals below 2^-14, overflow from
+// 65520 on) for all 2^32 inputs, checked exhaustively on the device.
+Q3VL_INLINE uint16_t f2h(float f) {
+    uint32_t h;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm("v_cvt_f16_f32 %0, %1" : "=v"(h) : "v"(f));
+#else
+    h = 0;
+#endif
+    return (uint16_t)h;
+}
+
 // Fixed fp32 reduction tree of add_reduce_mm_256 (simd_utils.hpp:5-19):
 // ((v0+v4)+(v1+v5)) + ((v2+v6)+(v3+v7)).
 Q3VL_INLINE float tree8(float v0, float v1, float v2, float v3, float v4,

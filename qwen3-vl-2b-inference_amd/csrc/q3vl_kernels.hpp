@@ -186,4 +186,61 @@ int gemm_wide_parts(int N, int cus);
 hipError_t launch_gemm_wide(const float *A, const int8_t *W, const float *S, float *C, int M, int N, int K, int gs,
                             float *part_val, int32_t *part_idx, int cus, hipStream_t st);
 
+// ------------------------------------------- rows of tokens over the caches
+constexpr int kDraftRows = 1024;  // most rows of one sequence that a plan's LDS holds
+hipError_t launch_draft_plan(const int32_t *parents, const int32_t *row_start, const int32_t *cache_len,
+                             const int32_t *pos_delta, int batch, int rows, int max_rows, int max_seq, uint64_t *mask,
+                             int words, int32_t *pos, int64_t *slots, hipStream_t st);
+
+struct QkRopeArgs {
+    const float *q, *k, *v;
+    int64_t ldq, ldk, ldv;
+    void *q_out;
+    int64_t ldo, rows;
+    const int64_t *slots;
+    const int32_t *pos;
+    const int8_t *q_w, *k_w;
+    const float *q_s, *k_s;
+    const float *cos, *sin;
+    uint16_t *k_cache, *v_cache;
+    size_t seq_stride, head_stride, row_stride;
+    int heads, kv_heads, batch, max_seq, gs, table_rows;
+    int sec0, sec1, sec2, interleaved;
+    float eps;
+};
+hipError_t launch_qk_norm_rope(const QkRopeArgs &a, int head_dim, bool half, int axes, hipStream_t st);
+
+struct TreeAttnArgs {
+    const void *q;
+    void *out;
+    int64_t ldq, ldo;
+    const uint16_t *k_cache, *v_cache;
+    size_t seq_stride, head_stride, row_stride;
+    const int32_t *row_start, *cache_len;
+    const uint64_t *mask;  // [rows, words], or null: a chain
+    float *part_o;         // splits > 1: [rows * heads][splits][head_dim]
+    float *part_ml;        //             [rows * heads][splits][2]
+    int rows, heads, kv_heads, batch, max_seq, max_rows, words, splits;
+    float scale_log2e;     // scale / ln 2
+};
+// Pieces a sequence's cache is split into.
+int tree_attention_splits(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len);
+hipError_t launch_tree_attention(const TreeAttnArgs &a, int head_dim, bool half, hipStream_t st);
+
+struct LogprobArgs {
+    const void *logits;
+    int64_t ld;
+    const int32_t *tokens;
+    int M, V, k, parts;
+    float *part;     // [M][parts][4]: maximum, sum of the rest, weighted sum, values ahead
+    float *sub_max;  // [M][logprob_subs(V)]
+    float *logprob, *entropy, *top_logprobs;
+    int32_t *rank, *top_ids;
+};
+constexpr int kLogprobTop = 64;     // most alternatives
+constexpr int kLogprobParts = 256;  // most parts of a row
+int logprob_subs(int V);
+int logprob_parts(int M, int V);
+hipError_t launch_token_logprobs(const LogprobArgs &a, bool half, hipStream_t st);
+
 }  // namespace q3vl

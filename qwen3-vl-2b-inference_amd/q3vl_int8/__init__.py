@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+from typing import NamedTuple
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libq3vl_int8.so")
@@ -60,6 +61,8 @@ def _declare(lib):
         "q3vl_weight_release": (i, [_vp]),
         "q3vl_weight_release_all": (i, []),
         "q3vl_quantize_groupwise": (i, [_vp, _sz, _sz, _vp, _vp, _vp]),
+        "q3vl_token_logprobs_workspace_bytes": (_sz, [_sz, _sz]),
+        "q3vl_token_logprobs": (i, [_vp, _sz, i, _vp, _sz, _sz, i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -282,6 +285,43 @@ def argmax_rows(logits, ids=None, workspace=None, stream=None):
     wp, wb = _ws(workspace)
     _check(lib().q3vl_argmax_rows(_ptr(logits), _ptr(ids), M, V, wp, wb, _stream(stream)))
     return ids
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: object       # fp32 [M]
+    rank: object          # int32 [M]
+    entropy: object       # fp32 [M]
+    top_ids: object       # int32 [M, top_k]
+    top_logprobs: object  # fp32 [M, top_k]
+
+
+def alloc_token_logprobs_workspace(M, V, device="cuda"):
+    """Device workspace for token_logprobs over [M, V] logits."""
+    torch = _torch()
+    return torch.empty(max(256, lib().q3vl_token_logprobs_workspace_bytes(M, V)), dtype=torch.uint8, device=device)
+
+
+def token_logprobs(logits, tokens, top_k=0, workspace=None, stream=None):
+    """Log probability, rank and the row's entropy for tokens int32 [M], and
+    the top_k best alternatives, from logits [M, V] (fp32 or fp16, rows may be
+    views of wider ones): a TokenLogprobs. Larger values come first, equal ones
+    by index; a token outside of [0, V) gives NaN and rank -1."""
+    torch = _torch()
+    from .attention import _empty, _rows, _vec
+    ld = _rows(logits, (torch.float32, torch.float16), "logits")
+    M, V = logits.shape
+    _vec(tokens, torch.int32, M, "tokens")
+    k = max(int(top_k), 0)
+    f = _empty((2, M), torch.float32, logits, stream)
+    rank = _empty((M,), torch.int32, logits, stream)
+    ids = _empty((M, k), torch.int32, logits, stream)
+    top = _empty((M, k), torch.float32, logits, stream)
+    lp, ent = f[0], f[1]
+    wp, wb = _ws(workspace)
+    _check(lib().q3vl_token_logprobs(logits.data_ptr(), ld, FP16 if logits.dtype is torch.float16 else FP32, tokens.data_ptr(),
+                                     M, V, top_k, lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(),
+                                     wp, wb, _stream(stream)))
+    return TokenLogprobs(lp, rank, ent, ids, top)
 
 
 def swiglu(gate, up, stream=None):

@@ -109,32 +109,539 @@ template <bool HALF> __device__ __forceinline__ void put(void *out, int64_t at, 
 
 }  // namespace
 
-int tree_attention_splits(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len) { return 1; }
+// ------------------------------------------------------------ the kernel
+// Scores transposed, S^T = K Q^T, by v_mfma_f32_16x16x32_f16: a lane then holds
+// four keys of one query row (column i = lane & 15, keys 4 g + e with g = lane
+// >> 4), so a row's running maximum, its bias and its sum stay in the lane, and
+// only the maximum of a step crosses lanes. The same registers, two 16-key
+// tiles side by side, are the B operand of O^T += V^T P^T: operand slot (g, e)
+// holds key 4 g + e of the first tile, slot (g, 4 + e) of the second, and V^T is
+// read in that order by the transposing LDS read. O^T's column is the same
+// query row, so its rescaling needs no exchange either.
+//
+// Query row r of a (sequence, kv head): token r / group, head r % group of the
+// group of query heads that share the kv head.
+//
+// K and V go to LDS by loads with an LDS destination (no registers, any number
+// in flight), 16-byte pieces swizzled by the row so that both reads spread over
+// the banks. Rows past the end read as zeros by the buffer's bounds.
+//
+// Two forms. Few rows (at most 64 of a kv head's): each wave walks its own 32
+// keys of every 128 with all rows, in a private ring of two stages, no barrier;
+// the four waves' results are joined in LDS at the end. That keeps 96 KB of
+// reads in flight a CU, which is what bounds it. Many rows: a wave has 32 rows
+// of its own, the block shares 64-key tiles in two buffers, one barrier a tile.
+//
+// fp32 queries are two fp16 terms, hi + lo, relative to the row's largest value
+// (a power of two, undone in the score's factor sc), and so are their
+// probabilities; products of fp16 are exact in fp32, so the scores keep 2^-21 of
+// sum |q k|. fp16 queries and their probabilities are one term each: half a
+// step of fp16 in each p, as the output's own rounding.
+//
+// With M the running maximum of a row's raw scores, p = 2^(s sc - bias') held as
+// 2^(s sc + bias), bias = 14 - M sc: probabilities up to 2^14 use fp16's range,
+// 2^-28 of the largest is still a normal number. A row's results are its sum O
+// and l with weights 2^(-bias).
+//
+// What no row sees never enters: rows past the end are zeros, scores of unseen
+// keys are replaced by -inf before the maximum. An unseen V row of another
+// row's draft can still hold an infinity or NaN, and 0 times it is NaN: a row
+// whose O or l is not finite is done again by row_attention; so is one whose
+// scores pass 2^23, where the rounding of M sc alone moves 2^14 by bits.
+template <int D, int NR, bool SHARED> struct Tile {
+    static constexpr int RB = 2 * D;             // bytes of a cached row
+    static constexpr int RI = D / 32;            // loads of 1 KiB for 16 rows
+    static constexpr int NS = SHARED ? 2 : 256 / D;
+    static constexpr int STAGE = (SHARED ? 64 : 32) * RB * 2;  // K, then V
+    static constexpr int RING = (SHARED ? 1 : WAVES) * NS * STAGE;
+    static constexpr int BM = 16 * NR * (SHARED ? WAVES : 1);  // query rows of a block
+    static constexpr int OS = D + 4;             // floats of a joined row (spread over the banks)
+    static constexpr int JOIN = SHARED ? 0 : WAVES * BM * OS * 4;
+    static constexpr int ML = RING > JOIN ? RING : JOIN;       // (M, l) of each wave's rows
+    static constexpr int FLAG = ML + (SHARED ? 0 : WAVES * BM * 8);
+    static constexpr int LDS = FLAG + (BM + 1) * 4;
+    static constexpr int UNIT = SHARED ? 64 : 32 * WAVES;      // keys of a turn
+    static_assert(LDS <= 160 * 1024 && sizeof(RowScratch) <= (size_t)RING, "LDS");
+};
 
-template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_attention_kernel(TreeAttnArgs a) {
-    __shared__ RowScratch sh;
-    const int head = blockIdx.x % a.heads, bt = blockIdx.x / a.heads;
-    const int b = bt / a.max_rows, t = bt - b * a.max_rows;
+typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ half4_t read_transposed(unsigned char *p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) fp16x4 *)p));
+#else
+    return half4_t{};
+#endif
+}
+
+// Largest value of the four lanes i, i + 16, i + 32, i + 48, in each of them.
+__device__ __forceinline__ float column_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// 32 bits of a row's mask line from bit i on (i may be negative: positions
+// before the drafts, all seen); n rows exist.
+__device__ __forceinline__ uint32_t mask_window(const uint64_t *line, int words, int n, int i) {
+    const int at = max(i, 0), w = at >> 6, sh = at & 63;
+    uint64_t v = w < words ? line[w] >> sh : 0;
+    if (sh && w + 1 < words) v |= line[w + 1] << (64 - sh);
+    const int left = n - at;
+    if (left < 64) v &= left > 0 ? (1ull << left) - 1 : 0;
+    if (i <= -32) return 0xFFFFFFFFu;
+    return i < 0 ? (uint32_t)(v << -i) | ((1u << -i) - 1) : (uint32_t)v;
+}
+
+template <int D, bool HALF, int NR, bool SHARED>
+__global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a, int tiles) {
+    using T = Tile<D, NR, SHARED>;
+    constexpr int KS = D / 32, NT = D / 16, NQ = HALF ? 1 : 2;
+    extern __shared__ __align__(16) unsigned char smem[];
+    // (loads with an LDS destination take its offset: 0, as the kernel has no other LDS)
+    const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
+    int x = blockIdx.x;  // kv head, split, tile (the last rows, which see most, first), sequence
+    const int h = x % a.kv_heads;
+    x /= a.kv_heads;
+    const int split = x % a.splits;
+    x /= a.splits;
+    const int tile = tiles - 1 - x % tiles, b = x / tiles;
+    const Seq s = sequence(a, b);
+    const int group = a.heads / a.kv_heads;
+    const int n = min(s.n, a.max_rows), nrows = n * group, r0 = tile * T::BM;
+    if (r0 >= nrows) return;
+
+    int row[NR], tok[NR], head[NR];  // of column i: its row, token, query head
+    bool live[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        row[nr] = r0 + (SHARED ? wid * 16 * NR : 0) + nr * 16 + i;
+        live[nr] = row[nr] < nrows;
+        tok[nr] = live[nr] ? row[nr] / group : 0;
+        head[nr] = h * group + (live[nr] ? row[nr] - tok[nr] * group : 0);
+    }
+    if (!s.ok) {
+        if (a.splits == 1)
+            for (int e = tid; e < min(T::BM, nrows - r0) * D; e += THREADS) {
+                const int r = r0 + e / D, t = r / group;
+                put<HALF>(a.out, (int64_t)(s.start + t) * a.ldo + (int64_t)(h * group + r - t * group) * D + e % D, __builtin_nanf(""));
+            }
+        return;
+    }
+
+    // ---- this block's positions: units of T::UNIT keys, a chain's up to the
+    // last one that the tile's rows see
+    const int last_tok = min((r0 + T::BM - 1) / group, n - 1);
+    const int total = s.len + (a.mask ? s.n : last_tok + 1);
+    const int units = (total + T::UNIT - 1) / T::UNIT;
+    const int u0 = (int)((int64_t)units * split / a.splits), u1 = (int)((int64_t)units * (split + 1) / a.splits);
+    const int j0 = u0 * T::UNIT, j1 = min(u1 * T::UNIT, total);
+
+    // ---- queries: operand registers, the score's factor
+    half8_t qf[NR][NQ][KS];
+    float sc[NR];
+    const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        const int64_t at = (int64_t)(s.start + tok[nr]) * a.ldq + (int64_t)head[nr] * D + 8 * g;
+        sc[nr] = sign == 0.0f ? 1.0f : fabsf(a.scale_log2e);
+        if constexpr (HALF) {
+            const _Float16 *p = static_cast<const _Float16 *>(a.q) + at;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[nr][0][ks][e] = live[nr] ? (_Float16)(p[32 * ks + e] * (_Float16)sign) : (_Float16)0.0f;
+        } else {
+            const float *p = static_cast<const float *>(a.q) + at;
+            float v[KS][8], top = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[ks][e] = live[nr] ? p[32 * ks + e] * sign : 0.0f;
+                    top = fmaxf(top, fabsf(v[ks][e]));
+                }
+            top = column_max(top);
+            // the largest value to [2^13, 2^14)
+            const int shift = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+            sc[nr] = ldexpf(sc[nr], -shift);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = ldexpf(v[ks][e], shift);
+                    qf[nr][0][ks][e] = (_Float16)y;
+                    qf[nr][1][ks][e] = (_Float16)(y - (float)qf[nr][0][ks][e]);
+                }
+        }
+    }
+
+    // ---- loads: lane's place in 16 rows of the cache, and of LDS
+    const size_t head_at = (size_t)b * a.seq_stride + (size_t)h * a.head_stride;
+    const int rsb = (int)(a.row_stride * 2);
+    constexpr int NL = (SHARED ? 1 : 2) * T::RI;  // loads of a K or V part
+    int voff[NL];
+#pragma unroll
+    for (int t = 0; t < NL; ++t) {
+        const int r = (t * 64 + lane) / (D / 8), c = lane % (D / 8);
+        voff[t] = (r + (SHARED ? wid * 16 : 0)) * rsb + (c ^ (D == 128 ? r & 15 : r >> 1 & 7)) * 16;
+    }
+    auto resource = [&](const uint16_t *c, int j, int most) {
+        const int left = min(j1 - j, most);
+        return make_rsrc(c + head_at + (size_t)j * a.row_stride, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
+    };
+    // rows from j on: 32 to this wave's own stage, or its 16 of a block's 64
+    auto load = [&](const uint16_t *c, int j, int lds) {
+        const rsrc_t r = resource(c, j, SHARED ? 64 : 32);
+#pragma unroll
+        for (int t = 0; t < NL; ++t) dma16(r, voff[t], 0, lds + ((SHARED ? wid * NL : 0) + t) * 1024);
+    };
+
+    // ---- one step: 32 keys from position j, K and V rows at LDS offsets
+    int kaddr[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kaddr[ks] = i * T::RB + ((ks * 4 + g) ^ (D == 128 ? i : i >> 1)) * 16;
+    const int vr = 4 * g + (i >> 2);  // row of a 16-key tile this lane's transposing read starts from
+    const int vaddr = vr * T::RB + (((i & 3) >> 1) ^ (D == 128 ? vr : vr >> 1 & 7)) * 16 + (i & 1) * 8;
+    float M[NR], bias[NR], l[NR];
+    float4_t O[NT][NR];
+    bool any[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        M[nr] = -INFINITY;
+        bias[nr] = l[nr] = 0.0f;
+        any[nr] = false;
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt) O[dt][nr] = float4_t{0, 0, 0, 0};
+    }
+    float4_t S[2][NR];
+    auto scores = [&](int klds) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) S[kb][nr] = float4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const half8_t kf = *reinterpret_cast<const half8_t *>(smem + klds + kaddr[ks] + kb * 16 * T::RB);
+#pragma unroll
+                for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr)
+                        S[kb][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[nr][q][ks], S[kb][nr], 0, 0, 0);
+            }
+        }
+    };
+    half8_t P[NR][NQ];
+    auto softmax = [&](int j) {
+        if (j + 32 > min(s.len, j1)) {  // some keys are not for every row
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                uint32_t w;
+                if (a.mask) {
+                    w = mask_window(a.mask + (size_t)(s.start + tok[nr]) * a.words, a.words, s.n, j - s.len);
+                } else {
+                    const int left = s.len + tok[nr] + 1 - j;
+                    w = left >= 32 ? 0xFFFFFFFFu : left > 0 ? (1u << left) - 1 : 0;
+                }
+                if (j1 - j < 32) w &= j1 > j ? (1u << (j1 - j)) - 1 : 0;
+                any[nr] = any[nr] || w;
+                w >>= 4 * g;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(w >> (16 * kb + e) & 1)) S[kb][nr][e] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) any[nr] = true;
+        }
+        float top[NR];
+        bool grow = false;
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            float t = S[0][nr][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) t = fmaxf(t, S[e >> 2][nr][e & 3]);
+            top[nr] = column_max(t);
+            grow = grow || top[nr] > M[nr];
+        }
+        if (__any(grow)) {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                const float m = fmaxf(M[nr], top[nr]);
+                const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], 14.0f);
+                const float f = M[nr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(nb - bias[nr]);
+                M[nr] = m;
+                bias[nr] = nb;
+                l[nr] *= f;
+#pragma unroll
+                for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= f;
+            }
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(S[e >> 2][nr][e & 3], sc[nr], bias[nr]));
+            l[nr] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                P[nr][0][e] = (_Float16)p[e];
+                if constexpr (!HALF) P[nr][1][e] = (_Float16)(p[e] - (float)P[nr][0][e]);
+            }
+        }
+    };
+    auto values = [&](int vlds) {
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt) {
+            const half4_t lo = read_transposed(smem + vlds + (vaddr ^ (dt * 32)));
+            const half4_t hi = read_transposed(smem + vlds + (vaddr ^ (dt * 32)) + 16 * T::RB);
+            const half8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr)
+                    O[dt][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, P[nr][q], O[dt][nr], 0, 0, 0);
+        }
+    };
+
+    if constexpr (SHARED) {
+        auto load_tile = [&](int u) {
+            const int lds = (u & 1) * T::STAGE;
+            load(a.k_cache, u * 64, lds);
+            load(a.v_cache, u * 64, lds + 64 * T::RB);
+        };
+        if (u0 < u1) load_tile(u0);
+        for (int u = u0; u < u1; ++u) {
+            dma_wait<0>();
+            lds_barrier();  // the tile is there, and every wave is done with the other buffer
+            if (u + 1 < u1) load_tile(u + 1);
+            const int lds = (u & 1) * T::STAGE;
+#pragma unroll 1
+            for (int k = 0; k < 2; ++k) {
+                scores(lds + k * 32 * T::RB);
+                softmax(u * 64 + k * 32);
+                values(lds + 64 * T::RB + k * 32 * T::RB);
+            }
+        }
+    } else {
+        // loads younger than the K or V part waited for
+        constexpr int YOUNGER = NL + (T::NS - 1) * 2 * NL;
+        const int mine = wid * T::NS * T::STAGE;
+        const int jw = j0 + wid * 32;
+        if (u0 < u1) {
+#pragma unroll
+            for (int k = 0; k < T::NS; ++k) {
+                load(a.k_cache, jw + k * T::UNIT, mine + k * T::STAGE);
+                load(a.v_cache, jw + k * T::UNIT, mine + k * T::STAGE + 32 * T::RB);
+            }
+        }
+        int lds = mine;
+        for (int u = u0, j = jw; u < u1; ++u, j += T::UNIT) {
+            dma_wait<YOUNGER>();
+            scores(lds);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the slot is refilled
+            load(a.k_cache, j + T::NS * T::UNIT, lds);
+            softmax(j);
+            dma_wait<YOUNGER>();
+            values(lds + 32 * T::RB);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load(a.v_cache, j + T::NS * T::UNIT, lds + 32 * T::RB);
+            lds += T::STAGE;
+            if (lds == mine + T::NS * T::STAGE) lds = mine;
+        }
+    }
+    dma_wait<0>();
+    lds_barrier();  // the ring is free
+
+    // ---- results: whole rows, what is not finite again
+    int *flag = reinterpret_cast<int *>(smem + T::FLAG);
+    for (int e = tid; e <= T::BM; e += THREADS) flag[e] = 0;
+    lds_barrier();
+    bool redo[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        l[nr] = column_sum(l[nr]);
+        float z = l[nr] * 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z = fmaf(O[dt][nr][e], 0.0f, z);
+        // (the largest score's p is 2^14 if its product with sc rounds to within a bit)
+        redo[nr] = live[nr] && (z != 0.0f || (any[nr] && !(l[nr] >= 8192.0f)));
+        if (redo[nr]) flag[row[nr] - r0] = flag[T::BM] = 1;
+    }
+    auto emit = [&](int t, int hd, int d, float4_t o, float m, float lsum) {
+        const int64_t r = s.start + t;
+        if (a.splits == 1) {
+            const float inv = m == -INFINITY ? 0.0f : 1.0f / lsum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) put<HALF>(a.out, r * a.ldo + (int64_t)hd * D + d + e, o[e] * inv);
+        } else {
+            const int64_t part = (r * a.heads + hd) * a.splits + split;
+            *reinterpret_cast<float4_t *>(a.part_o + part * D + d) = o;
+            if (d == 0) {
+                a.part_ml[part * 2] = m;
+                a.part_ml[part * 2 + 1] = lsum;
+            }
+        }
+    };
+    if constexpr (SHARED) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+            if (live[nr] && !flag[row[nr] - r0])
+#pragma unroll
+                for (int dt = 0; dt < NT; ++dt)
+                    emit(tok[nr], head[nr], dt * 16 + 4 * g, O[dt][nr], M[nr] == -INFINITY ? -INFINITY : -bias[nr], l[nr]);
+        lds_barrier();
+    } else {
+        float *join = reinterpret_cast<float *>(smem);
+        float *ml = reinterpret_cast<float *>(smem + T::ML);
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            const int at = wid * T::BM + nr * 16 + i;
+#pragma unroll
+            for (int dt = 0; dt < NT; ++dt) *reinterpret_cast<float4_t *>(join + at * T::OS + dt * 16 + 4 * g) = O[dt][nr];
+            if (g == 0) {
+                ml[at * 2] = M[nr] == -INFINITY ? -INFINITY : -bias[nr];
+                ml[at * 2 + 1] = l[nr];
+            }
+        }
+        lds_barrier();
+        for (int e = tid; e < T::BM * (D / 4); e += THREADS) {
+            const int k = e / (D / 4), d = e % (D / 4) * 4, r = r0 + k;
+            if (r >= nrows || flag[k]) continue;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[(w * T::BM + k) * 2]);
+            float4_t o = {0, 0, 0, 0};
+            float lsum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float mw = ml[(w * T::BM + k) * 2];
+                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+                lsum = fmaf(ml[(w * T::BM + k) * 2 + 1], f, lsum);
+                o += *reinterpret_cast<const float4_t *>(join + (w * T::BM + k) * T::OS + d) * f;
+            }
+            const int t = r / group;
+            emit(t, h * group + r - t * group, d, o, m, lsum);
+        }
+        lds_barrier();
+    }
+    if (!flag[T::BM]) return;
+    RowScratch &sh = *reinterpret_cast<RowScratch *>(smem);
+    for (int k = 0; k < T::BM; ++k) {
+        if (!flag[k]) continue;  // (uniform)
+        const int t = (r0 + k) / group, hd = h * group + r0 + k - t * group;
+        float o, m, lsum;
+        row_attention<D, HALF>(a, s, b, t, hd, j0, j1, sh, o, m, lsum);
+        if (tid < D) {
+            const int64_t r = s.start + t;
+            if (a.splits == 1) {
+                put<HALF>(a.out, r * a.ldo + (int64_t)hd * D + tid, m == -INFINITY ? 0.0f : o / lsum);
+            } else {
+                const int64_t part = (r * a.heads + hd) * a.splits + split;
+                a.part_o[part * D + tid] = o;
+                if (tid == 0) {
+                    a.part_ml[part * 2] = m;
+                    a.part_ml[part * 2 + 1] = lsum;
+                }
+            }
+        }
+    }
+}
+
+// Joins a row's splits: one wave a (row, query head).
+template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeAttnArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int x = blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const int hd = x % a.heads, bt = x / a.heads, t = bt % a.max_rows, b = bt / a.max_rows;
+    if (b >= a.batch) return;
     const Seq s = sequence(a, b);
     if (t >= s.n) return;
-    float o = __builtin_nanf(""), m, l;
+    const int64_t r = s.start + t, part = (r * a.heads + hd) * a.splits;
+    float o[D / 64];
+    for (int e = 0; e < D / 64; ++e) o[e] = __builtin_nanf("");
     if (s.ok) {
-        row_attention<D, HALF>(a, s, b, t, head, 0, s.len + s.n, sh, o, m, l);
-        o = m == -INFINITY ? 0.0f : o / l;
+        const float m = lane < a.splits ? a.part_ml[(part + lane) * 2] : -INFINITY;
+        float lw = lane < a.splits ? a.part_ml[(part + lane) * 2 + 1] : 0.0f;
+        float top = m;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        lw = m == -INFINITY ? 0.0f : lw * f;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) lw += __shfl_xor(lw, k);
+        for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
+        for (int k = 0; k < a.splits; ++k) {
+            const float mk = __shfl(m, k), fk = __shfl(f, k);
+            if (mk == -INFINITY) continue;  // nothing seen there
+            for (int e = 0; e < D / 64; ++e) o[e] = fmaf(a.part_o[(part + k) * D + e * 64 + lane], fk, o[e]);
+        }
+        for (int e = 0; e < D / 64; ++e) o[e] = top == -INFINITY ? 0.0f : o[e] / lw;
     }
-    if (threadIdx.x < D) put<HALF>(a.out, (int64_t)(s.start + t) * a.ldo + (int64_t)head * D + threadIdx.x, o);
+    for (int e = 0; e < D / 64; ++e) put<HALF>(a.out, r * a.ldo + (int64_t)hd * D + e * 64 + lane, o[e]);
+}
+
+namespace {
+
+constexpr int kSplits = 64;  // most, a lane of the joining wave each
+
+// Rows of a block: 16 or 32 with their own keys a wave, 64 or 128 with shared tiles.
+int block_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+
+}  // namespace
+
+// Blocks and splits. A launch has 2^24 blocks of 256 threads at most.
+int tree_attention_splits(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len) {
+    const int64_t kv_rows = (int64_t)max_rows * (heads / kv_heads);
+    const int bm = block_rows(kv_rows);
+    const int64_t tiles = (kv_rows + bm - 1) / bm, base = tiles * batch * kv_heads;
+    if (base > (1 << 24) - 1 || (int64_t)batch * max_rows > (int64_t)((1 << 24) - 1) * WAVES / heads) return -1;
+    if (base == 0) return 1;
+    const int64_t want = (512 + base - 1) / base;
+    const int64_t most = ((int64_t)max_len + 255) / 256;  // 256 positions a split at least
+    int64_t k = want < most ? want : most;
+    k = k < 1 ? 1 : k > kSplits ? kSplits : k;
+    return base * k > (1 << 24) - 1 ? 1 : (int)k;
+}
+
+template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, hipStream_t st) {
+    const int64_t kv_rows = (int64_t)a.max_rows * (a.heads / a.kv_heads);
+    const int bm = block_rows(kv_rows);
+    const int tiles = (int)((kv_rows + bm - 1) / bm);
+    const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
+    auto go = [&](auto kernel, int lds) {
+        if (lds > 64 * 1024) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+            if (e != hipSuccess) return e;
+        }
+        kernel<<<grid, THREADS, lds, st>>>(a, tiles);
+        return hipGetLastError();
+    };
+    hipError_t e;
+    if (bm == 16) e = go(tree_attention_kernel<D, HALF, 1, false>, Tile<D, 1, false>::LDS);
+    else if (bm == 32) e = go(tree_attention_kernel<D, HALF, 2, false>, Tile<D, 2, false>::LDS);
+    else if (bm == 64) e = go(tree_attention_kernel<D, HALF, 1, true>, Tile<D, 1, true>::LDS);
+    else e = go(tree_attention_kernel<D, HALF, 2, true>, Tile<D, 2, true>::LDS);
+    if (e != hipSuccess || a.splits == 1) return e;
+    const unsigned waves = (unsigned)a.batch * a.max_rows * a.heads;
+    tree_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(a);
+    return hipGetLastError();
 }
 
 hipError_t launch_tree_attention(const TreeAttnArgs &a, int head_dim, bool half, hipStream_t st) {
-    const unsigned grid = (unsigned)a.batch * (unsigned)a.max_rows * (unsigned)a.heads;
-    if (head_dim == 128) {
-        if (half) tree_attention_kernel<128, true><<<grid, THREADS, 0, st>>>(a);
-        else tree_attention_kernel<128, false><<<grid, THREADS, 0, st>>>(a);
-    } else {
-        if (half) tree_attention_kernel<64, true><<<grid, THREADS, 0, st>>>(a);
-        else tree_attention_kernel<64, false><<<grid, THREADS, 0, st>>>(a);
-    }
-    return hipGetLastError();
+    if (head_dim == 128) return half ? launch_d<128, true>(a, st) : launch_d<128, false>(a, st);
+    return half ? launch_d<64, true>(a, st) : launch_d<64, false>(a, st);
 }
 
 }  // namespace q3vl

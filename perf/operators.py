@@ -216,7 +216,7 @@ def _make(case, seed):
 def prepare(case, seed):
     st = _make(case, seed)
     if own:
-        qa, q = _framework()
+        qa, q = st["lib"] = _framework()
         kind = st["kind"]
         if kind == "rope":
             st["cache"] = qa.KVCache(st["kc"], st["vc"])
@@ -246,7 +246,7 @@ def run(st):
 
 
 def _run_own(st):
-    qa, q = _framework()
+    qa, q = st["lib"]
     kind = st["kind"]
     if kind == "plan":
         mask, pos, slots = qa.draft_plan(st["parents"], st["row_start"], st["cache_len"], st["max_seq"], st["max_rows"], pos_delta=st["delta"])

@@ -12,20 +12,41 @@
 // The k best values lie in the k sub-chunks whose maxima come first (larger
 // first, equal ones by place): each of k others ahead of a sub-chunk has a
 // value ahead of all of its own. The second kernel picks those sub-chunks and
-// reads them again, k of V / 256, instead of every block keeping a list.
+// reads them again, k of V / 512, instead of every block keeping a list.
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
+#include "q3vl_mfma.hpp"
 
 namespace q3vl {
 
 namespace {
 
-constexpr int SUB = 256;          // values of a sub-chunk
-constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int SUB = 512;                             // values of a sub-chunk
+constexpr int THREADS = 256, WAVES = THREADS / 64;   // of the scan
+constexpr int FIN_WAVES = 8;                         // of the second kernel, with alternatives
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float FAR = -300.0f;    // exponent (base 2) from which 2^x is 0 in fp32
 
-typedef uint32_t lp_u32x4 __attribute__((ext_vector_type(4)));
+// v_max_f32 and v_min_f32 as they are, for operands that are no NaN: no
+// instruction goes to quieting one first.
+__device__ __forceinline__ float vmax(float a, float b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+#else
+    return a > b ? a : b;
+#endif
+}
+__device__ __forceinline__ float vmin(float a, float b) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    float r;
+    asm("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+#else
+    return a < b ? a : b;
+#endif
+}
 
 // (maximum, sum of the rest, weighted sum in base 2) of some values
 struct Sums {
@@ -39,23 +60,36 @@ __device__ __forceinline__ float weight(float lo, float m, float &arg) {
     return __builtin_amdgcn_exp2f(arg);
 }
 
-__device__ __forceinline__ Sums join(Sums a, Sums b) {
-    Sums o;
-    o.m = fmaxf(a.m, b.m);
-    const float ref = fmaxf(o.m, -FLT_MAX);
-    float ea, eb;
-    const float wa = weight(a.m, ref, ea), wb = weight(b.m, ref, eb);
-    // one of the two maxima stays out of the sum; the other enters it
-    const bool a_top = a.m >= b.m;
-    o.r = (a.r * wa + b.r * wb) + (a_top ? wb : wa);
-    o.t = (fmaf(a.r, ea, a.t) * wa + fmaf(b.r, eb, b.t) * wb) + (a_top ? wb * eb : wa * ea);
-    return o;
+__device__ __forceinline__ float lane_swap_max(float v) {
+    v = row16_max(v);
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = vmax(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return vmax(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float lane_swap_sum(float v) {
+    v += dpp_f(v, dpp_xor1);
+    v += dpp_f(v, dpp_xor2);
+    v += dpp_f(v, dpp_half_mirror);
+    v += dpp_f(v, dpp_mirror);
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The 64 lanes' sums as one, in every lane: each scaled to the common maximum;
+// every lane's own maximum enters r but one that is the common one.
 __device__ __forceinline__ Sums wave_join(Sums s) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) s = join(s, Sums{__shfl_xor(s.m, o), __shfl_xor(s.r, o), __shfl_xor(s.t, o)});
-    return s;
+    Sums o;
+    o.m = lane_swap_max(s.m);
+    const uint64_t top = __ballot(s.m == o.m);
+    float arg;
+    const float w = weight(s.m, fmaxf(o.m, -FLT_MAX), arg);
+    const bool out = __lane_id() == (uint32_t)__builtin_ctzll(top | 1ull << 63);
+    o.r = lane_swap_sum(fmaf(s.r, w, out ? 0.0f : w));
+    o.t = lane_swap_sum(fmaf(fmaf(s.r, arg, s.t), w, out ? 0.0f : w * arg));
+    return o;
 }
 
 // A value's place in the order: larger floats first, -0 as 0, NaN as -inf.
@@ -81,65 +115,185 @@ __device__ __forceinline__ bool ahead(float x, int i, float xt, int t) { return 
 
 }  // namespace
 
-int logprob_subs(int V) { return (V + SUB - 1) / SUB; }
+// Sub-chunks lie on 16-byte boundaries, so a row may touch one more than its size asks for.
+int logprob_subs(int V) { return (V + 7 + SUB - 1) / SUB; }
 
+// Blocks a row: four a CU over all rows, a wave of each with two sub-chunks at least.
 int logprob_parts(int M, int V) {
-    const int subs = logprob_subs(V), most = (subs + WAVES - 1) / WAVES;
-    const int want = (2048 + M - 1) / M;
+    const int most = (logprob_subs(V) + 2 * WAVES - 1) / (2 * WAVES), want = (1024 + M - 1) / M;
     const int p = want < most ? want : most;
     return p < 1 ? 1 : p < kLogprobParts ? p : kLogprobParts;
 }
 
+// A lane's 16 bytes of a row, values [i, i + VEC), -inf outside of [0, V);
+// inside: the whole wave's piece lies in the row.
+template <bool HALF> __device__ __forceinline__ u32x4 read_piece(const void *x, int i, int V, bool inside) {
+    constexpr int VEC = HALF ? 8 : 4;
+    const unsigned char *p = static_cast<const unsigned char *>(x) + (int64_t)i * (HALF ? 2 : 4);
+    if (inside || (i >= 0 && i + VEC <= V)) return *reinterpret_cast<const u32x4 *>(p);
+    u32x4 r;
+    if constexpr (HALF) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int k = i + 2 * e;
+            const uint32_t lo = k >= 0 && k < V ? static_cast<const uint16_t *>(x)[k] : 0xFC00u;
+            const uint32_t hi = k + 1 >= 0 && k + 1 < V ? static_cast<const uint16_t *>(x)[k + 1] : 0xFC00u;
+            r[e] = lo | hi << 16;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[e] = i + e >= 0 && i + e < V ? static_cast<const uint32_t *>(x)[i + e] : 0xFF800000u;
+    }
+    return r;
+}
+template <bool HALF> __device__ __forceinline__ float piece_value(u32x4 r, int e) {
+    return HALF ? h2f((uint16_t)(r[e >> 1] >> (16 * (e & 1)))) : __uint_as_float(r[e & 3]);
+}
+
+// Values before the row's first 16-byte boundary counted back to it.
+template <bool HALF> __device__ __forceinline__ int row_offset(const void *x) {
+    return HALF ? (int)((uintptr_t)x / 2 % 8) : (int)((uintptr_t)x / 4 % 4);
+}
+
+// A wave takes two sub-chunks a turn, 16 values a lane. The largest of them and
+// of the lane's running maximum wins a tournament whose losers are exactly the
+// values that enter the sum: one more instruction a value than a maximum alone.
+// About 15 VALU instructions a value, 4 of them the exponential, against 10
+// bytes a clock that HBM has for a CU.
 template <bool HALF>
-__global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a) {
+__global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a, int subs_max) {
+    constexpr int VEC = HALF ? 8 : 4, U = 16 / VEC;  // values a load, loads a turn
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, tid = threadIdx.x, lane = tid & 63;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const void *x = HALF ? (const void *)(static_cast<const uint16_t *>(a.logits) + row * a.ld)
                          : (const void *)(static_cast<const float *>(a.logits) + row * a.ld);
-    const int subs = (a.V + SUB - 1) / SUB;
-    const int first = (int)((int64_t)subs * part / a.parts), last = (int)((int64_t)subs * (part + 1) / a.parts);
+    const int off = row_offset<HALF>(x);
+    const int turns = (a.V + off + 2 * SUB - 1) / (2 * SUB);
+    const int first = (int)((int64_t)turns * part / a.parts), last = (int)((int64_t)turns * (part + 1) / a.parts);
+    u32x4 raw[U];  // the turn's values, loaded a turn ahead
+    auto load = [&](int c) {
+        const int base = c * 2 * SUB - off;
+        const bool inside = base >= 0 && base + 2 * SUB <= a.V;
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = read_piece<HALF>(x, base + (u * 64 + lane) * VEC, a.V, inside);
+    };
+    if (first + wid < last) load(first + wid);
     const int t = a.tokens[row];
     const bool ok = t >= 0 && t < a.V;
     float xt = ok ? logit<HALF>(x, t) : 0.0f;
     if (!(xt > -INFINITY)) xt = -INFINITY;
     Sums s{-INFINITY, 0.0f, 0.0f};
+    float z = 0.0f;  // NaN once a NaN (or infinities of both signs) has been read
     int n = 0;
-    bool bad = false;
-    for (int c = first + (tid >> 6); c < last; c += WAVES) {
-        float best = -INFINITY;
+    for (int c = first + wid; c < last; c += WAVES) {
+        const int base = c * 2 * SUB - off;
+        float v[U][VEC];
 #pragma unroll
-        for (int u = 0; u < SUB / 64; ++u) {
-            const int i = c * SUB + u * 64 + lane;
-            if (i >= a.V) continue;
-            const float raw = logit<HALF>(x, i);
-            bad = bad || raw != raw;
-            const float v = raw > -INFINITY ? raw : -INFINITY;
-            n += ahead(v, i, xt, t);
-            best = fmaxf(best, v);
-            s = join(s, Sums{v, 0.0f, 0.0f});
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[u][e] = piece_value<HALF>(raw[u], e);
+        if (c + WAVES < last) load(c + WAVES);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) z = fmaf(v[u][e], 0x1p-64f, z);
+        if (__any(z != z)) {  // NaN as -inf (a signalling one would win the tournament)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[u][e] = v[u][e] > -INFINITY ? v[u][e] : -INFINITY;
+        }
+        // values ahead of the token: larger ones, and equal ones before it
+        if (xt > -INFINITY) {
+            if (base + 2 * SUB <= t) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) n += __builtin_popcountll(__ballot(v[u][e] >= xt));
+            } else if (base > t) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) n += __builtin_popcountll(__ballot(v[u][e] > xt));
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        n += __builtin_popcountll(__ballot(ahead(v[u][e], base + (u * 64 + lane) * VEC + e, xt, t)));
+            }
+        } else {  // everything above -inf, and what stands with it before the token
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const int i = base + (u * 64 + lane) * VEC + e;
+                    n += __builtin_popcountll(__ballot(i >= 0 && i < a.V && (v[u][e] > -INFINITY || i < t)));
+                }
+        }
+        float lose[16], win[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float p = v[2 * i / VEC][2 * i % VEC], q = v[2 * i / VEC][2 * i % VEC + 1];
+            win[i] = vmax(p, q);
+            lose[i] = vmin(p, q);
+        }
+        // (win: pairs in order, so halves of it are the turn's sub-chunks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lose[8 + i] = vmin(win[2 * i], win[2 * i + 1]);
+            win[i] = vmax(win[2 * i], win[2 * i + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            lose[12 + i] = vmin(win[2 * i], win[2 * i + 1]);
+            win[i] = vmax(win[2 * i], win[2 * i + 1]);
         }
         if (a.k) {
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) best = fmaxf(best, __shfl_xor(best, o));
-            if (lane == 0) a.sub_max[(size_t)row * subs + c] = best;
+            const float m0 = lane_swap_max(win[0]), m1 = lane_swap_max(win[1]);
+            if (lane < 2 && 2 * c + lane < subs_max) a.sub_max[(size_t)row * subs_max + 2 * c + lane] = lane ? m1 : m0;
         }
-    }
-    if (bad) s.r = __builtin_nanf("");
-    s = wave_join(s);
+        lose[14] = vmin(win[0], win[1]);
+        const float best = vmax(win[0], win[1]);
+        lose[15] = vmin(best, s.m);
+        const float m = vmax(best, s.m), ref = vmax(m, -FLT_MAX);
+        if (__any(best > s.m)) {
+            float arg;
+            const float w = weight(s.m, ref, arg);
+            s.t = fmaf(s.r, arg, s.t) * w;
+            s.r *= w;
+            s.m = m;
+        }
+        float r0 = 0.0f, r1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+        for (int i = 0; i < 16; i += 2) {
+            float arg;
+            float w = weight(lose[i], ref, arg);
+            r0 += w;
+            t0 = fmaf(w, arg, t0);
+            w = weight(lose[i + 1], ref, arg);
+            r1 += w;
+            t1 = fmaf(w, arg, t1);
+        }
+        s.r += r0 + r1;
+        s.t += t0 + t1;
+    }
+    if (z != z) s.r = z;
+    s = wave_join(s);
     __shared__ float sh[WAVES][4];
     if (lane == 0) {
-        sh[tid >> 6][0] = s.m;
-        sh[tid >> 6][1] = s.r;
-        sh[tid >> 6][2] = s.t;
-        sh[tid >> 6][3] = __int_as_float(n);
+        sh[wid][0] = s.m;
+        sh[wid][1] = s.r;
+        sh[wid][2] = s.t;
+        sh[wid][3] = __int_as_float(n);
     }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < WAVES; ++w) {
-            s = join(s, Sums{sh[w][0], sh[w][1], sh[w][2]});
-            n += __float_as_int(sh[w][3]);
-        }
+    if (tid >= 64) return;
+    const bool mine = lane < WAVES;
+    s = wave_join(Sums{mine ? sh[lane & 3][0] : -INFINITY, mine ? sh[lane & 3][1] : 0.0f, mine ? sh[lane & 3][2] : 0.0f});
+    if (lane == 0) {
+        n = 0;
+        for (int w = 0; w < WAVES; ++w) n += __float_as_int(sh[w][3]);
         float *o = a.part + ((size_t)row * a.parts + part) * 4;
         o[0] = s.m;
         o[1] = s.r;
@@ -148,83 +302,207 @@ __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a) {
     }
 }
 
-template <bool HALF>
-__global__ __launch_bounds__(THREADS) void logprob_finish_kernel(LogprobArgs a) {
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const void *x = HALF ? (const void *)(static_cast<const uint16_t *>(a.logits) + row * a.ld)
-                         : (const void *)(static_cast<const float *>(a.logits) + row * a.ld);
-    const int subs = (a.V + SUB - 1) / SUB;
-    __shared__ float sh[WAVES][4];
-    __shared__ uint64_t best[WAVES];
-    Sums s{-INFINITY, 0.0f, 0.0f};
-    int n = 0;
-    for (int p = tid; p < a.parts; p += THREADS) {
-        const float *o = a.part + ((size_t)row * a.parts + p) * 4;
-        s = join(s, Sums{o[0], o[1], o[2]});
-        n += __float_as_int(o[3]);
-    }
-    s = wave_join(s);
+// The best keys that one wave has seen: up to 64 kept in order, and room for a
+// push of 64 more. A key's rank is how many of the others are larger (keys are
+// distinct), found by broadcasting each; once k are kept, what is not above the
+// last of them is not taken up.
+__device__ __forceinline__ uint64_t from_lane(uint64_t v, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
+struct Best {
+    uint64_t *buf;  // LDS, 128
+    int k, n;
+    uint64_t floor;
+
+    __device__ void sort() {
+        const int lane = __lane_id();
+        wave_lds_sync();
+        const uint64_t p = lane < n ? buf[lane] : 0, q = lane + 64 < n ? buf[lane + 64] : 0;
+        int rp = 0, rq = 0;
+        // (absent keys are 0, larger than none)
+        if (n <= 64) {
+            for (int i = 0; i < n; i += 8)
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
-    if (lane == 0) {
-        sh[tid >> 6][0] = s.m;
-        sh[tid >> 6][1] = s.r;
-        sh[tid >> 6][2] = s.t;
-        sh[tid >> 6][3] = __int_as_float(n);
+                for (int u = 0; u < 8; ++u) rp += from_lane(p, i + u) > p;
+        } else {
+            for (int i = 0; i < 64; i += 4)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const uint64_t o = from_lane(p, i + u), w = from_lane(q, i + u);
+                    rp += (o > p) + (w > p);
+                    rq += (o > q) + (w > q);
+                }
+        }
+        wave_lds_sync();
+        if (lane < n && rp < k) buf[rp] = p;
+        if (lane + 64 < n && rq < k) buf[rq] = q;
+        n = min(n, k);
+        wave_lds_sync();
+        if (n == k) {
+            const uint64_t last = from_lane(buf[k - 1], 0);
+            floor = last > floor ? last : floor;
+        }
+    }
+    __device__ __forceinline__ void push(uint64_t key, bool take) {
+        take = take && key > floor;
+        const uint64_t m = __ballot(take);
+        if (!m) return;
+        if (take) buf[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = key;
+        n += __builtin_popcountll(m);
+        if (n > 64 || (n == 64 && k <= 32)) sort();
+    }
+};
+
+// LDS of the second kernel.
+struct FinishLds {
+    uint64_t buf[FIN_WAVES][128];
+    uint64_t list[FIN_WAVES * kLogprobTop];  // of all waves, what can be among the first k
+    uint64_t out[kLogprobTop];               // the first k in order
+    int rank[FIN_WAVES * kLogprobTop];
+    int count[FIN_WAVES];
+    int n;
+};
+
+// The waves' lists as one, in sh.out; how many there are (k at most). The
+// largest of the waves' own k-th keys bounds the answer's from below; a
+// candidate's comparisons are spread over the waves.
+__device__ int merge(Best &best, FinishLds &sh, int wid, bool mine) {
+    const int lane = __lane_id(), tid = threadIdx.x, k = best.k;
+    if (mine) {
+        best.sort();
+        if (lane == 0) sh.count[wid] = best.n;
+    }
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    uint64_t bound = 0;
+    if (mine) {
+        for (int w = 0; w < FIN_WAVES; ++w)
+            if (sh.count[w] == k) bound = sh.buf[w][k - 1] > bound ? sh.buf[w][k - 1] : bound;
+        const bool take = lane < best.n && best.buf[lane] >= bound;
+        const uint64_t m = __ballot(take);  // (lists are in order: a leading run)
+        int at = 0;
+        if (lane == 0 && m) at = atomicAdd(&sh.n, __builtin_popcountll(m));
+        at = __builtin_amdgcn_readfirstlane(at);
+        if (take) {
+            sh.list[at + lane] = best.buf[lane];
+            sh.rank[at + lane] = 0;
+        }
     }
     __syncthreads();
-    s = Sums{sh[0][0], sh[0][1], sh[0][2]};
-    n = __float_as_int(sh[0][3]);
-    for (int w = 1; w < WAVES; ++w) {
-        s = join(s, Sums{sh[w][0], sh[w][1], sh[w][2]});
-        n += __float_as_int(sh[w][3]);
+    const int n = sh.n;
+    if (mine) {
+        for (int c = lane; c < n; c += 64) {
+            const uint64_t key = sh.list[c];
+            int r = 0;
+            for (int i = wid; i < n; i += FIN_WAVES) r += sh.list[i] > key;
+            if (r) atomicAdd(&sh.rank[c], r);
+        }
     }
+    __syncthreads();
+    if (mine)
+        for (int c = tid; c < n; c += 64 * FIN_WAVES)
+            if (sh.rank[c] < k) sh.out[sh.rank[c]] = sh.list[c];
+    __syncthreads();
+    return min(n, k);
+}
+
+// One block a row: a wave joins the parts' sums; eight others (TOP) find the
+// alternatives.
+template <bool HALF, bool TOP>
+__global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finish_kernel(LogprobArgs a, int subs_max) {
+    constexpr int VEC = HALF ? 8 : 4, PER = SUB / (64 * VEC);
+    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const void *x = HALF ? (const void *)(static_cast<const uint16_t *>(a.logits) + row * a.ld)
+                         : (const void *)(static_cast<const float *>(a.logits) + row * a.ld);
     const float nan = __builtin_nanf("");
-    const bool fine = s.m > -INFINITY && s.m < INFINITY;
-    const float logs = fine ? log1pf(s.r) : nan;
-    if (tid == 0) {
+    __shared__ float whole[2];
+    if (wid == (TOP ? FIN_WAVES : 0)) {
         const int t = a.tokens[row];
         const bool ok = t >= 0 && t < a.V;
-        a.logprob[row] = ok ? (logit<HALF>(x, t) - s.m) - logs : nan;
-        if (a.rank) a.rank[row] = ok ? n : -1;
-        if (a.entropy) a.entropy[row] = logs - LN2 * s.t / (1.0f + s.r);
+        const float xt = ok ? logit<HALF>(x, t) : nan;
+        Sums s{-INFINITY, 0.0f, 0.0f};
+        int n = 0;
+        for (int p = 0; p < a.parts; p += 64) {
+            Sums q{-INFINITY, 0.0f, 0.0f};
+            int c = 0;
+            if (p + lane < a.parts) {
+                const float4_t o = *reinterpret_cast<const float4_t *>(a.part + ((size_t)row * a.parts + p + lane) * 4);
+                q = Sums{o[0], o[1], o[2]};
+                c = __float_as_int(o[3]);
+            }
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) c += __shfl_xor(c, o);
+            n += c;
+            q = wave_join(q);
+            if (p == 0) s = q;
+            else s = wave_join(Sums{lane == 0 ? s.m : lane == 1 ? q.m : -INFINITY, lane == 0 ? s.r : lane == 1 ? q.r : 0.0f,
+                                    lane == 0 ? s.t : lane == 1 ? q.t : 0.0f});
+        }
+        const float logs = s.m > -INFINITY && s.m < INFINITY ? log1pf(s.r) : nan;
+        if (lane == 0) {
+            whole[0] = s.m;
+            whole[1] = logs;
+            a.logprob[row] = (xt - s.m) - logs;
+            if (a.rank) a.rank[row] = ok ? n : -1;
+            if (a.entropy) a.entropy[row] = logs - LN2 * s.t / (1.0f + s.r);
+        }
     }
-    // the k best: the first key below the last one taken, k times
-    uint64_t below = ~0ull;
-    for (int j = 0; j < a.k; ++j) {
-        uint64_t mine = 0;
-        for (int c = tid >> 6; c < subs; c += WAVES) {
-            if (key_of(a.sub_max[(size_t)row * subs + c], 0) < mine) continue;
-            for (int i = c * SUB + lane; i < min(a.V, (c + 1) * SUB); i += 64) {
-                const uint64_t key = key_of(logit<HALF>(x, i), i);
-                if (key < below && key > mine) mine = key;
+    if constexpr (TOP) {
+        __shared__ FinishLds sh;
+        const bool mine = wid < FIN_WAVES;
+        const int off = row_offset<HALF>(x), subs = (a.V + off + SUB - 1) / SUB;
+        Best best{sh.buf[mine ? wid : 0], a.k, 0, 0};
+        if (mine)
+            for (int c = wid * 64; c < subs; c += 64 * FIN_WAVES) {
+                const int i = c + lane;
+                best.push(i < subs ? key_of(a.sub_max[(size_t)row * subs_max + i], i) : 0, i < subs);
+            }
+        const int chunks = merge(best, sh, wid, mine);
+        if (mine) {
+            // values below the k-th sub-chunk's maximum have k others ahead of them
+            const uint64_t bound = chunks == a.k ? sh.out[a.k - 1] & ~0xFFFFFFFFull : 0;
+            best = Best{sh.buf[wid], a.k, 0, 0};
+            for (int c = wid; c < chunks; c += FIN_WAVES) {
+                const int base = (int)index_of(sh.out[c]) * SUB - off;
+                u32x4 raw[PER];
+#pragma unroll
+                for (int u = 0; u < PER; ++u) raw[u] = read_piece<HALF>(x, base + (u * 64 + lane) * VEC, a.V, false);
+#pragma unroll
+                for (int u = 0; u < PER; ++u)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int i = base + (u * 64 + lane) * VEC + e;
+                        const uint64_t key = key_of(piece_value<HALF>(raw[u], e), i);
+                        best.push(key, key >= bound && i >= 0 && i < a.V);
+                    }
             }
         }
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)mine, o);
-            mine = other > mine ? other : mine;
-        }
-        __syncthreads();
-        if (lane == 0) best[tid >> 6] = mine;
-        __syncthreads();
-        below = best[0];
-        for (int w = 1; w < WAVES; ++w) below = best[w] > below ? best[w] : below;
-        if (tid == 0) {
-            a.top_ids[(size_t)row * a.k + j] = (int32_t)index_of(below);
-            a.top_logprobs[(size_t)row * a.k + j] = (value_of(below) - s.m) - logs;
+        merge(best, sh, wid, mine);
+        if (wid == 0 && lane < a.k) {
+            const uint64_t key = sh.out[lane];
+            a.top_ids[(size_t)row * a.k + lane] = (int32_t)index_of(key);
+            a.top_logprobs[(size_t)row * a.k + lane] = (value_of(key) - whole[0]) - whole[1];
         }
     }
 }
 
 hipError_t launch_token_logprobs(const LogprobArgs &a, bool half, hipStream_t st) {
     const unsigned grid = (unsigned)a.parts * (unsigned)a.M;
-    if (half) logprob_scan_kernel<true><<<grid, THREADS, 0, st>>>(a);
-    else logprob_scan_kernel<false><<<grid, THREADS, 0, st>>>(a);
+    const int subs = logprob_subs(a.V);
+    if (half) logprob_scan_kernel<true><<<grid, THREADS, 0, st>>>(a, subs);
+    else logprob_scan_kernel<false><<<grid, THREADS, 0, st>>>(a, subs);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (half) logprob_finish_kernel<true><<<a.M, THREADS, 0, st>>>(a);
-    else logprob_finish_kernel<false><<<a.M, THREADS, 0, st>>>(a);
+    if (a.k) {
+        if (half) logprob_finish_kernel<true, true><<<a.M, 64 * (FIN_WAVES + 1), 0, st>>>(a, subs);
+        else logprob_finish_kernel<false, true><<<a.M, 64 * (FIN_WAVES + 1), 0, st>>>(a, subs);
+    } else {
+        if (half) logprob_finish_kernel<true, false><<<a.M, 64, 0, st>>>(a, subs);
+        else logprob_finish_kernel<false, false><<<a.M, 64, 0, st>>>(a, subs);
+    }
     return hipGetLastError();
 }
 

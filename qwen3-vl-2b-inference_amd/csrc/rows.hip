@@ -100,112 +100,160 @@ hipError_t launch_draft_plan(const int32_t *parents, const int32_t *row_start, c
 }
 
 // ------------------------------------------------- head norms, rotation, cache
-// Four lanes a head: lane j of the quad holds x[8m + 2j] and x[8m + 2j + 1] for
-// m = 0 .. D/8 - 1. The reference's sum of squares (8 chains, chain c over
-// x[c], x[c+8], ..., folded left to right) then runs as two chains a lane with
-// no exchange before the fold, and the pair (x_i, x_{i + D/2}) that the
-// rotation mixes lies in one lane. A wave takes 16 heads of one row, counted q,
-// k, v.
-#define Q3VL_QUADB(v, j) \
-    __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), (j) * 0x55, 0xF, 0xF, true))
+// Four lanes a head: lane j of the quad holds x[16 q + 4 j + e], q = 0 .. D/16 -
+// 1, e = 0 .. 3, so that a quad reads and writes 64 bytes in one piece, and the
+// pair (x_i, x_{i + D/2}) that the rotation mixes lies in one lane. A wave takes
+// 16 heads of one row, counted q, k, v.
+//
+// The sum of squares keeps the reference's order (chain c = 0 .. 7 over x[c],
+// x[c + 8], ..., folded left to right): lanes j and j ^ 2 each hold half of the
+// same four chains, exchange their values and run all of them.
+//
+// Bound by HBM: 8 D bytes a query head in and out, 6 D a key or value head.
+// Pairs of two values a lane (32-byte pieces, no exchange) took 65.8 us for 4999
+// rows of 16 + 8 + 8 heads with three positions.
+#define Q3VL_QUADP(v, ctrl) \
+    __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xF, 0xF, true))
+
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));      // rows of any stride
+typedef uint16_t h4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint16_t h4_row __attribute__((ext_vector_type(4)));
 
 template <int D, bool HALF, bool AXES3>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkRopeArgs a) {
-    constexpr int M = D / 8, MH = M / 2;
+    constexpr int Q = D / 16, QH = Q / 2;
+    __shared__ __align__(16) float wsh[2][D], ssh[2][D];  // norm weights and their scales, q and k
     const int lane = threadIdx.x & 63, j = lane & 3;
     const int per_row = (a.heads + 2 * a.kv_heads + 15) >> 4;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int64_t row = unit / per_row;
-    if (row >= a.rows) return;
-    const int head = (int)(unit - row * per_row) * 16 + (lane >> 2);
-    if (head >= a.heads + 2 * a.kv_heads) return;  // (whole quads)
-    const int32_t *pr = a.pos + row * (AXES3 ? 3 : 1);
-    const int p0 = pr[0];
-    if (p0 == -1) return;
-    bool ok = p0 >= 0 && p0 < a.table_rows;
-    int p1 = p0, p2 = p0;
+    const int64_t units = a.rows * per_row, stride = (int64_t)gridDim.x * 4;
+    int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (threadIdx.x < D) {
+        const int d = threadIdx.x, g = d / a.gs;
+        wsh[0][d] = (float)a.q_w[d];
+        wsh[1][d] = (float)a.k_w[d];
+        ssh[0][d] = a.q_s[g];
+        ssh[1][d] = a.k_s[g];
+    }
+    int axes[QH];  // AXES3: this lane's frequencies' axes, two bits each
     if constexpr (AXES3) {
-        p1 = pr[1];
-        p2 = pr[2];
-        ok = ok && p1 >= 0 && p1 < a.table_rows && p2 >= 0 && p2 < a.table_rows;
-    }
-    const int64_t slot = a.slots[row];
-    const bool kept = ok && slot >= 0 && slot < (int64_t)a.batch * a.max_seq;
-    const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.kv_heads;
-    const int h = is_q ? head : head - a.heads - (is_k ? 0 : a.kv_heads);
-    const size_t at = kept ? (size_t)(slot / a.max_seq) * a.seq_stride + (size_t)h * a.head_stride +
-                                 (size_t)(slot % a.max_seq) * a.row_stride
-                           : 0;
-    const float *x = (is_q ? a.q + row * a.ldq : is_k ? a.k + row * a.ldk : a.v + row * a.ldv) + (size_t)h * D + 2 * j;
-    if (!is_q && !kept) return;
-    float2 v[M];
 #pragma unroll
-    for (int m = 0; m < M; ++m) v[m] = make_float2(x[8 * m], x[8 * m + 1]);
-    if (!is_q && !is_k) {
-        uint16_t *o = a.v_cache + at + 2 * j;
+        for (int q = 0; q < QH; ++q) {
+            axes[q] = 0;
 #pragma unroll
-        for (int m = 0; m < M; ++m) *reinterpret_cast<uint32_t *>(o + 8 * m) = f2h(v[m].x) | (uint32_t)f2h(v[m].y) << 16;
-        return;
-    }
-    const int8_t *w = is_q ? a.q_w : a.k_w;
-    const float *ws = is_q ? a.q_s : a.k_s;
-    float c0 = 0.0f, c1 = 0.0f;
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        c0 = fmaf(v[m].x, v[m].x, c0);
-        c1 = fmaf(v[m].y, v[m].y, c1);
-    }
-    float ss = Q3VL_QUADB(c0, 0) + Q3VL_QUADB(c1, 0);
-    ss = (ss + Q3VL_QUADB(c0, 1)) + Q3VL_QUADB(c1, 1);
-    ss = (ss + Q3VL_QUADB(c0, 2)) + Q3VL_QUADB(c1, 2);
-    ss = (ss + Q3VL_QUADB(c0, 3)) + Q3VL_QUADB(c1, 3);
-    const float inv = rcp_rn(sqrt_rn(ss * (1.0f / D) + a.eps));
-    auto turn = [&](float lo, float hi, int i, float &olo, float &ohi) {
-        int p = p0;
-        if constexpr (AXES3) {
-            if (a.interleaved) {
-                const int ax = i % 3;
-                p = ax == 1 && i < 3 * a.sec1 ? p1 : ax == 2 && i < 3 * a.sec2 ? p2 : p0;
-            } else {
-                p = i < a.sec0 ? p0 : i < a.sec0 + a.sec1 ? p1 : p2;
+            for (int e = 0; e < 4; ++e) {
+                const int i = 16 * q + 4 * j + e, r = i % 3;
+                const int ax = a.interleaved ? (r == 1 && i < 3 * a.sec1 ? 1 : r == 2 && i < 3 * a.sec2 ? 2 : 0)
+                                             : (i < a.sec0 ? 0 : i < a.sec0 + a.sec1 ? 1 : 2);
+                axes[q] |= ax << (2 * e);
             }
         }
-        const float c = ok ? a.cos[(size_t)p * (D / 2) + i] : __builtin_nanf("");
-        const float s = ok ? a.sin[(size_t)p * (D / 2) + i] : __builtin_nanf("");
-        const float y = (float)w[i] * ((ws[i / a.gs] * inv) * lo);
-        const float z = (float)w[i + D / 2] * ((ws[(i + D / 2) / a.gs] * inv) * hi);
-        olo = fmaf(y, c, -(z * s));
-        ohi = fmaf(y, s, z * c);
-    };
-#pragma unroll
-    for (int m = 0; m < MH; ++m) {
-        const int i = 8 * m + 2 * j;
-        float2 lo, hi;
-        turn(v[m].x, v[m + MH].x, i, lo.x, hi.x);
-        turn(v[m].y, v[m + MH].y, i + 1, lo.y, hi.y);
-        v[m] = lo;
-        v[m + MH] = hi;
     }
-    if (is_q && !HALF) {
-        float *o = static_cast<float *>(a.q_out) + row * a.ldo + (size_t)h * D + 2 * j;
-#pragma unroll
-        for (int m = 0; m < M; ++m) {
-            o[8 * m] = v[m].x;
-            o[8 * m + 1] = v[m].y;
+    __syncthreads();
+    for (; unit < units; unit += stride) {
+        const int64_t row = unit / per_row;
+        const int head = (int)(unit - row * per_row) * 16 + (lane >> 2);
+        const int32_t *pr = a.pos + row * (AXES3 ? 3 : 1);
+        const int p0 = pr[0];
+        if (p0 == -1 || head >= a.heads + 2 * a.kv_heads) continue;  // (whole quads)
+        bool ok = p0 >= 0 && p0 < a.table_rows;
+        int p1 = p0, p2 = p0;
+        if constexpr (AXES3) {
+            p1 = pr[1];
+            p2 = pr[2];
+            ok = ok && p1 >= 0 && p1 < a.table_rows && p2 >= 0 && p2 < a.table_rows;
         }
-    } else {
-        uint16_t *o = is_q ? static_cast<uint16_t *>(a.q_out) + row * a.ldo + (size_t)h * D + 2 * j : a.k_cache + at + 2 * j;
+        const int64_t slot = a.slots[row];
+        const bool kept = ok && slot >= 0 && slot < (int64_t)a.batch * a.max_seq;
+        const bool is_q = head < a.heads, is_k = !is_q && head < a.heads + a.kv_heads;
+        if (!is_q && !kept) continue;
+        const int h = is_q ? head : head - a.heads - (is_k ? 0 : a.kv_heads);
+        const float *x = (is_q ? a.q + row * a.ldq : is_k ? a.k + row * a.ldk : a.v + row * a.ldv) + (size_t)h * D + 4 * j;
+        float v[Q][4];
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            o[8 * m] = f2h(v[m].x);
-            o[8 * m + 1] = f2h(v[m].y);
+        for (int q = 0; q < Q; ++q) {
+            const f4_any r = *reinterpret_cast<const f4_any *>(x + 16 * q);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[q][e] = r[e];
+        }
+        if (is_q || is_k) {
+            // the rotation's factors (a NaN row where a position is past the tables)
+            float c[QH][4], n[QH][4];
+#pragma unroll
+            for (int q = 0; q < QH; ++q) {
+                const int i = 16 * q + 4 * j;
+                if constexpr (AXES3) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int ax = axes[q] >> (2 * e) & 3, p = ok ? (ax == 0 ? p0 : ax == 1 ? p1 : p2) : 0;
+                        c[q][e] = a.cos[(size_t)p * (D / 2) + i + e];
+                        n[q][e] = a.sin[(size_t)p * (D / 2) + i + e];
+                    }
+                } else {
+                    const size_t at = (size_t)(ok ? p0 : 0) * (D / 2) + i;
+                    const f4_any rc = *reinterpret_cast<const f4_any *>(a.cos + at), rn = *reinterpret_cast<const f4_any *>(a.sin + at);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        c[q][e] = rc[e];
+                        n[q][e] = rn[e];
+                    }
+                }
+            }
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const bool upper = j >= 2;  // holds the odd elements of its chains
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float o = Q3VL_QUADP(v[q][e], 0x4E);  // quad_perm [2,3,0,1]
+                    const float first = upper ? o : v[q][e], second = upper ? v[q][e] : o;
+                    sum[e] = fmaf(first, first, sum[e]);
+                    sum[e] = fmaf(second, second, sum[e]);
+                }
+            float ss = Q3VL_QUADP(sum[0], 0x00);
+#pragma unroll
+            for (int e = 1; e < 4; ++e) ss = ss + Q3VL_QUADP(sum[e], 0x00);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ss = ss + Q3VL_QUADP(sum[e], 0x55);
+            float inv = rcp_rn(sqrt_rn(ss * (1.0f / D) + a.eps));
+            if (!ok) inv = __builtin_nanf("");
+            const float *w = wsh[is_q ? 0 : 1] + 4 * j, *ws = ssh[is_q ? 0 : 1] + 4 * j;
+#pragma unroll
+            for (int q = 0; q < QH; ++q) {
+                const float4 wl = *reinterpret_cast<const float4 *>(w + 16 * q), wh = *reinterpret_cast<const float4 *>(w + 16 * q + D / 2);
+                const float4 sl = *reinterpret_cast<const float4 *>(ws + 16 * q), sh = *reinterpret_cast<const float4 *>(ws + 16 * q + D / 2);
+                const float wle[4] = {wl.x, wl.y, wl.z, wl.w}, whe[4] = {wh.x, wh.y, wh.z, wh.w};
+                const float sle[4] = {sl.x, sl.y, sl.z, sl.w}, she[4] = {sh.x, sh.y, sh.z, sh.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float y = wle[e] * ((sle[e] * inv) * v[q][e]);
+                    const float z = whe[e] * ((she[e] * inv) * v[q + QH][e]);
+                    v[q][e] = fmaf(y, c[q][e], -(z * n[q][e]));
+                    v[q + QH][e] = fmaf(y, n[q][e], z * c[q][e]);
+                }
+            }
+        }
+        if (is_q && !HALF) {
+            float *o = static_cast<float *>(a.q_out) + row * a.ldo + (size_t)h * D + 4 * j;
+#pragma unroll
+            for (int q = 0; q < Q; ++q) *reinterpret_cast<f4_any *>(o + 16 * q) = f4_any{v[q][0], v[q][1], v[q][2], v[q][3]};
+        } else if (is_q) {
+            uint16_t *o = static_cast<uint16_t *>(a.q_out) + row * a.ldo + (size_t)h * D + 4 * j;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                *reinterpret_cast<h4_any *>(o + 16 * q) = h4_any{f2h(v[q][0]), f2h(v[q][1]), f2h(v[q][2]), f2h(v[q][3])};
+        } else {
+            uint16_t *o = (is_k ? a.k_cache : a.v_cache) + (size_t)(slot / a.max_seq) * a.seq_stride + (size_t)h * a.head_stride +
+                          (size_t)(slot % a.max_seq) * a.row_stride + 4 * j;
+#pragma unroll
+            for (int q = 0; q < Q; ++q)
+                *reinterpret_cast<h4_row *>(o + 16 * q) = h4_row{f2h(v[q][0]), f2h(v[q][1]), f2h(v[q][2]), f2h(v[q][3])};
         }
     }
 }
 
 hipError_t launch_qk_norm_rope(const QkRopeArgs &a, int head_dim, bool half, int axes, hipStream_t st) {
-    const int64_t per_row = (a.heads + 2 * a.kv_heads + 15) / 16;
-    const unsigned grid = (unsigned)((a.rows * per_row + 3) / 4);
+    const int64_t per_row = (a.heads + 2 * a.kv_heads + 15) / 16, blocks = (a.rows * per_row + 3) / 4;
+    const unsigned grid = (unsigned)(blocks < 2048 ? blocks : 2048);  // eight a CU, each its share
     auto go = [&](auto kernel) {
         kernel<<<grid, 256, 0, st>>>(a);
         return hipGetLastError();

@@ -22,6 +22,7 @@ __global__ __launch_bounds__(1024) void draft_plan_kernel(const int32_t *parents
                                                           int batch, int rows, int max_rows, int max_seq,
                                                           uint64_t *mask, int words, int32_t *pos, int64_t *slots) {
     extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int more[16];  // per turn: whether some row has ancestors left
     const int b = blockIdx.x, tid = threadIdx.x, nt = blockDim.x;
     const int start = min(max(row_start[b], 0), rows);
     if (b == batch) {  // rows that hold no token
@@ -32,53 +33,67 @@ __global__ __launch_bounds__(1024) void draft_plan_kernel(const int32_t *parents
         for (size_t i = (size_t)start * words + tid; i < (size_t)rows * words; i += nt) mask[i] = 0;
         return;
     }
-    const int end = min(max(row_start[b + 1], start), rows);
+    const int end = min(max(row_start[b + 1], start), rows), len = cache_len[b];
+    const int64_t base = (int64_t)len + (pos_delta ? pos_delta[b] : 0);
     const int n = min(end - start, max_rows);
     const int wn = (n + 63) >> 6;  // words that n rows can set
+    const int ws = wn > 1 ? 32 - __builtin_clz(wn - 1) : 0, wm = (1 << ws) - 1;  // (row, word) items by shifts
     uint64_t *m = reinterpret_cast<uint64_t *>(smem);                        // [n][wn]
     int16_t *up = reinterpret_cast<int16_t *>(smem + (size_t)n * wn * 8);  // [2][n]
+    if (tid < 16) more[tid] = 0;
     for (int t = tid; t < n; t += nt) {
         const int p = parents[start + t];
         up[t] = (int16_t)(p >= -1 && p < t ? p : -2);
     }
-    for (int i = tid; i < n * wn; i += nt) {
-        const int t = i / wn, w = i - t * wn;
-        m[i] = w == t >> 6 ? 1ull << (t & 63) : 0;
+    for (int i = tid; i < n << ws; i += nt) {
+        const int t = i >> ws, w = i & wm;
+        if (w < wn) m[t * wn + w] = w == t >> 6 ? 1ull << (t & 63) : 0;
     }
-    for (int turn = 0;; turn ^= 1) {
-        const int16_t *u = up + turn * n;
-        int16_t *next = up + (turn ^ 1) * n;
-        int more = 0;
-        __syncthreads();  // up and the masks of the last turn are written
+    __syncthreads();
+    for (int turn = 0;; ++turn) {  // (12 at most: each doubles what is covered)
+        const int16_t *u = up + (turn & 1) * n;
+        int16_t *next = up + (~turn & 1) * n;
+        bool again = false;
         for (int t = tid; t < n; t += nt) {
             const int p = u[t], q = p >= 0 ? u[p] : p;
             next[t] = (int16_t)q;
-            more |= q >= 0;
+            again = again || q >= 0;
         }
-        for (int i = tid; i < n * wn; i += nt) {
-            const int t = i / wn, w = i - t * wn, p = u[t];
-            if (p >= 0 && w <= p >> 6) m[i] |= m[p * wn + w];
+        for (int i = tid; i < n << ws; i += nt) {
+            const int t = i >> ws, w = i & wm, p = u[t];
+            if (p >= 0 && w <= p >> 6) m[t * wn + w] |= m[p * wn + w];
         }
-        if (!__syncthreads_or(more)) {
+        if (again) more[turn] = 1;
+        __syncthreads();
+        if (!more[turn]) {
             up = next;
             break;
         }
     }
     // (past the last turn's barrier: every mask is whole)
-    const int len = cache_len[b];
-    const int64_t base = (int64_t)len + (pos_delta ? pos_delta[b] : 0);
+    int16_t *done = up == reinterpret_cast<int16_t *>(m + (size_t)n * wn) ? up + n : up - n;  // (the other buffer)
     for (int t = tid; t < end - start; t += nt) {
-        const size_t r = (size_t)start + t;
         int64_t at = -2, slot = -1;
         if (t < n && up[t] == -1 && len >= 0 && (int64_t)len + t < max_seq) {
             at = base - 1;
-            for (int w = 0; w < wn; ++w) at += __popcll(m[t * wn + w]);
+            for (int w = 0; w <= t >> 6; ++w) at += __popcll(m[t * wn + w]);
             if (at < 0 || at > 0x7fffffff) at = -2;
             else slot = (int64_t)b * max_seq + len + t;
         }
-        pos[r] = (int32_t)at;
-        slots[r] = slot;
-        for (int w = 0; w < words; ++w) mask[r * words + w] = slot >= 0 && w < wn ? m[t * wn + w] : 0;
+        pos[start + t] = (int32_t)at;
+        slots[start + t] = slot;
+        if (t < n) done[t] = slot >= 0;
+    }
+    __syncthreads();
+    const int64_t left = (int64_t)(end - start) * words;
+    uint64_t *out = mask + (size_t)start * words;
+    if (words == wn && n == end - start && ws >= 0 && wm + 1 == wn) {  // a row's words are what LDS holds
+        for (int i = tid; i < n << ws; i += nt) out[i] = done[i >> ws] ? m[i] : 0;
+        return;
+    }
+    for (int64_t i = tid; i < left; i += nt) {
+        const int t = (int)(i / words), w = (int)(i - (int64_t)t * words);
+        out[i] = t < n && w < wn && done[t] ? m[t * wn + w] : 0;
     }
 }
 

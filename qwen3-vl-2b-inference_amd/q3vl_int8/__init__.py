@@ -307,16 +307,14 @@ def token_logprobs(logits, tokens, top_k=0, workspace=None, stream=None):
     views of wider ones): a TokenLogprobs. Larger values come first, equal ones
     by index; a token outside of [0, V) gives NaN and rank -1."""
     torch = _torch()
-    from .attention import _empty, _rows, _vec
-    ld = _rows(logits, (torch.float32, torch.float16), "logits")
+    from .attention import _device, _empty, _rows, _vec
+    dev, f32, i32 = _device(), torch.float32, torch.int32
+    ld = _rows(logits, (f32, torch.float16), "logits", dev)
     M, V = logits.shape
-    _vec(tokens, torch.int32, M, "tokens")
-    k = max(int(top_k), 0)
-    f = _empty((2, M), torch.float32, logits, stream)
-    rank = _empty((M,), torch.int32, logits, stream)
-    ids = _empty((M, k), torch.int32, logits, stream)
-    top = _empty((M, k), torch.float32, logits, stream)
-    lp, ent = f[0], f[1]
+    _vec(tokens, i32, M, "tokens", dev)
+    k = max(top_k, 0)
+    lp, ent, top = (_empty(logits, stream, *n, dtype=f32) for n in ((M,), (M,), (M, k)))
+    rank, ids = _empty(tokens, stream, M), _empty(tokens, stream, M, k)
     wp, wb = _ws(workspace)
     _check(lib().q3vl_token_logprobs(logits.data_ptr(), ld, FP16 if logits.dtype is torch.float16 else FP32, tokens.data_ptr(),
                                      M, V, top_k, lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(),

@@ -58,41 +58,69 @@ def _L():
     return _lib
 
 
-def _here(t, name):
-    if t.device.index != _torch()._C._cuda_getDevice():
+# A call costs 4 to 6 us in the library (its launches), so the checks around it
+# are kept short, as the linears' are: the usual tensor passes in one
+# expression and only another one is looked at again for its error.
+def _device():
+    try:
+        return _torch()._C._cuda_getDevice()
+    except RuntimeError:  # no device at all
+        return -2
+
+
+def _here(t, name, dev):
+    if t.get_device() != dev:
         raise ValueError(f"{name} must be on the current device")
 
 
-def _rows(t, dtypes, name):
-    """A 2-d device tensor whose rows are contiguous (views of wider rows too)."""
+def _rows(t, dtypes, name, dev):
+    """Row stride of a 2-d device tensor whose rows are contiguous (views of
+    wider rows too)."""
     torch = _torch()
-    if (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == 2
-            and (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1)):
-        _here(t, name)
-        return max(t.stride(0), t.shape[1])
+    if isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype in dtypes and t.dim() == 2:
+        n, m = t.shape
+        s, u = t.stride()
+        if u == 1 and s >= m:
+            return s
+        if (u == 1 or m <= 1) and (s >= m or n <= 1):
+            return max(s, m)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a device tensor")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(map(str, dtypes))}, got {t.dtype}")
+    _here(t, name, dev)
     raise ValueError(f"{name} must be 2-d with contiguous rows")
 
 
-def _vec(t, dtype, n, name):
+def _vec(t, dtype, n, name, dev):
+    """A contiguous device tensor of n values (None: any number)."""
+    if isinstance(t, _torch().Tensor) and t.get_device() == dev and t.dtype is dtype and t.is_contiguous() and (n is None or t.numel() == n):
+        return
     _need(t, dtype, name)
-    _here(t, name)
-    if n is not None and t.numel() != n:
-        raise ValueError(f"{name} must hold {n} values, got {t.numel()}")
+    _here(t, name, dev)
+    raise ValueError(f"{name} must hold {n} values, got {t.numel()}")
 
 
-def _empty(shape, dtype, like, stream):
-    """An output of a call on `stream`: memory of that stream's own."""
+def _mask_words(mask, rows, dev):
     torch = _torch()
+    if not (isinstance(mask, torch.Tensor) and mask.get_device() == dev and mask.dtype is torch.int64 and mask.is_contiguous()
+            and mask.dim() == 2):
+        _need(mask, torch.int64, "mask", 2)
+        _here(mask, "mask", dev)
+    n, words = mask.shape
+    if n != rows:
+        raise ValueError("mask must have a line for each row")
+    return words
+
+
+def _empty(like, stream, *shape, dtype=None):
+    """An output of a call on `stream`: memory of that stream's own."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(*shape) if dtype is None else like.new_empty(*shape, dtype=dtype)
+    with _torch().cuda.stream(stream):
+        return like.new_empty(*shape, dtype=dtype or like.dtype)
 
 
 class KVCache:
@@ -121,7 +149,7 @@ class KVCache:
         self.k, self.v = k, v
         self.c = _CacheC(k.data_ptr(), v.data_ptr(), B, H, S, D, *st)
         self.ref = ctypes.byref(self.c)
-        self.device = k.device
+        self.device, self.dev = k.device, k.get_device()
 
 
 class QKNorm:
@@ -138,7 +166,9 @@ class QKNorm:
         if q_w.numel() != k_w.numel():
             raise ValueError("q_w and k_w must have the same size")
         self.t = (q_w, q_s, k_w, k_s)
-        self.head_dim = q_w.numel()
+        self.head_dim, self.dev = q_w.numel(), q_w.get_device()
+        if any(t.get_device() != self.dev for t in self.t):
+            raise ValueError("the norm's tensors must be on one device")
         self.c = _NormC(q_w.data_ptr(), q_s.data_ptr(), k_w.data_ptr(), k_s.data_ptr(), gs, eps)
         self.ref = ctypes.byref(self.c)
 
@@ -155,7 +185,9 @@ class Rope:
             _need(t, torch.float32, n, 2)
         if cos.shape != sin.shape:
             raise ValueError("cos and sin must have the same shape")
-        self.t = (cos, sin)
+        if cos.device != sin.device:
+            raise ValueError("cos and sin must be on one device")
+        self.t, self.dev = (cos, sin), cos.get_device()
         self.head_dim, self.axes = 2 * cos.shape[1], 1 if sections is None else 3
         sec = (0, 0, 0) if sections is None else tuple(sections)
         if len(sec) != 3:
@@ -173,25 +205,26 @@ def draft_plan(parents, row_start, cache_len, max_seq, max_rows, pos_delta=None,
     position and slot -1, rows that cannot be planned (a bad parent, no room in
     the cache, past max_rows) position -2 and slot -1."""
     torch = _torch()
-    _vec(parents, torch.int32, None, "parents")
+    dev, i32 = _device(), torch.int32
+    _vec(parents, i32, None, "parents", dev)
+    _vec(cache_len, i32, None, "cache_len", dev)
     rows, batch = parents.numel(), cache_len.numel()
-    _vec(cache_len, torch.int32, None, "cache_len")
-    _vec(row_start, torch.int32, batch + 1, "row_start")
+    _vec(row_start, i32, batch + 1, "row_start", dev)
     if pos_delta is not None:
-        _vec(pos_delta, torch.int32, batch, "pos_delta")
-    words = max(1, -(-max_rows // 64))
+        _vec(pos_delta, i32, batch, "pos_delta", dev)
     if mask is None:
-        mask = _empty((rows, words), torch.int64, parents, stream)
+        words = max(1, -(-max_rows // 64))
+        mask = _empty(parents, stream, rows, words, dtype=torch.int64)
     else:
-        _need(mask, torch.int64, "mask", 2)
-        _here(mask, "mask")
-        words = mask.shape[1]
-        if mask.shape[0] != rows:
-            raise ValueError("mask must have a line for each row")
-    pos = _empty((rows,), torch.int32, parents, stream) if pos is None else pos
-    slots = _empty((rows,), torch.int64, parents, stream) if slots is None else slots
-    _vec(pos, torch.int32, rows, "pos")
-    _vec(slots, torch.int64, rows, "slots")
+        words = _mask_words(mask, rows, dev)
+    if pos is None:
+        pos = _empty(parents, stream, rows)
+    else:
+        _vec(pos, i32, rows, "pos", dev)
+    if slots is None:
+        slots = _empty(parents, stream, rows, dtype=torch.int64)
+    else:
+        _vec(slots, torch.int64, rows, "slots", dev)
     _check(_L().q3vl_draft_plan(parents.data_ptr(), row_start.data_ptr(), cache_len.data_ptr(), _ptr(pos_delta), batch, rows,
                                 max_rows, max_seq, mask.data_ptr(), words, pos.data_ptr(), slots.data_ptr(), _stream(stream)))
     return mask, pos, slots
@@ -206,23 +239,26 @@ def qk_norm_rope(q, k, v, cache, slots, pos, norm, rope, out=None, out_dtype=Non
     [rows], or [rows, 3] under a Rope with sections. Rows at position -1 hold
     no token and are left alone; out may be q."""
     torch = _torch()
-    f32 = (torch.float32,)
-    ldq, ldk, ldv = _rows(q, f32, "q"), _rows(k, f32, "k"), _rows(v, f32, "v")
-    D = cache.c.head_dim
+    dev, f32 = _device(), (torch.float32,)
+    ldq, ldk, ldv = _rows(q, f32, "q", dev), _rows(k, f32, "k", dev), _rows(v, f32, "v", dev)
+    c = cache.c
+    D = c.head_dim
     rows, qn = q.shape
-    if qn % D or k.shape != (rows, cache.c.kv_heads * D) or v.shape != k.shape:
+    if qn % D or k.shape != (rows, c.kv_heads * D) or v.shape != k.shape:
         raise ValueError("shape mismatch between q, k, v and the cache")
     if norm.head_dim != D or rope.head_dim != D:
         raise ValueError("norm and rope must have the cache's head_dim")
+    if not cache.dev == norm.dev == rope.dev == dev:
+        raise ValueError("cache, norm and rope must be on the current device")
     if out is None:
-        out = _empty((rows, qn), out_dtype or torch.float32, q, stream)
+        out = _empty(q, stream, rows, qn, dtype=out_dtype)
     elif out_dtype is not None and out.dtype != out_dtype:
         raise TypeError("out has another dtype than out_dtype")
-    ldo = _rows(out, (torch.float32, torch.float16), "out")
+    ldo = _rows(out, (torch.float32, torch.float16), "out", dev)
     if out.shape != q.shape:
         raise ValueError("out must have q's shape")
-    _vec(slots, torch.int64, rows, "slots")
-    _vec(pos, torch.int32, rows * rope.axes, "pos")
+    _vec(slots, torch.int64, rows, "slots", dev)
+    _vec(pos, torch.int32, rows * rope.axes, "pos", dev)
     _check(_L().q3vl_qk_norm_rope(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
                                   FP16 if out.dtype is torch.float16 else FP32, rows, qn // D, cache.ref, slots.data_ptr(),
                                   pos.data_ptr(), norm.ref, rope.ref, _stream(stream)))
@@ -251,26 +287,25 @@ def tree_attention(q, cache, row_start, cache_len, max_rows, mask=None, max_len=
     of one (a hint for splitting the work, default the whole cache). scale:
     default 1 / sqrt(head_dim). A row that sees nothing gives 0."""
     torch = _torch()
-    ldq = _rows(q, (torch.float32, torch.float16), "q")
+    dev = _device()
+    ldq = _rows(q, (torch.float32, torch.float16), "q", dev)
     c = cache.c
     D, batch = c.head_dim, c.batch
     rows, qn = q.shape
     if qn % D:
         raise ValueError("q's rows must be whole heads of the cache's head_dim")
+    if cache.dev != dev:
+        raise ValueError("cache must be on the current device")
     if out is None:
-        out = _empty((rows, qn), q.dtype, q, stream)
-    ldo = _rows(out, (q.dtype,), "out")
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
-    _vec(row_start, torch.int32, batch + 1, "row_start")
-    _vec(cache_len, torch.int32, batch, "cache_len")
-    words = 0
-    if mask is not None:
-        _need(mask, torch.int64, "mask", 2)
-        _here(mask, "mask")
-        words = mask.shape[1]
-        if mask.shape[0] != rows:
-            raise ValueError("mask must have a line for each row")
+        out = _empty(q, stream, rows, qn)
+        ldo = qn
+    else:
+        ldo = _rows(out, (q.dtype,), "out", dev)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    _vec(row_start, torch.int32, batch + 1, "row_start", dev)
+    _vec(cache_len, torch.int32, batch, "cache_len", dev)
+    words = 0 if mask is None else _mask_words(mask, rows, dev)
     wp, wb = _ws(workspace)
     _check(_L().q3vl_tree_attention(q.data_ptr(), ldq, out.data_ptr(), ldo, FP16 if q.dtype is torch.float16 else FP32, rows,
                                     qn // D, cache.ref, row_start.data_ptr(), cache_len.data_ptr(), _ptr(mask), words,

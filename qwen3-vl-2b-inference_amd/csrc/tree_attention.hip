@@ -138,16 +138,20 @@ template <bool HALF> __device__ __forceinline__ void put(void *out, int64_t at, 
 // sum |q k|. fp16 queries and their probabilities are one term each: half a
 // step of fp16 in each p, as the output's own rounding.
 //
-// With M the running maximum of a row's raw scores, p = 2^(s sc - bias') held as
-// 2^(s sc + bias), bias = 14 - M sc: probabilities up to 2^14 use fp16's range,
-// 2^-28 of the largest is still a normal number. A row's results are its sum O
-// and l with weights 2^(-bias).
+// p is held as 2^(s sc + bias), bias = BASE - M sc, M a row's largest raw score
+// when the bias was last set: a score that passes it by up to GROW stays under
+// fp16's 2^16, so the accumulators are rescaled in the first step and seldom
+// after (with every new maximum, some row of 32 had one in most steps: 267 VALU
+// instructions a step). 2^-20 of the largest p is still a normal number, and of
+// fp32's two terms the smaller keeps 2^-31 of it. A row's results are its O and
+// l with weights 2^(-bias). l is summed by the matrix cores too, as V's column
+// of ones: a product a step instead of an addition a score.
 //
 // What no row sees never enters: rows past the end are zeros, scores of unseen
 // keys are replaced by -inf before the maximum. An unseen V row of another
 // row's draft can still hold an infinity or NaN, and 0 times it is NaN: a row
 // whose O or l is not finite is done again by row_attention; so is one whose
-// scores pass 2^23, where the rounding of M sc alone moves 2^14 by bits.
+// scores pass 2^23, where the rounding of M sc alone moves p by bits.
 template <int D, int NR, bool SHARED> struct Tile {
     static constexpr int RB = 2 * D;             // bytes of a cached row
     static constexpr int RI = D / 32;            // loads of 1 KiB for 16 rows
@@ -164,6 +168,12 @@ template <int D, int NR, bool SHARED> struct Tile {
     static_assert(LDS <= 160 * 1024 && sizeof(RowScratch) <= (size_t)RING, "LDS");
 };
 
+constexpr float BASE = 6.0f, GROW = 9.0f;
+
+// (rows of q and out may lie anywhere)
+typedef _Float16 half8_any __attribute__((ext_vector_type(8), aligned(2)));
+typedef float float4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t half4_bits __attribute__((ext_vector_type(4), aligned(2)));
 typedef __fp16 fp16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 
@@ -182,13 +192,6 @@ __device__ __forceinline__ float column_max(float v) {
     auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
-__device__ __forceinline__ float column_sum(float v) {
-    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // 32 bits of a row's mask line from bit i on (i may be negative: positions
 // before the drafts, all seen); n rows exist.
 __device__ __forceinline__ uint32_t mask_window(const uint64_t *line, int words, int n, int i) {
@@ -255,18 +258,27 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         sc[nr] = sign == 0.0f ? 1.0f : fabsf(a.scale_log2e);
         if constexpr (HALF) {
             const _Float16 *p = static_cast<const _Float16 *>(a.q) + at;
+            half8_any r[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) r[ks] = *reinterpret_cast<const half8_any *>(p + 32 * ks);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) qf[nr][0][ks][e] = live[nr] ? (_Float16)(p[32 * ks + e] * (_Float16)sign) : (_Float16)0.0f;
+                for (int e = 0; e < 8; ++e) qf[nr][0][ks][e] = live[nr] ? (_Float16)(r[ks][e] * (_Float16)sign) : (_Float16)0.0f;
         } else {
             const float *p = static_cast<const float *>(a.q) + at;
             float v[KS][8], top = 0.0f;
+            float4_any r[KS][2];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                r[ks][0] = *reinterpret_cast<const float4_any *>(p + 32 * ks);
+                r[ks][1] = *reinterpret_cast<const float4_any *>(p + 32 * ks + 4);
+            }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    v[ks][e] = live[nr] ? p[32 * ks + e] * sign : 0.0f;
+                    v[ks][e] = live[nr] ? r[ks][e >> 2][e & 3] * sign : 0.0f;
                     top = fmaxf(top, fabsf(v[ks][e]));
                 }
             top = column_max(top);
@@ -311,33 +323,48 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     for (int ks = 0; ks < KS; ++ks) kaddr[ks] = i * T::RB + ((ks * 4 + g) ^ (D == 128 ? i : i >> 1)) * 16;
     const int vr = 4 * g + (i >> 2);  // row of a 16-key tile this lane's transposing read starts from
     const int vaddr = vr * T::RB + (((i & 3) >> 1) ^ (D == 128 ? vr : vr >> 1 & 7)) * 16 + (i & 1) * 8;
-    float M[NR], bias[NR], l[NR];
-    float4_t O[NT][NR];
+    const half8_t ones = {(_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1};
+    float M[NR], bias[NR];
+    float4_t O[NT][NR], L[NR];  // L: the sum of p, in each register and lane of the column
     bool any[NR];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
         M[nr] = -INFINITY;
-        bias[nr] = l[nr] = 0.0f;
+        bias[nr] = 0.0f;
         any[nr] = false;
+        L[nr] = float4_t{0, 0, 0, 0};
 #pragma unroll
         for (int dt = 0; dt < NT; ++dt) O[dt][nr] = float4_t{0, 0, 0, 0};
     }
     float4_t S[2][NR];
-    auto scores = [&](int klds) {
+    // operand reads, half a step's at a time: the next half is on its way while
+    // the matrix cores work on this one (left to itself, the compiler reads one
+    // operand ahead and each product pair waits out the LDS)
+    auto read_k = [&](half8_t (&f)[KS], int klds, int kb) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int ks = 0; ks < KS; ++ks) f[ks] = *reinterpret_cast<const half8_t *>(smem + klds + kaddr[ks] + kb * 16 * T::RB);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto read_v = [&](half8_t (&f)[NT / 2], int vlds, int part) {
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) S[kb][nr] = float4_t{0, 0, 0, 0};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const half8_t kf = *reinterpret_cast<const half8_t *>(smem + klds + kaddr[ks] + kb * 16 * T::RB);
-#pragma unroll
-                for (int q = NQ - 1; q >= 0; --q)
-#pragma unroll
-                    for (int nr = 0; nr < NR; ++nr)
-                        S[kb][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[nr][q][ks], S[kb][nr], 0, 0, 0);
-            }
+        for (int t = 0; t < NT / 2; ++t) {
+            const int dt = part * (NT / 2) + t;
+            const half4_t lo = read_transposed(smem + vlds + (vaddr ^ (dt * 32)));
+            const half4_t hi = read_transposed(smem + vlds + (vaddr ^ (dt * 32)) + 16 * T::RB);
+            f[t] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto scores = [&](const half8_t (&f)[KS], int kb) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) S[kb][nr] = float4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr)
+                    S[kb][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[ks], qf[nr][q][ks], S[kb][nr], 0, 0, 0);
     };
     half8_t P[NR][NQ];
     auto softmax = [&](int j) {
@@ -372,17 +399,17 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
 #pragma unroll
             for (int e = 1; e < 8; ++e) t = fmaxf(t, S[e >> 2][nr][e & 3]);
             top[nr] = column_max(t);
-            grow = grow || top[nr] > M[nr];
+            grow = grow || (top[nr] - M[nr]) * sc[nr] > GROW || M[nr] == -INFINITY;
         }
         if (__any(grow)) {
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
                 const float m = fmaxf(M[nr], top[nr]);
-                const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], 14.0f);
+                const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], BASE);
                 const float f = M[nr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(nb - bias[nr]);
                 M[nr] = m;
                 bias[nr] = nb;
-                l[nr] *= f;
+                L[nr] *= f;
 #pragma unroll
                 for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= f;
             }
@@ -392,7 +419,6 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(S[e >> 2][nr][e & 3], sc[nr], bias[nr]));
-            l[nr] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 P[nr][0][e] = (_Float16)p[e];
@@ -400,19 +426,23 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
             }
         }
     };
-    auto values = [&](int vlds) {
+    auto values = [&](const half8_t (&f)[NT / 2], int part) {
 #pragma unroll
-        for (int dt = 0; dt < NT; ++dt) {
-            const half4_t lo = read_transposed(smem + vlds + (vaddr ^ (dt * 32)));
-            const half4_t hi = read_transposed(smem + vlds + (vaddr ^ (dt * 32)) + 16 * T::RB);
-            const half8_t vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int t = 0; t < NT / 2; ++t)
 #pragma unroll
             for (int q = NQ - 1; q >= 0; --q)
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr)
-                    O[dt][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, P[nr][q], O[dt][nr], 0, 0, 0);
-        }
+                    O[part * (NT / 2) + t][nr] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_f16(f[t], P[nr][q], O[part * (NT / 2) + t][nr], 0, 0, 0);
     };
+    auto sums = [&] {
+#pragma unroll
+        for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) L[nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nr][q], L[nr], 0, 0, 0);
+    };
+    half8_t ka[KS], kb[KS], va[NT / 2], vb[NT / 2];
 
     if constexpr (SHARED) {
         auto load_tile = [&](int u) {
@@ -426,11 +456,20 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
             lds_barrier();  // the tile is there, and every wave is done with the other buffer
             if (u + 1 < u1) load_tile(u + 1);
             const int lds = (u & 1) * T::STAGE;
-#pragma unroll 1
+            read_k(ka, lds, 0);
+#pragma unroll
             for (int k = 0; k < 2; ++k) {
-                scores(lds + k * 32 * T::RB);
+                const int klds = lds + k * 32 * T::RB, vlds = klds + 64 * T::RB;
+                read_k(kb, klds, 1);
+                scores(ka, 0);
+                scores(kb, 1);
+                read_v(va, vlds, 0);
                 softmax(u * 64 + k * 32);
-                values(lds + 64 * T::RB + k * 32 * T::RB);
+                read_v(vb, vlds, 1);
+                sums();
+                values(va, 0);
+                if (k == 0) read_k(ka, klds + 32 * T::RB, 0);
+                values(vb, 1);
             }
         }
     } else {
@@ -448,12 +487,19 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         int lds = mine;
         for (int u = u0, j = jw; u < u1; ++u, j += T::UNIT) {
             dma_wait<YOUNGER>();
-            scores(lds);
+            read_k(ka, lds, 0);
+            read_k(kb, lds, 1);
+            scores(ka, 0);
+            scores(kb, 1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the slot is refilled
             load(a.k_cache, j + T::NS * T::UNIT, lds);
             softmax(j);
             dma_wait<YOUNGER>();
-            values(lds + 32 * T::RB);
+            read_v(va, lds + 32 * T::RB, 0);
+            read_v(vb, lds + 32 * T::RB, 1);
+            sums();
+            values(va, 0);
+            values(vb, 1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             load(a.v_cache, j + T::NS * T::UNIT, lds + 32 * T::RB);
             lds += T::STAGE;
@@ -468,24 +514,29 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     for (int e = tid; e <= T::BM; e += THREADS) flag[e] = 0;
     lds_barrier();
     bool redo[NR];
+    float l[NR];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-        l[nr] = column_sum(l[nr]);
+        l[nr] = L[nr][0];
         float z = l[nr] * 0.0f;
 #pragma unroll
         for (int dt = 0; dt < NT; ++dt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) z = fmaf(O[dt][nr][e], 0.0f, z);
-        // (the largest score's p is 2^14 if its product with sc rounds to within a bit)
-        redo[nr] = live[nr] && (z != 0.0f || (any[nr] && !(l[nr] >= 8192.0f)));
+        // (the largest score's p is 2^BASE at least if its product with sc rounds to within a bit)
+        redo[nr] = live[nr] && (z != 0.0f || (any[nr] && !(l[nr] >= 32.0f)));
         if (redo[nr]) flag[row[nr] - r0] = flag[T::BM] = 1;
     }
     auto emit = [&](int t, int hd, int d, float4_t o, float m, float lsum) {
         const int64_t r = s.start + t;
         if (a.splits == 1) {
             const float inv = m == -INFINITY ? 0.0f : 1.0f / lsum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) put<HALF>(a.out, r * a.ldo + (int64_t)hd * D + d + e, o[e] * inv);
+            o *= inv;
+            const int64_t at = r * a.ldo + (int64_t)hd * D + d;
+            if constexpr (HALF)
+                *reinterpret_cast<half4_bits *>(static_cast<uint16_t *>(a.out) + at) = half4_bits{f2h(o[0]), f2h(o[1]), f2h(o[2]), f2h(o[3])};
+            else
+                *reinterpret_cast<float4_any *>(static_cast<float *>(a.out) + at) = o;
         } else {
             const int64_t part = (r * a.heads + hd) * a.splits + split;
             *reinterpret_cast<float4_t *>(a.part_o + part * D + d) = o;

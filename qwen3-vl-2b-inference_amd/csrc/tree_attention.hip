@@ -314,16 +314,19 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         const int r = (t * 64 + lane) / (D / 8), c = lane % (D / 8);
         voff[t] = (r + (SHARED ? wid * 16 : 0)) * rsb + (c ^ swizzle<D>(r)) * 16;
     }
-    auto resource = [&](const uint16_t *c, int j, int most) {
-        const int left = min(j1 - j, most);
-        return make_rsrc(c + head_at + (size_t)j * a.row_stride, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
-    };
-    // rows from j on: 32 to this wave's own stage, or its 16 of a block's 64
-    auto load = [&](const uint16_t *c, int j, int lds) {
-        const rsrc_t r = resource(c, j, SHARED ? 64 : 32);
+    // rows from p on, `left` of them there: 32 to this wave's own stage, or its
+    // 16 of a block's 64
+    auto load = [&](const uint16_t *p, int left, int lds) {
+        left = min(left, SHARED ? 64 : 32);
+        const rsrc_t r = make_rsrc(p, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
 #pragma unroll
         for (int t = 0; t < NL; ++t) dma16(r, voff[t], 0, lds + ((SHARED ? wid * NL : 0) + t) * 1024);
     };
+    const size_t first_at = head_at + (size_t)(j0 + (SHARED ? 0 : wid * 32)) * a.row_stride, turn = (size_t)T::UNIT * a.row_stride;
+    const uint16_t *kp = a.k_cache + first_at, *vp = a.v_cache + first_at;  // of the next loads
+    // positions below this are seen by all of this wave's rows
+    const int first_tok = (r0 + (SHARED ? wid * 16 * NR : 0)) / group;
+    const int clear = min(s.len + (a.mask ? 0 : min(first_tok, n - 1) + 1), j1);
 
     // ---- one step: 32 keys from position j, K and V rows at LDS offsets
     int kaddr[KS];
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     };
     half8_t P[NR][NQ];
     auto softmax = [&](int j) {
-        if (j + 32 > min(s.len, j1)) {  // some keys are not for every row
+        if (j + 32 > clear) {  // some keys are not for every row
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
                 uint32_t w;
@@ -456,8 +459,10 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     if constexpr (SHARED) {
         auto load_tile = [&](int u) {
             const int lds = (u & 1) * T::STAGE;
-            load(a.k_cache, u * 64, lds);
-            load(a.v_cache, u * 64, lds + 64 * T::RB);
+            load(kp, j1 - u * 64, lds);
+            load(vp, j1 - u * 64, lds + 64 * T::RB);
+            kp += turn;
+            vp += turn;
         };
         if (u0 < u1) load_tile(u0);
         for (int u = u0; u < u1; ++u) {
@@ -485,23 +490,26 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         // loads younger than the K or V part waited for
         constexpr int YOUNGER = NL + (T::NS - 1) * 2 * NL;
         const int mine = wid * T::NS * T::STAGE;
-        const int jw = j0 + wid * 32;
+        int left = j1 - j0 - wid * 32;  // positions from the next loads' first on
         if (u0 < u1) {
 #pragma unroll
             for (int k = 0; k < T::NS; ++k) {
-                load(a.k_cache, jw + k * T::UNIT, mine + k * T::STAGE);
-                load(a.v_cache, jw + k * T::UNIT, mine + k * T::STAGE + 32 * T::RB);
+                load(kp, left, mine + k * T::STAGE);
+                load(vp, left, mine + k * T::STAGE + 32 * T::RB);
+                kp += turn;
+                vp += turn;
+                left -= T::UNIT;
             }
         }
         int lds = mine;
-        for (int u = u0, j = jw; u < u1; ++u, j += T::UNIT) {
+        for (int u = u0, j = j0 + wid * 32; u < u1; ++u, j += T::UNIT) {
             dma_wait<YOUNGER>();
             read_k(ka, lds, 0);
             read_k(kb, lds, 1);
             scores(ka, 0);
             scores(kb, 1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the slot is refilled
-            load(a.k_cache, j + T::NS * T::UNIT, lds);
+            load(kp, left, lds);
             softmax(j);
             dma_wait<YOUNGER>();
             read_v(va, lds + 32 * T::RB, 0);
@@ -510,7 +518,10 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
             values(va, 0);
             values(vb, 1);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            load(a.v_cache, j + T::NS * T::UNIT, lds + 32 * T::RB);
+            load(vp, left, lds + 32 * T::RB);
+            kp += turn;
+            vp += turn;
+            left -= T::UNIT;
             lds += T::STAGE;
             if (lds == mine + T::NS * T::STAGE) lds = mine;
         }

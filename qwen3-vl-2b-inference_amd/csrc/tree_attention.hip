@@ -256,53 +256,24 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     const int u0 = (int)((int64_t)units * split / a.splits), u1 = (int)((int64_t)units * (split + 1) / a.splits);
     const int j0 = u0 * T::UNIT, j1 = min(u1 * T::UNIT, total);
 
-    // ---- queries: operand registers, the score's factor
-    half8_t qf[NR][NQ][KS];
-    float sc[NR];
-    const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
+    // ---- queries (the first tiles' loads go out behind theirs, before they are used)
+    half8_any qh[NR][KS];
+    float4_any qs[NR][KS][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
         const int64_t at = (int64_t)(s.start + tok[nr]) * a.ldq + (int64_t)head[nr] * D + 8 * g;
-        sc[nr] = sign == 0.0f ? 1.0f : fabsf(a.scale_log2e);
-        if constexpr (HALF) {
-            const _Float16 *p = static_cast<const _Float16 *>(a.q) + at;
-            half8_any r[KS];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) r[ks] = *reinterpret_cast<const half8_any *>(p + 32 * ks);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) qf[nr][0][ks][e] = live[nr] ? (_Float16)(r[ks][e] * (_Float16)sign) : (_Float16)0.0f;
-        } else {
-            const float *p = static_cast<const float *>(a.q) + at;
-            float v[KS][8], top = 0.0f;
-            float4_any r[KS][2];
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                r[ks][0] = *reinterpret_cast<const float4_any *>(p + 32 * ks);
-                r[ks][1] = *reinterpret_cast<const float4_any *>(p + 32 * ks + 4);
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (HALF) {
+                qh[nr][ks] = *reinterpret_cast<const half8_any *>(static_cast<const _Float16 *>(a.q) + at + 32 * ks);
+            } else {
+                const float *p = static_cast<const float *>(a.q) + at + 32 * ks;
+                qs[nr][ks][0] = *reinterpret_cast<const float4_any *>(p);
+                qs[nr][ks][1] = *reinterpret_cast<const float4_any *>(p + 4);
             }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    v[ks][e] = live[nr] ? r[ks][e >> 2][e & 3] * sign : 0.0f;
-                    top = fmaxf(top, fabsf(v[ks][e]));
-                }
-            top = column_max(top);
-            // the largest value to [2^13, 2^14)
-            const int shift = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
-            sc[nr] = ldexpf(sc[nr], -shift);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float y = ldexpf(v[ks][e], shift);
-                    qf[nr][0][ks][e] = (_Float16)y;
-                    qf[nr][1][ks][e] = (_Float16)(y - (float)qf[nr][0][ks][e]);
-                }
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
 
     // ---- loads: lane's place in 16 rows of the cache, and of LDS
     const size_t head_at = (size_t)b * a.seq_stride + (size_t)h * a.head_stride;
@@ -324,6 +295,66 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     };
     const size_t first_at = head_at + (size_t)(j0 + (SHARED ? 0 : wid * 32)) * a.row_stride, turn = (size_t)T::UNIT * a.row_stride;
     const uint16_t *kp = a.k_cache + first_at, *vp = a.v_cache + first_at;  // of the next loads
+    auto load_tile = [&](int u) {  // (SHARED)
+        const int lds = (u & 1) * T::STAGE;
+        load(kp, j1 - u * 64, lds);
+        load(vp, j1 - u * 64, lds + 64 * T::RB);
+        kp += turn;
+        vp += turn;
+    };
+    const int mine = wid * T::NS * T::STAGE;  // (else: this wave's ring,
+    int left = j1 - j0 - wid * 32;            // positions from the next loads' first on)
+    if (u0 < u1) {
+        if constexpr (SHARED) {
+            load_tile(u0);
+        } else {
+#pragma unroll
+            for (int k = 0; k < T::NS; ++k) {
+                load(kp, left, mine + k * T::STAGE);
+                load(vp, left, mine + k * T::STAGE + 32 * T::RB);
+                kp += turn;
+                vp += turn;
+                left -= T::UNIT;
+            }
+        }
+    }
+
+    // ---- operand registers, the score's factor
+    half8_t qf[NR][NQ][KS];
+    float sc[NR];
+    const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        sc[nr] = sign == 0.0f ? 1.0f : fabsf(a.scale_log2e);
+        if constexpr (HALF) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qf[nr][0][ks][e] = live[nr] ? (_Float16)(qh[nr][ks][e] * (_Float16)sign) : (_Float16)0.0f;
+        } else {
+            float v[KS][8], top = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    v[ks][e] = live[nr] ? qs[nr][ks][e >> 2][e & 3] * sign : 0.0f;
+                    top = fmaxf(top, fabsf(v[ks][e]));
+                }
+            top = column_max(top);
+            // the largest value to [2^13, 2^14)
+            const int shift = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+            sc[nr] = ldexpf(sc[nr], -shift);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float y = ldexpf(v[ks][e], shift);
+                    qf[nr][0][ks][e] = (_Float16)y;
+                    qf[nr][1][ks][e] = (_Float16)(y - (float)qf[nr][0][ks][e]);
+                }
+        }
+    }
+
     // positions below this are seen by all of this wave's rows
     const int first_tok = (r0 + (SHARED ? wid * 16 * NR : 0)) / group;
     const int clear = min(s.len + (a.mask ? 0 : min(first_tok, n - 1) + 1), j1);
@@ -457,14 +488,6 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     half8_t ka[KS], kb[KS], va[NT / 2], vb[NT / 2];
 
     if constexpr (SHARED) {
-        auto load_tile = [&](int u) {
-            const int lds = (u & 1) * T::STAGE;
-            load(kp, j1 - u * 64, lds);
-            load(vp, j1 - u * 64, lds + 64 * T::RB);
-            kp += turn;
-            vp += turn;
-        };
-        if (u0 < u1) load_tile(u0);
         for (int u = u0; u < u1; ++u) {
             dma_wait<0>();
             lds_barrier();  // the tile is there, and every wave is done with the other buffer
@@ -489,18 +512,6 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     } else {
         // loads younger than the K or V part waited for
         constexpr int YOUNGER = NL + (T::NS - 1) * 2 * NL;
-        const int mine = wid * T::NS * T::STAGE;
-        int left = j1 - j0 - wid * 32;  // positions from the next loads' first on
-        if (u0 < u1) {
-#pragma unroll
-            for (int k = 0; k < T::NS; ++k) {
-                load(kp, left, mine + k * T::STAGE);
-                load(vp, left, mine + k * T::STAGE + 32 * T::RB);
-                kp += turn;
-                vp += turn;
-                left -= T::UNIT;
-            }
-        }
         int lds = mine;
         for (int u = u0, j = j0 + wid * 32; u < u1; ++u, j += T::UNIT) {
             dma_wait<YOUNGER>();
@@ -631,59 +642,92 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     }
 }
 
-// Joins a row's splits: one wave a (row, query head).
+// Joins a row's splits: one wave a (row, query head), four values a lane, 64 /
+// (D / 4) splits side by side and four such loads under way.
 template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeAttnArgs a) {
-    const int lane = threadIdx.x & 63;
+    constexpr int LANES = D / 4, SIDE = 64 / LANES;
+    const int lane = threadIdx.x & 63, d = lane % LANES * 4, side = lane / LANES;
     const int x = blockIdx.x * WAVES + (threadIdx.x >> 6);
     const int hd = x % a.heads, bt = x / a.heads, t = bt % a.max_rows, b = bt / a.max_rows;
     if (b >= a.batch) return;
     const Seq s = sequence(a, b);
     if (t >= s.n) return;
     const int64_t r = s.start + t, part = (r * a.heads + hd) * a.splits;
-    float o[D / 64];
-    for (int e = 0; e < D / 64; ++e) o[e] = __builtin_nanf("");
+    float4_t o = {0, 0, 0, 0};
     if (s.ok) {
-        const float m = lane < a.splits ? a.part_ml[(part + lane) * 2] : -INFINITY;
-        float lw = lane < a.splits ? a.part_ml[(part + lane) * 2 + 1] : 0.0f;
+        float m = -INFINITY, lw = 0.0f;
+        if (lane < a.splits) {
+            m = a.part_ml[(part + lane) * 2];
+            lw = a.part_ml[(part + lane) * 2 + 1];
+        }
         float top = m;
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        lw = m == -INFINITY ? 0.0f : lw * f;
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);  // (nothing seen there: o = l = 0)
+        lw *= f;
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) lw += __shfl_xor(lw, k);
-        for (int e = 0; e < D / 64; ++e) o[e] = 0.0f;
-        for (int k = 0; k < a.splits; ++k) {
-            const float mk = __shfl(m, k), fk = __shfl(f, k);
-            if (mk == -INFINITY) continue;  // nothing seen there
-            for (int e = 0; e < D / 64; ++e) o[e] = fmaf(a.part_o[(part + k) * D + e * 64 + lane], fk, o[e]);
+        const float *p = a.part_o + part * D + d;
+        for (int k = 0; k < a.splits; k += 4 * SIDE) {
+            float4_t v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int i = k + u * SIDE + side;
+                v[u] = i < a.splits ? *reinterpret_cast<const float4_t *>(p + (size_t)i * D) : float4_t{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float fk = __shfl(f, min(k + u * SIDE + side, 63));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(v[u][e], fk, o[e]);
+            }
         }
-        for (int e = 0; e < D / 64; ++e) o[e] = top == -INFINITY ? 0.0f : o[e] / lw;
+#pragma unroll
+        for (int k = LANES; k < 64; k <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k);
+        const float inv = top == -INFINITY ? 0.0f : 1.0f / lw;
+        o *= inv;
+    } else {
+        const float nan = __builtin_nanf("");
+        o = float4_t{nan, nan, nan, nan};
     }
-    for (int e = 0; e < D / 64; ++e) put<HALF>(a.out, r * a.ldo + (int64_t)hd * D + e * 64 + lane, o[e]);
+    if (side) return;
+    const int64_t at = r * a.ldo + (int64_t)hd * D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put<HALF>(a.out, at + e, o[e]);
 }
 
 namespace {
 
-constexpr int kSplits = 64;  // most, a lane of the joining wave each
+constexpr int kSplits = 32;  // most (a lane of the joining wave each; 64 gained nothing and cost up to half more)
 
 // Rows of a block: 16 or 32 with their own keys a wave, 64 or 128 with shared tiles.
 int block_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 
 }  // namespace
 
-// Blocks and splits. A launch has 2^24 blocks of 256 threads at most.
+// Splits. A CU holds one block of the few-row form, two of the other; as many
+// splits as fill the chip once (us over splits, 256 CUs; 16 / 8 heads of 128):
+// one token at 32000, 8 blocks unsplit: 184 at 1, 28.3 at 32; two trees of 16
+// rows over 16000, 16 blocks: 151 at 1, 29.1 at 16, 38 at 21; three of 61, 24
+// blocks: 454 at 1, 56 at 21 (504 blocks), 65 at 22 and more. Where that leaves
+// part of the chip idle, a few rounds of smaller blocks instead: 24 sequences of
+// 6000, 192 blocks: 88.5 at 1, 83.7 at 4; 40 of 3000, 320 blocks: 74 at 1, 68 at
+// 3. Not below 128 positions a split (one token at 1024: 12.3 at 1, 10.5 at 8).
+// A launch has 2^24 blocks of 256 threads at most.
 int tree_attention_splits(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len) {
     const int64_t kv_rows = (int64_t)max_rows * (heads / kv_heads);
     const int bm = block_rows(kv_rows);
     const int64_t tiles = (kv_rows + bm - 1) / bm, base = tiles * batch * kv_heads;
     if (base > (1 << 24) - 1 || (int64_t)batch * max_rows > (int64_t)((1 << 24) - 1) * WAVES / heads) return -1;
     if (base == 0) return 1;
-    const int64_t want = (512 + base - 1) / base;
-    const int64_t most = ((int64_t)max_len + 255) / 256;  // 256 positions a split at least
-    int64_t k = want < most ? want : most;
+    const int64_t slots = bm <= 32 ? 256 : 512, most = ((int64_t)max_len + 127) / 128;
+    int64_t k = slots / base;
+    if (bm <= 32 && k * base * 20 < slots * 17) k = 1024 / base;
+    k = k < most ? k : most;
     k = k < 1 ? 1 : k > kSplits ? kSplits : k;
-    return base * k > (1 << 24) - 1 ? 1 : (int)k;
+    return (int)k;
 }
 
 template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, hipStream_t st) {

@@ -1526,30 +1526,40 @@ int q3vl_qk_norm_rope(const float *q, size_t ldq, const float *k, size_t ldk, co
     return Q3VL_OK;
 }
 
-// Sizes of a call, checked; its splits and workspace bytes.
-static int tree_attention_plan(size_t rows, int heads, int max_rows, int max_len, const q3vl_kv_cache *c, int *splits,
-                               size_t *bytes) {
+static int check_tree_attention(size_t rows, int heads, int max_rows, int max_len, const q3vl_kv_cache *c) {
     const int rc = check_cache(c);
     if (rc) return rc;
     if (heads < 1 || heads % c->kv_heads)
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "heads=%d is not a multiple of kv_heads=%d", heads, c->kv_heads);
     if (max_rows < 0 || max_len < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "max_rows=%d max_len=%d", max_rows, max_len);
-    if (rows > 0x7fffffff / (size_t)heads || (int64_t)max_rows * (heads / c->kv_heads) > 0x7fffff00)
-        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu heads=%d)", rows, heads);
+    const size_t most = (size_t)max_rows < rows ? (size_t)max_rows : rows;
+    if (rows > 0x7fffffff / (size_t)heads || most * (size_t)(heads / c->kv_heads) > 0x7fffff00 ||
+        !tree_attention_fits((int64_t)most * (heads / c->kv_heads), c->kv_heads, c->batch, (int)most, heads))
+        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu heads=%d batch=%d)", rows, heads, c->batch);
+    return Q3VL_OK;
+}
+
+// A call's tile and splits, and its workspace bytes.
+static TreePlan plan_tree_attention(size_t rows, int heads, int max_rows, int max_len, const q3vl_kv_cache *c, bool half,
+                                    bool chain, size_t *bytes) {
     if ((size_t)max_rows > rows) max_rows = (int)rows;
     if (max_len == 0 || max_len > c->max_seq) max_len = c->max_seq;
-    *splits = tree_attention_splits((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, max_len);
-    if (*splits < 0) return fail(Q3VL_ERR_UNSUPPORTED, "too many blocks (batch=%d max_rows=%d)", c->batch, max_rows);
-    const size_t parts = rows * (size_t)heads * (size_t)*splits;
-    *bytes = *splits > 1 ? align256(parts * (size_t)c->head_dim * 4) + align256(parts * 8) : 0;
-    return Q3VL_OK;
+    const TreePlan p = tree_attention_plan((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, max_len, c->head_dim, half, chain);
+    const size_t parts = rows * (size_t)heads * (size_t)p.splits;
+    *bytes = p.splits > 1 ? align256(parts * (size_t)c->head_dim * 4) + align256(parts * 8) : 0;
+    return p;
 }
 
 size_t q3vl_tree_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
                                            const q3vl_kv_cache *cache) {
-    int splits = 0;
-    size_t bytes = 0;
-    return tree_attention_plan(rows, heads, max_rows, max_len, cache, &splits, &bytes) ? 0 : bytes;
+    if (check_tree_attention(rows, heads, max_rows, max_len, cache)) return 0;
+    size_t most = 0;
+    for (int i = 0; i < 4; ++i) {  // types, chains and trees
+        size_t bytes = 0;
+        plan_tree_attention(rows, heads, max_rows, max_len, cache, i & 1, i >> 1, &bytes);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,
@@ -1557,9 +1567,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
                         const int32_t *cache_len, const uint64_t *mask, int mask_words,
                         int max_rows, int max_len, float scale, void *workspace,
                         size_t workspace_bytes, q3vl_stream stream) {
-    int splits = 0;
-    size_t need = 0;
-    int rc = tree_attention_plan(rows, heads, max_rows, max_len, cache, &splits, &need);
+    int rc = check_tree_attention(rows, heads, max_rows, max_len, cache);
     if (rc) return rc;
     if (dtype != Q3VL_DTYPE_FP32 && dtype != Q3VL_DTYPE_FP16)
         return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
@@ -1570,6 +1578,9 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     if (!(scale > -INFINITY && scale < INFINITY)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "scale is not finite");
     if (rows == 0 || max_rows == 0) return Q3VL_OK;
     if (!q || !out || !row_start || !cache_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    const bool half = dtype == Q3VL_DTYPE_FP16;
+    size_t need = 0;
+    const TreePlan plan = plan_tree_attention(rows, heads, max_rows, max_len, cache, half, !mask, &need);
     char *w = nullptr;
     if (need && (rc = resolve_ws(workspace, workspace_bytes, need, &w))) return rc;
     TreeAttnArgs a{};
@@ -1586,7 +1597,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     a.cache_len = cache_len;
     a.mask = mask;
     a.part_o = reinterpret_cast<float *>(w);
-    a.part_ml = need ? reinterpret_cast<float *>(w + align256(rows * (size_t)heads * splits * cache->head_dim * 4)) : nullptr;
+    a.part_ml = need ? reinterpret_cast<float *>(w + align256(rows * (size_t)heads * plan.splits * cache->head_dim * 4)) : nullptr;
     a.rows = (int)rows;
     a.heads = heads;
     a.kv_heads = cache->kv_heads;
@@ -1594,9 +1605,9 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     a.max_seq = cache->max_seq;
     a.max_rows = (size_t)max_rows > rows ? (int)rows : max_rows;
     a.words = mask_words;
-    a.splits = splits;
+    a.splits = plan.splits;
     a.scale_log2e = (float)((double)scale * 1.4426950408889634);
-    Q3VL_HIP(launch_tree_attention(a, cache->head_dim, dtype == Q3VL_DTYPE_FP16, (hipStream_t)stream), "attention launch");
+    Q3VL_HIP(launch_tree_attention(a, cache->head_dim, half, plan.rows, (hipStream_t)stream), "attention launch");
     return Q3VL_OK;
 }
 

@@ -223,9 +223,15 @@ struct TreeAttnArgs {
     int rows, heads, kv_heads, batch, max_seq, max_rows, words, splits;
     float scale_log2e;     // scale / ln 2
 };
-// Pieces a sequence's cache is split into.
-int tree_attention_splits(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len);
-hipError_t launch_tree_attention(const TreeAttnArgs &a, int head_dim, bool half, hipStream_t st);
+struct TreePlan {
+    int rows;    // query rows of a block: 16 or 32 (waves walk their own keys), 64 or 128
+    int splits;  // pieces a sequence's cache is split into
+};
+TreePlan tree_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim,
+                             bool half, bool chain);
+// Whether the launches of a call fit a grid at all.
+bool tree_attention_fits(int64_t kv_rows, int kv_heads, int batch, int max_rows, int heads);
+hipError_t launch_tree_attention(const TreeAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st);
 
 struct LogprobArgs {
     const void *logits;

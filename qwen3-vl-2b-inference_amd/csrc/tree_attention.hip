@@ -213,18 +213,23 @@ __device__ __forceinline__ uint32_t mask_window(const uint64_t *line, int words,
 }
 
 template <int D, bool HALF, int NR, bool SHARED>
-__global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a, int tiles) {
+__global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a, int tiles, bool paired) {
     using T = Tile<D, NR, SHARED>;
     constexpr int KS = D / 32, NT = D / 16, NQ = HALF ? 1 : 2;
     extern __shared__ __align__(16) unsigned char smem[];
     // (loads with an LDS destination take its offset: 0, as the kernel has no other LDS)
     const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
-    int x = blockIdx.x;  // kv head, split, tile (the last rows, which see most, first), sequence
+    int x = blockIdx.x;  // kv head, split, tile, sequence
     const int h = x % a.kv_heads;
     x /= a.kv_heads;
     const int split = x % a.splits;
     x /= a.splits;
-    const int tile = tiles - 1 - x % tiles, b = x / tiles;
+    const int b = x / tiles;
+    x -= b * tiles;
+    // a chain's last rows see most: they go first, and where every block has a
+    // place at once (two a CU, the second half of them beside the first), the
+    // second half goes the other way round
+    const int tile = paired && 2 * x >= tiles ? x - (tiles + 1) / 2 : tiles - 1 - x;
     const Seq s = sequence(a, b);
     const int group = a.heads / a.kv_heads;
     const int n = min(s.n, a.max_rows), nrows = n * group, r0 = tile * T::BM;
@@ -701,46 +706,78 @@ template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join
 namespace {
 
 constexpr int kSplits = 32;  // most (a lane of the joining wave each; 64 gained nothing and cost up to half more)
-
-// Rows of a block: 16 or 32 with their own keys a wave, 64 or 128 with shared tiles.
-int block_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+constexpr int64_t kBlocks = (1 << 24) - 1;  // of 256 threads in a launch
 
 }  // namespace
 
-// Splits. A CU holds one block of the few-row form, two of the other; as many
-// splits as fill the chip once (us over splits, 256 CUs; 16 / 8 heads of 128):
-// one token at 32000, 8 blocks unsplit: 184 at 1, 28.3 at 32; two trees of 16
-// rows over 16000, 16 blocks: 151 at 1, 29.1 at 16, 38 at 21; three of 61, 24
-// blocks: 454 at 1, 56 at 21 (504 blocks), 65 at 22 and more. Where that leaves
-// part of the chip idle, a few rounds of smaller blocks instead: 24 sequences of
-// 6000, 192 blocks: 88.5 at 1, 83.7 at 4; 40 of 3000, 320 blocks: 74 at 1, 68 at
-// 3. Not below 128 positions a split (one token at 1024: 12.3 at 1, 10.5 at 8).
-// A launch has 2^24 blocks of 256 threads at most.
-int tree_attention_splits(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len) {
-    const int64_t kv_rows = (int64_t)max_rows * (heads / kv_heads);
-    const int bm = block_rows(kv_rows);
-    const int64_t tiles = (kv_rows + bm - 1) / bm, base = tiles * batch * kv_heads;
-    if (base > (1 << 24) - 1 || (int64_t)batch * max_rows > (int64_t)((1 << 24) - 1) * WAVES / heads) return -1;
-    if (base == 0) return 1;
-    const int64_t slots = bm <= 32 ? 256 : 512, most = ((int64_t)max_len + 127) / 128;
-    int64_t k = slots / base;
-    if (bm <= 32 && k * base * 20 < slots * 17) k = 1024 / base;
-    k = k < most ? k : most;
-    k = k < 1 ? 1 : k > kSplits ? kSplits : k;
-    return (int)k;
+// Rows of a block and splits.
+//
+// Up to 32 rows a kv head: blocks of 16 or 32 rows whose waves walk their own
+// keys, one to a CU, bound by its reads; as many splits as fill the chip once.
+// us over splits (16 / 8 heads of 128, fp32): one token at 32000, 8 blocks
+// unsplit: 184 at 1, 28.3 at 32; two trees of 16 rows over 16000, 16 blocks: 151
+// at 1, 29.1 at 16, 38 at 21. Where that leaves part of the chip idle, a few
+// rounds of smaller blocks: 24 sequences of 6000, 192 blocks: 88.5 at 1, 83.7 at
+// 4; 40 of 3000, 320 blocks: 74 at 1, 68 at 3. Not below 128 positions a split
+// (one token at 1024: 12.3 at 1, 10.5 at 8).
+//
+// More rows: blocks of 64 or 128, two to a CU. A turn of 64 positions takes 0.78
+// us at 64 rows in fp16, 1.1 in fp32, 1.18 and 1.9 at 128, times the blocks on
+// the CU (products and softmax keep the chip at its power limit), a quarter more
+// for a block alone; three and more wait for a place. A
+// split call writes and reads its partial results (4 TB/s) and has one launch
+// more (2.5 us). Both sides measured: 2000 rows behind 1200, fp16: 64 rows 57.5,
+// 128 rows 67 unsplit, 63 split; 4000 rows: 91 and 88; three trees of 61 over
+// 16000, fp32: 64 rows 72 at 5 splits, 65 at 10, 128 rows 72 at 10, 66 at 21; 16
+// trees of 64 over 500: 15.2 at 1 split, 28 at 2; 8 trees of 40 over 8000: 64
+// rows 66, 128 rows 56.
+TreePlan tree_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim,
+                             bool half, bool chain) {
+    const int64_t kv_rows = (int64_t)max_rows * (heads / kv_heads), most = ((int64_t)max_len + 127) / 128;
+    auto blocks_of = [&](int bm) { return (kv_rows + bm - 1) / bm * batch * kv_heads; };
+    if (kv_rows <= 32) {
+        const int bm = kv_rows <= 16 ? 16 : 32;
+        const int64_t base = blocks_of(bm);
+        if (base < 1) return {bm, 1};
+        int64_t k = 256 / base;
+        if (k * base * 20 < 256 * 17) k = 1024 / base;
+        k = k < most ? k : most;
+        return {bm, (int)(k < 1 ? 1 : k < kSplits ? k : kSplits)};
+    }
+    TreePlan best{64, 1};
+    double least = 1e30;
+    for (int bm = 64; bm <= 128; bm *= 2) {
+        const double turn = (bm == 64 ? (half ? 0.78 : 1.1) : (half ? 1.18 : 1.9)) * (head_dim == 64 ? 0.65 : 1.0);
+        // the block that sees most, and the mean of a chain's
+        const double all = max_len / 64.0, mean = chain ? all - (max_rows < max_len ? max_rows : max_len) / 128.0 : all;
+        for (int k = 1; k <= kSplits && (k == 1 || k <= most); ++k) {
+            const double load = (double)blocks_of(bm) * k / 256.0;
+            const double alone = all / k * turn * 1.25, shared = mean / k * turn * (load < 1.0 ? 1.0 : load);
+            const double t = (alone > shared ? alone : shared) +
+                             (k > 1 ? 2.5 + 8e-6 / 4.0 * (double)rows * heads * k * head_dim : 0.0);
+            if (t < least) {
+                least = t;
+                best = {bm, k};
+            }
+        }
+    }
+    if (blocks_of(best.rows) * best.splits > kBlocks) best.splits = 1;
+    return best;
 }
 
-template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, hipStream_t st) {
-    const int64_t kv_rows = (int64_t)a.max_rows * (a.heads / a.kv_heads);
-    const int bm = block_rows(kv_rows);
-    const int tiles = (int)((kv_rows + bm - 1) / bm);
+bool tree_attention_fits(int64_t kv_rows, int kv_heads, int batch, int max_rows, int heads) {
+    return (kv_rows + 15) / 16 * batch <= kBlocks / kv_heads && (int64_t)batch * max_rows <= kBlocks * WAVES / heads;
+}
+
+template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, int bm, hipStream_t st) {
+    const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
     const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
     auto go = [&](auto kernel, int lds) {
         if (lds > 64 * 1024) {
             const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
             if (e != hipSuccess) return e;
         }
-        kernel<<<grid, THREADS, lds, st>>>(a, tiles);
+        kernel<<<grid, THREADS, lds, st>>>(a, tiles, grid <= 512);
         return hipGetLastError();
     };
     hipError_t e;
@@ -754,9 +791,9 @@ template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, hi
     return hipGetLastError();
 }
 
-hipError_t launch_tree_attention(const TreeAttnArgs &a, int head_dim, bool half, hipStream_t st) {
-    if (head_dim == 128) return half ? launch_d<128, true>(a, st) : launch_d<128, false>(a, st);
-    return half ? launch_d<64, true>(a, st) : launch_d<64, false>(a, st);
+hipError_t launch_tree_attention(const TreeAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st) {
+    if (head_dim == 128) return half ? launch_d<128, true>(a, block_rows, st) : launch_d<128, false>(a, block_rows, st);
+    return half ? launch_d<64, true>(a, block_rows, st) : launch_d<64, false>(a, block_rows, st);
 }
 
 }  // namespace q3vl

@@ -724,7 +724,8 @@ constexpr int64_t kBlocks = (1 << 24) - 1;  // of 256 threads in a launch
 // More rows: blocks of 64 or 128, two to a CU. A turn of 64 positions takes 0.78
 // us at 64 rows in fp16, 1.1 in fp32, 1.18 and 1.9 at 128, times the blocks on
 // the CU (products and softmax keep the chip at its power limit), a quarter more
-// for a block alone; three and more wait for a place. A
+// for a block alone; three and more wait for a place. (A tree's rows are few and
+// its cache long: that two tiles read it costs 8 %.) A
 // split call writes and reads its partial results (4 TB/s) and has one launch
 // more (2.5 us). Both sides measured: 2000 rows behind 1200, fp16: 64 rows 57.5,
 // 128 rows 67 unsplit, 63 split; 4000 rows: 91 and 88; three trees of 61 over
@@ -747,12 +748,14 @@ TreePlan tree_attention_plan(int64_t rows, int heads, int kv_heads, int batch, i
     TreePlan best{64, 1};
     double least = 1e30;
     for (int bm = 64; bm <= 128; bm *= 2) {
-        const double turn = (bm == 64 ? (half ? 0.78 : 1.1) : (half ? 1.18 : 1.9)) * (head_dim == 64 ? 0.65 : 1.0);
+        const double turn = (bm == 64 ? (half ? 0.78 : 1.1) * (chain ? 1.0 : 1.08) : (half ? 1.18 : 1.9)) *
+                            (head_dim == 64 ? 0.65 : 1.0);
         // the block that sees most, and the mean of a chain's
         const double all = max_len / 64.0, mean = chain ? all - (max_rows < max_len ? max_rows : max_len) / 128.0 : all;
         for (int k = 1; k <= kSplits && (k == 1 || k <= most); ++k) {
-            const double load = (double)blocks_of(bm) * k / 256.0;
-            const double alone = all / k * turn * 1.25, shared = mean / k * turn * (load < 1.0 ? 1.0 : load);
+            const int64_t blocks = blocks_of(bm) * k;
+            const double load = blocks <= 256 ? 1.0 : blocks <= 512 ? 2.0 : (double)blocks / 256.0;  // on the fullest CU
+            const double alone = all / k * turn * 1.25, shared = mean / k * turn * load;
             const double t = (alone > shared ? alone : shared) +
                              (k > 1 ? 2.5 + 8e-6 / 4.0 * (double)rows * heads * k * head_dim : 0.0);
             if (t < least) {

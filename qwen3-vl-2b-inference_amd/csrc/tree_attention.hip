@@ -754,7 +754,7 @@ TreePlan tree_attention_plan(int64_t rows, int heads, int kv_heads, int batch, i
         const double all = max_len / 64.0, mean = chain ? all - (max_rows < max_len ? max_rows : max_len) / 128.0 : all;
         for (int k = 1; k <= kSplits && (k == 1 || k <= most); ++k) {
             const int64_t blocks = blocks_of(bm) * k;
-            const double load = blocks <= 256 ? 1.0 : blocks <= 512 ? 2.0 : (double)blocks / 256.0;  // on the fullest CU
+            const double load = blocks <= 1536 ? (double)((blocks + 255) / 256) : (double)blocks / 256.0;  // of the fullest CU
             const double alone = all / k * turn * 1.25, shared = mean / k * turn * load;
             const double t = (alone > shared ? alone : shared) +
                              (k > 1 ? 2.5 + 8e-6 / 4.0 * (double)rows * heads * k * head_dim : 0.0);

@@ -426,7 +426,10 @@ int q3vl_qk_norm_rope(const float *q, size_t ldq, const float *k, size_t ldk, co
  * behind the last sequence, and rows of a sequence past max_rows, are left as
  * they were in `out`. max_rows: the most rows of one sequence. max_len: the
  * most cached positions of one sequence with its rows, used only to choose how
- * far the work is split (0: max_seq). head_dim 64 or 128. */
+ * far the work is split (0: max_seq). `out` may be q itself, with its stride.
+ * Scores of 2^23 and more (in powers of 2), infinities and NaN that a row sees
+ * take a slow path of plain fp32. head_dim 64 or 128. Workspace: the bytes for
+ * the same rows, heads, max_rows, max_len and cache, any type and mask. */
 size_t q3vl_tree_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
                                            const q3vl_kv_cache *cache);
 int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,

@@ -52,6 +52,7 @@ inline size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 constexpr size_t kMaxGemvParts = 8192;  // >= grid of any GEMV launch
+constexpr size_t kLogprobMaxM = 1 << 22, kLogprobMaxV = 1 << 30;  // blocks of a launch, indexes of a row
 constexpr int kGemmArgmaxParts = 64;    // argmax partials per row after a GEMM
 
 bool gs_ok_gemv(size_t gs) { return gs == 16 || gs == 32 || gs == 64 || gs == 128 || gs == 256; }
@@ -1426,6 +1427,8 @@ static int check_cache(const q3vl_kv_cache *c) {
         return fail(Q3VL_ERR_UNSUPPORTED, "head_dim=%d: 64 or 128 are served", c->head_dim);
     if (!aligned16(c->k) || !aligned16(c->v) || c->seq_stride % 8 || c->head_stride % 8 || c->row_stride % 8)
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "cache rows must be 16-byte aligned");
+    if (c->max_seq > 0x7fffff00 || c->batch > 0x7ffffffe)
+        return fail(Q3VL_ERR_UNSUPPORTED, "cache too large: batch=%d max_seq=%d", c->batch, c->max_seq);
     const size_t d = (size_t)c->head_dim;
     // (a tile of the attention addresses its rows by 32-bit byte offsets)
     if (c->row_stride < d || c->row_stride > (1u << 23) || c->seq_stride > (SIZE_MAX >> 20) || c->head_stride > (SIZE_MAX >> 20))
@@ -1612,7 +1615,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
 }
 
 size_t q3vl_token_logprobs_workspace_bytes(size_t M, size_t V) {
-    if (M == 0 || V == 0 || V > 0x7fffff00 || M > 0x7fffffff) return 0;
+    if (M == 0 || V == 0 || V > kLogprobMaxV || M > kLogprobMaxM) return 0;
     return align256(M * (size_t)logprob_parts((int)M, (int)V) * 16) + align256(M * (size_t)logprob_subs((int)V) * 4);
 }
 
@@ -1622,13 +1625,12 @@ int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t 
                         size_t workspace_bytes, q3vl_stream stream) {
     if (dtype != Q3VL_DTYPE_FP32 && dtype != Q3VL_DTYPE_FP16)
         return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
-    if (V == 0 || V > 0x7fffff00 || ld < V || ld > (SIZE_MAX >> 24))
+    if (V == 0 || ld < V || ld > (SIZE_MAX >> 32))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape V=%zu ld=%zu", V, ld);
     if (top_k < 0 || top_k > kLogprobTop || (size_t)top_k > V)
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "top_k=%d: 0 to %d, at most V=%zu", top_k, kLogprobTop, V);
     if (M == 0) return Q3VL_OK;
-    if (M > 0x7fffffff || M * (size_t)logprob_parts((int)M, (int)V) > 0x7fffffff)
-        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (M=%zu V=%zu)", M, V);
+    if (M > kLogprobMaxM || V > kLogprobMaxV) return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (M=%zu V=%zu)", M, V);
     if (!logits || !tokens || !logprob || (top_k && (!top_ids || !top_logprobs)))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     if ((uintptr_t)logits % (dtype == Q3VL_DTYPE_FP16 ? 2 : 4)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned logits");

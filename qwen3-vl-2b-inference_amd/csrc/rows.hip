@@ -165,7 +165,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkRopeArgs a) {
     }
     __syncthreads();
     for (; unit < units; unit += stride) {
-        const int64_t row = unit / per_row;
+        const int64_t row = (uint32_t)unit / (uint32_t)per_row;  // (units fit 31 bits)
         const int head = (int)(unit - row * per_row) * 16 + (lane >> 2);
         const int32_t *pr = a.pos + row * (AXES3 ? 3 : 1);
         const int p0 = pr[0];
@@ -257,8 +257,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkRopeArgs a) {
             for (int q = 0; q < Q; ++q)
                 *reinterpret_cast<h4_any *>(o + 16 * q) = h4_any{f2h(v[q][0]), f2h(v[q][1]), f2h(v[q][2]), f2h(v[q][3])};
         } else {
-            uint16_t *o = (is_k ? a.k_cache : a.v_cache) + (size_t)(slot / a.max_seq) * a.seq_stride + (size_t)h * a.head_stride +
-                          (size_t)(slot % a.max_seq) * a.row_stride + 4 * j;
+            // (slots mostly fit 32 bits, whose division is a fraction of the 64-bit one)
+            const uint64_t seq = slot <= 0xFFFFFFFFll ? (uint32_t)slot / (uint32_t)a.max_seq : (uint64_t)slot / (uint32_t)a.max_seq;
+            uint16_t *o = (is_k ? a.k_cache : a.v_cache) + seq * a.seq_stride + (size_t)h * a.head_stride +
+                          ((size_t)slot - seq * (uint32_t)a.max_seq) * a.row_stride + 4 * j;
 #pragma unroll
             for (int q = 0; q < Q; ++q)
                 *reinterpret_cast<h4_row *>(o + 16 * q) = h4_row{f2h(v[q][0]), f2h(v[q][1]), f2h(v[q][2]), f2h(v[q][3])};

@@ -1,6 +1,8 @@
 // tree_attention.hip -- attention of several rows a sequence over its cache:
 // one token of each sequence of a batch, a prompt's chunk, or a tree of
 // drafted tokens. gfx950.
+#include <atomic>
+
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 #include "q3vl_mfma.hpp"
@@ -772,22 +774,36 @@ bool tree_attention_fits(int64_t kv_rows, int kv_heads, int batch, int max_rows,
     return (kv_rows + 15) / 16 * batch <= kBlocks / kv_heads && (int64_t)batch * max_rows <= kBlocks * WAVES / heads;
 }
 
-template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, int bm, hipStream_t st) {
-    const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
+// Raises the kernel's LDS limit, once a device.
+template <auto Kernel> static hipError_t allow_lds(int bytes) {
+    if (bytes <= 64 * 1024) return hipSuccess;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+template <int D, bool HALF, int NR, bool SHARED> static hipError_t launch_tile(const TreeAttnArgs &a, hipStream_t st) {
+    using T = Tile<D, NR, SHARED>;
+    const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + T::BM - 1) / T::BM);
     const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
-    auto go = [&](auto kernel, int lds) {
-        if (lds > 64 * 1024) {
-            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-            if (e != hipSuccess) return e;
-        }
-        kernel<<<grid, THREADS, lds, st>>>(a, tiles, grid <= 512);
-        return hipGetLastError();
-    };
+    const hipError_t e = allow_lds<&tree_attention_kernel<D, HALF, NR, SHARED>>(T::LDS);
+    if (e != hipSuccess) return e;
+    tree_attention_kernel<D, HALF, NR, SHARED><<<grid, THREADS, T::LDS, st>>>(a, tiles, grid <= 512);
+    return hipGetLastError();
+}
+
+template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, int bm, hipStream_t st) {
     hipError_t e;
-    if (bm == 16) e = go(tree_attention_kernel<D, HALF, 1, false>, Tile<D, 1, false>::LDS);
-    else if (bm == 32) e = go(tree_attention_kernel<D, HALF, 2, false>, Tile<D, 2, false>::LDS);
-    else if (bm == 64) e = go(tree_attention_kernel<D, HALF, 1, true>, Tile<D, 1, true>::LDS);
-    else e = go(tree_attention_kernel<D, HALF, 2, true>, Tile<D, 2, true>::LDS);
+    if (bm == 16) e = launch_tile<D, HALF, 1, false>(a, st);
+    else if (bm == 32) e = launch_tile<D, HALF, 2, false>(a, st);
+    else if (bm == 64) e = launch_tile<D, HALF, 1, true>(a, st);
+    else e = launch_tile<D, HALF, 2, true>(a, st);
     if (e != hipSuccess || a.splits == 1) return e;
     const unsigned waves = (unsigned)a.batch * a.max_rows * a.heads;
     tree_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(a);

@@ -285,7 +285,9 @@ def tree_attention(q, cache, row_start, cache_len, max_rows, mask=None, max_len=
     t. Their keys and values are in the cache already (qk_norm_rope). max_rows:
     the most rows of one sequence; max_len: the most positions, cached and new,
     of one (a hint for splitting the work, default the whole cache). scale:
-    default 1 / sqrt(head_dim). A row that sees nothing gives 0."""
+    default 1 / sqrt(head_dim). out may be q. A row that sees nothing gives 0.
+    workspace: alloc_tree_attention_workspace with the same max_rows and
+    max_len."""
     torch = _torch()
     dev = _device()
     ldq = _rows(q, (torch.float32, torch.float16), "q", dev)

@@ -440,6 +440,15 @@ def test_attention_layouts():
     one.check(one.run(cache=qa.KVCache(layers[0][1][None], layers[1][1][None])))
 
 
+@pytest.mark.parametrize("rows,lens", [([1, 1], [900, 5]), ([40, 7], [700, 3]), ([150, 20], [64, 40])], ids=str)
+def test_attention_in_place(rows, lens):
+    """out over q gives what a separate out gives."""
+    for half in (False, True):
+        B = Batch(16, rows, lens, 8, 4, 128, half, True)
+        x = dev(B.q)
+        np.testing.assert_array_equal(B.run(q=x, out=x), B.run())
+
+
 def test_attention_offsets_past_32_bits():
     """A cache of over 2^32 bytes a head and 2^33 in all: the last positions."""
     S, D = (1 << 25) + 1024, 64

@@ -70,6 +70,7 @@ BAD, UNS = q.ERR_INVALID_ARGUMENT, q.ERR_UNSUPPORTED
     (dict(cache_over=dict(row_stride=64)), BAD, "strides"),
     (dict(cache_over=dict(row_stride=1 << 24)), BAD, "strides"),
     (dict(cache_over=dict(max_seq=0)), BAD, "bad cache"),
+    (dict(cache_over=dict(max_seq=2 ** 31 - 1)), UNS, "too large"),
     (dict(cache=None), BAD, "null cache"),
     (dict(norm=None), BAD, "null norm"),
     (dict(dtype=q.INT8), UNS, "q_dtype"),
@@ -118,6 +119,7 @@ def attn(cache_over={}, **over):
     (dict(q=None), BAD, "null"),
     (dict(cache_len=None), BAD, "null"),
     (dict(rows=1 << 30), UNS, "too large"),
+    (dict(cache_over=dict(batch=1 << 24), rows=1 << 20, max_rows=64), UNS, "too large"),
 ])
 def test_tree_attention_refusals(over, code, text):
     refused(attn(**over), code, text)
@@ -136,6 +138,8 @@ def logp(**over):
     (dict(k=-1), BAD, "top_k=-1"),
     (dict(k=65), BAD, "top_k=65"),
     (dict(V=3, k=4), BAD, "top_k=4"),
+    (dict(M=(1 << 22) + 1), UNS, "too large"),
+    (dict(V=(1 << 30) + 1, ld=1 << 31), UNS, "too large"),
     (dict(x=P + 2), BAD, "misaligned"),
     (dict(x=None), BAD, "null"),
     (dict(lp=None), BAD, "null"),

@@ -13,6 +13,8 @@
 // first, equal ones by place): each of k others ahead of a sub-chunk has a
 // value ahead of all of its own. The second kernel picks those sub-chunks and
 // reads them again, k of V / 512, instead of every block keeping a list.
+#include <type_traits>
+
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 #include "q3vl_mfma.hpp"
@@ -53,10 +55,12 @@ struct Sums {
     float m, r, t;
 };
 
-// 2^((lo - m) log2 e) for lo <= m, and its exponent, cut off where it is 0:
-// keeps -inf (0 times infinity otherwise) out of t. m is finite here.
-__device__ __forceinline__ float weight(float lo, float m, float &arg) {
-    arg = fmaxf((lo - m) * LOG2E, FAR);
+// 2^((lo - m) log2 e) for lo <= m, and its exponent. CUT: the exponent cut off
+// where the weight is 0, which keeps -inf (0 times infinity otherwise) out of t.
+// m is finite here.
+template <bool CUT = true> __device__ __forceinline__ float weight(float lo, float m, float &arg) {
+    arg = (lo - m) * LOG2E;
+    if (CUT) arg = fmaxf(arg, FAR);
     return __builtin_amdgcn_exp2f(arg);
 }
 
@@ -118,11 +122,14 @@ __device__ __forceinline__ bool ahead(float x, int i, float xt, int t) { return 
 // Sub-chunks lie on 16-byte boundaries, so a row may touch one more than its size asks for.
 int logprob_subs(int V) { return (V + 7 + SUB - 1) / SUB; }
 
-// Blocks a row: four a CU over all rows, a wave of each with two sub-chunks at least.
+// Blocks a row: about 4096 over all rows, every wave with the same number of
+// turns but the last (a turn is two sub-chunks).
 int logprob_parts(int M, int V) {
-    const int most = (logprob_subs(V) + 2 * WAVES - 1) / (2 * WAVES), want = (1024 + M - 1) / M;
-    const int p = want < most ? want : most;
-    return p < 1 ? 1 : p < kLogprobParts ? p : kLogprobParts;
+    const int64_t turns = (V + 7 + 2 * SUB - 1) / (2 * SUB);
+    int64_t each = (turns * M + 2 * WAVES * 2048) / (WAVES * 4096);
+    if (each < 1) each = 1;
+    const int64_t p = (turns + WAVES * each - 1) / (WAVES * each);
+    return (int)(p < kLogprobParts ? p : kLogprobParts);
 }
 
 // A lane's 16 bytes of a row, values [i, i + VEC), -inf outside of [0, V);
@@ -181,6 +188,7 @@ __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a, in
     const int t = a.tokens[row];
     const bool ok = t >= 0 && t < a.V;
     float xt = ok ? logit<HALF>(x, t) : 0.0f;
+    if (part == 0 && tid == 0) a.logprob[row] = ok ? xt : __builtin_nanf("");  // (for the second kernel)
     if (!(xt > -INFINITY)) xt = -INFINITY;
     Sums s{-INFINITY, 0.0f, 0.0f};
     float z = 0.0f;  // NaN once a NaN (or infinities of both signs) has been read
@@ -264,19 +272,21 @@ __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a, in
             s.r *= w;
             s.m = m;
         }
-        float r0 = 0.0f, r1 = 0.0f, t0 = 0.0f, t1 = 0.0f;
+        float r[2] = {0.0f, 0.0f}, q[2] = {0.0f, 0.0f};
+        auto add = [&](auto cut) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            float arg;
-            float w = weight(lose[i], ref, arg);
-            r0 += w;
-            t0 = fmaf(w, arg, t0);
-            w = weight(lose[i + 1], ref, arg);
-            r1 += w;
-            t1 = fmaf(w, arg, t1);
-        }
-        s.r += r0 + r1;
-        s.t += t0 + t1;
+            for (int i = 0; i < 16; ++i) {
+                float arg;
+                const float w = weight<decltype(cut)::value>(lose[i], ref, arg);
+                r[i & 1] += w;
+                q[i & 1] = fmaf(w, arg, q[i & 1]);
+            }
+        };
+        // (z is finite until a value was not; lose[15] is -inf in the first turn)
+        if (__any(!(__builtin_fabsf(z) < INFINITY) || lose[15] == -INFINITY)) add(std::true_type{});
+        else add(std::false_type{});
+        s.r += r[0] + r[1];
+        s.t += q[0] + q[1];
     }
     if (z != z) s.r = z;
     s = wave_join(s);
@@ -298,7 +308,7 @@ __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a, in
         o[0] = s.m;
         o[1] = s.r;
         o[2] = s.t;
-        o[3] = __int_as_float(n);
+        o[3] = __int_as_float(ok ? n : -1);
     }
 }
 
@@ -376,10 +386,14 @@ __device__ int merge(Best &best, FinishLds &sh, int wid, bool mine) {
     }
     if (tid == 0) sh.n = 0;
     __syncthreads();
-    uint64_t bound = 0;
     if (mine) {
-        for (int w = 0; w < FIN_WAVES; ++w)
-            if (sh.count[w] == k) bound = sh.buf[w][k - 1] > bound ? sh.buf[w][k - 1] : bound;
+        uint64_t bound = lane < FIN_WAVES && sh.count[lane] == k ? sh.buf[lane][k - 1] : 0;
+#pragma unroll
+        for (int o = 1; o < FIN_WAVES; o <<= 1) {
+            const uint64_t other = __shfl_xor((unsigned long long)bound, o);
+            bound = other > bound ? other : bound;
+        }
+        bound = from_lane(bound, 0);
         const bool take = lane < best.n && best.buf[lane] >= bound;
         const uint64_t m = __ballot(take);  // (lists are in order: a leading run)
         int at = 0;
@@ -396,7 +410,13 @@ __device__ int merge(Best &best, FinishLds &sh, int wid, bool mine) {
         for (int c = lane; c < n; c += 64) {
             const uint64_t key = sh.list[c];
             int r = 0;
-            for (int i = wid; i < n; i += FIN_WAVES) r += sh.list[i] > key;
+            for (int i = wid; i < n; i += 4 * FIN_WAVES) {
+                uint64_t o[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) o[u] = sh.list[min(i + u * FIN_WAVES, n - 1)];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) r += i + u * FIN_WAVES < n && o[u] > key;
+            }
             if (r) atomicAdd(&sh.rank[c], r);
         }
     }
@@ -420,11 +440,9 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
     const float nan = __builtin_nanf("");
     __shared__ float whole[2];
     if (wid == (TOP ? FIN_WAVES : 0)) {
-        const int t = a.tokens[row];
-        const bool ok = t >= 0 && t < a.V;
-        const float xt = ok ? logit<HALF>(x, t) : nan;
+        const float xt = a.logprob[row];  // the token's value, from the scan
         Sums s{-INFINITY, 0.0f, 0.0f};
-        int n = 0;
+        int n = 0;  // below 0: no such token
         for (int p = 0; p < a.parts; p += 64) {
             Sums q{-INFINITY, 0.0f, 0.0f};
             int c = 0;
@@ -446,7 +464,7 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
             whole[0] = s.m;
             whole[1] = logs;
             a.logprob[row] = (xt - s.m) - logs;
-            if (a.rank) a.rank[row] = ok ? n : -1;
+            if (a.rank) a.rank[row] = n < 0 ? -1 : n;
             if (a.entropy) a.entropy[row] = logs - LN2 * s.t / (1.0f + s.r);
         }
     }
@@ -465,19 +483,29 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
             // values below the k-th sub-chunk's maximum have k others ahead of them
             const uint64_t bound = chunks == a.k ? sh.out[a.k - 1] & ~0xFFFFFFFFull : 0;
             best = Best{sh.buf[wid], a.k, 0, 0};
-            for (int c = wid; c < chunks; c += FIN_WAVES) {
-                const int base = (int)index_of(sh.out[c]) * SUB - off;
-                u32x4 raw[PER];
+            constexpr int AHEAD = 4;  // sub-chunks under way
+            for (int c = wid; c < chunks; c += AHEAD * FIN_WAVES) {
+                u32x4 raw[AHEAD][PER];
+                int base[AHEAD];
 #pragma unroll
-                for (int u = 0; u < PER; ++u) raw[u] = read_piece<HALF>(x, base + (u * 64 + lane) * VEC, a.V, false);
+                for (int g = 0; g < AHEAD; ++g) {
+                    if (c + g * FIN_WAVES >= chunks) break;  // (uniform)
+                    base[g] = (int)index_of(sh.out[c + g * FIN_WAVES]) * SUB - off;
 #pragma unroll
-                for (int u = 0; u < PER; ++u)
+                    for (int u = 0; u < PER; ++u) raw[g][u] = read_piece<HALF>(x, base[g] + (u * 64 + lane) * VEC, a.V, false);
+                }
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
-                        const int i = base + (u * 64 + lane) * VEC + e;
-                        const uint64_t key = key_of(piece_value<HALF>(raw[u], e), i);
-                        best.push(key, key >= bound && i >= 0 && i < a.V);
-                    }
+                for (int g = 0; g < AHEAD; ++g) {
+                    if (c + g * FIN_WAVES >= chunks) break;
+#pragma unroll
+                    for (int u = 0; u < PER; ++u)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) {
+                            const int i = base[g] + (u * 64 + lane) * VEC + e;
+                            const uint64_t key = key_of(piece_value<HALF>(raw[g][u], e), i);
+                            best.push(key, key >= bound && i >= 0 && i < a.V);
+                        }
+                }
             }
         }
         merge(best, sh, wid, mine);

@@ -306,19 +306,25 @@ def token_logprobs(logits, tokens, top_k=0, workspace=None, stream=None):
     the top_k best alternatives, from logits [M, V] (fp32 or fp16, rows may be
     views of wider ones): a TokenLogprobs. Larger values come first, equal ones
     by index; a token outside of [0, V) gives NaN and rank -1."""
-    torch = _torch()
-    from .attention import _device, _empty, _rows, _vec
-    dev, f32, i32 = _device(), torch.float32, torch.int32
+    from .attention import _device, _empty, _raw_stream, _rows, _vec
+    torch, dev = _device()
+    f32, i32 = torch.float32, torch.int32
     ld = _rows(logits, (f32, torch.float16), "logits", dev)
     M, V = logits.shape
     _vec(tokens, i32, M, "tokens", dev)
-    k = max(top_k, 0)
-    lp, ent, top = (_empty(logits, stream, *n, dtype=f32) for n in ((M,), (M,), (M, k)))
-    rank, ids = _empty(tokens, stream, M), _empty(tokens, stream, M, k)
+    k = top_k if top_k > 0 else 0
+    if stream is None:
+        lp, ent, top = tokens.new_empty(M, dtype=f32), tokens.new_empty(M, dtype=f32), tokens.new_empty(M, k, dtype=f32)
+        rank, ids = tokens.new_empty(M), tokens.new_empty(M, k)
+    else:
+        lp, ent, top = (_empty(tokens, stream, *n, dtype=f32) for n in ((M,), (M,), (M, k)))
+        rank, ids = _empty(tokens, stream, M), _empty(tokens, stream, M, k)
     wp, wb = _ws(workspace)
-    _check(lib().q3vl_token_logprobs(logits.data_ptr(), ld, FP16 if logits.dtype is torch.float16 else FP32, tokens.data_ptr(),
-                                     M, V, top_k, lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(),
-                                     wp, wb, _stream(stream)))
+    rc = lib().q3vl_token_logprobs(logits.data_ptr(), ld, FP32 if logits.dtype is f32 else FP16, tokens.data_ptr(), M, V, top_k,
+                                   lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), wp, wb,
+                                   _raw_stream(stream, torch, dev))
+    if rc:
+        _check(rc)
     return TokenLogprobs(lp, rank, ent, ids, top)
 
 

@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import FP16, FP32, _check, _need, _ptr, _stream, _torch, _ws, lib
+from . import FP16, FP32, _check, _need, _ptr, _torch, _ws, lib
 
 _sz = ctypes.c_size_t
 _vp = ctypes.c_void_p
@@ -37,11 +37,11 @@ class _RopeC(ctypes.Structure):
     _fields_ = [("cos", _vp), ("sin", _vp), ("rows", _i), ("axes", _i), ("sections", _i * 3), ("interleaved", _i)]
 
 
-_lib = None
+_lib = _plan_fn = _rope_fn = _attn_fn = None
 
 
 def _L():
-    global _lib
+    global _lib, _plan_fn, _rope_fn, _attn_fn
     if _lib is None:
         L = lib()
         sigs = {
@@ -54,18 +54,25 @@ def _L():
         for name, (res, args) in sigs.items():
             fn = getattr(L, name)
             fn.restype, fn.argtypes = res, args
+        _plan_fn, _rope_fn, _attn_fn = L.q3vl_draft_plan, L.q3vl_qk_norm_rope, L.q3vl_tree_attention
         _lib = L
     return _lib
 
 
-# A call costs 4 to 6 us in the library (its launches), so the checks around it
+# A call costs 3 to 6 us in the library (its launches), so the checks around it
 # are kept short, as the linears' are: the usual tensor passes in one
 # expression and only another one is looked at again for its error.
 def _device():
+    """(torch, the current device's index)"""
+    torch = _torch()
     try:
-        return _torch()._C._cuda_getDevice()
+        return torch, torch._C._cuda_getDevice()
     except RuntimeError:  # no device at all
-        return -2
+        return torch, -2
+
+
+def _raw_stream(stream, torch, dev):
+    return torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
 
 
 def _here(t, name, dev):
@@ -80,7 +87,7 @@ def _rows(t, dtypes, name, dev):
     if isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype in dtypes and t.dim() == 2:
         n, m = t.shape
         s, u = t.stride()
-        if u == 1 and s >= m:
+        if s >= m and u == 1:
             return s
         if (u == 1 or m <= 1) and (s >= m or n <= 1):
             return max(s, m)
@@ -94,9 +101,14 @@ def _rows(t, dtypes, name, dev):
     raise ValueError(f"{name} must be 2-d with contiguous rows")
 
 
+def _is_vec(t, dtype, dev):
+    return isinstance(t, _torch().Tensor) and t.get_device() == dev and t.dtype is dtype and t.is_contiguous()
+
+
 def _vec(t, dtype, n, name, dev):
-    """A contiguous device tensor of n values (None: any number)."""
-    if isinstance(t, _torch().Tensor) and t.get_device() == dev and t.dtype is dtype and t.is_contiguous() and (n is None or t.numel() == n):
+    """Refuses what is not a contiguous device tensor of n values (None: any
+    number). Callers ask _is_vec first."""
+    if _is_vec(t, dtype, dev) and (n is None or t.numel() == n):
         return
     _need(t, dtype, name)
     _here(t, name, dev)
@@ -204,12 +216,16 @@ def draft_plan(parents, row_start, cache_len, max_seq, max_rows, pos_delta=None,
     int32 [rows] and slots int64 [rows]. Rows behind the last sequence get
     position and slot -1, rows that cannot be planned (a bad parent, no room in
     the cache, past max_rows) position -2 and slot -1."""
-    torch = _torch()
-    dev, i32 = _device(), torch.int32
-    _vec(parents, i32, None, "parents", dev)
-    _vec(cache_len, i32, None, "cache_len", dev)
+    torch, dev = _device()
+    i32, T = torch.int32, torch.Tensor
+    if not (isinstance(parents, T) and parents.dtype is i32 and parents.get_device() == dev and parents.is_contiguous()):
+        _vec(parents, i32, None, "parents", dev)
+    if not (isinstance(cache_len, T) and cache_len.dtype is i32 and cache_len.get_device() == dev and cache_len.is_contiguous()):
+        _vec(cache_len, i32, None, "cache_len", dev)
     rows, batch = parents.numel(), cache_len.numel()
-    _vec(row_start, i32, batch + 1, "row_start", dev)
+    if not (isinstance(row_start, T) and row_start.dtype is i32 and row_start.get_device() == dev and row_start.is_contiguous()
+            and row_start.numel() == batch + 1):
+        _vec(row_start, i32, batch + 1, "row_start", dev)
     if pos_delta is not None:
         _vec(pos_delta, i32, batch, "pos_delta", dev)
     if mask is None:
@@ -225,8 +241,11 @@ def draft_plan(parents, row_start, cache_len, max_seq, max_rows, pos_delta=None,
         slots = _empty(parents, stream, rows, dtype=torch.int64)
     else:
         _vec(slots, torch.int64, rows, "slots", dev)
-    _check(_L().q3vl_draft_plan(parents.data_ptr(), row_start.data_ptr(), cache_len.data_ptr(), _ptr(pos_delta), batch, rows,
-                                max_rows, max_seq, mask.data_ptr(), words, pos.data_ptr(), slots.data_ptr(), _stream(stream)))
+    rc = (_plan_fn or _L().q3vl_draft_plan)(
+        parents.data_ptr(), row_start.data_ptr(), cache_len.data_ptr(), _ptr(pos_delta), batch, rows, max_rows, max_seq,
+        mask.data_ptr(), words, pos.data_ptr(), slots.data_ptr(), _raw_stream(stream, torch, dev))
+    if rc:
+        _check(rc)
     return mask, pos, slots
 
 
@@ -238,8 +257,8 @@ def qk_norm_rope(q, k, v, cache, slots, pos, norm, rope, out=None, out_dtype=Non
     names (batch index * max_seq + row; another value: not stored). pos int32
     [rows], or [rows, 3] under a Rope with sections. Rows at position -1 hold
     no token and are left alone; out may be q."""
-    torch = _torch()
-    dev, f32 = _device(), (torch.float32,)
+    torch, dev = _device()
+    f32 = (torch.float32,)
     ldq, ldk, ldv = _rows(q, f32, "q", dev), _rows(k, f32, "k", dev), _rows(v, f32, "v", dev)
     c = cache.c
     D = c.head_dim
@@ -259,9 +278,12 @@ def qk_norm_rope(q, k, v, cache, slots, pos, norm, rope, out=None, out_dtype=Non
         raise ValueError("out must have q's shape")
     _vec(slots, torch.int64, rows, "slots", dev)
     _vec(pos, torch.int32, rows * rope.axes, "pos", dev)
-    _check(_L().q3vl_qk_norm_rope(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
-                                  FP16 if out.dtype is torch.float16 else FP32, rows, qn // D, cache.ref, slots.data_ptr(),
-                                  pos.data_ptr(), norm.ref, rope.ref, _stream(stream)))
+    rc = (_rope_fn or _L().q3vl_qk_norm_rope)(
+        q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, out.data_ptr(), ldo,
+        FP16 if out.dtype is torch.float16 else FP32, rows, qn // D, cache.ref, slots.data_ptr(), pos.data_ptr(), norm.ref,
+        rope.ref, _raw_stream(stream, torch, dev))
+    if rc:
+        _check(rc)
     return out
 
 
@@ -288,8 +310,7 @@ def tree_attention(q, cache, row_start, cache_len, max_rows, mask=None, max_len=
     default 1 / sqrt(head_dim). out may be q. A row that sees nothing gives 0.
     workspace: alloc_tree_attention_workspace with the same max_rows and
     max_len."""
-    torch = _torch()
-    dev = _device()
+    torch, dev = _device()
     ldq = _rows(q, (torch.float32, torch.float16), "q", dev)
     c = cache.c
     D, batch = c.head_dim, c.batch
@@ -309,7 +330,10 @@ def tree_attention(q, cache, row_start, cache_len, max_rows, mask=None, max_len=
     _vec(cache_len, torch.int32, batch, "cache_len", dev)
     words = 0 if mask is None else _mask_words(mask, rows, dev)
     wp, wb = _ws(workspace)
-    _check(_L().q3vl_tree_attention(q.data_ptr(), ldq, out.data_ptr(), ldo, FP16 if q.dtype is torch.float16 else FP32, rows,
-                                    qn // D, cache.ref, row_start.data_ptr(), cache_len.data_ptr(), _ptr(mask), words,
-                                    max_rows, max_len or 0, D ** -0.5 if scale is None else scale, wp, wb, _stream(stream)))
+    rc = (_attn_fn or _L().q3vl_tree_attention)(
+        q.data_ptr(), ldq, out.data_ptr(), ldo, FP16 if q.dtype is torch.float16 else FP32, rows, qn // D, cache.ref,
+        row_start.data_ptr(), cache_len.data_ptr(), _ptr(mask), words, max_rows, max_len or 0,
+        D ** -0.5 if scale is None else scale, wp, wb, _raw_stream(stream, torch, dev))
+    if rc:
+        _check(rc)
     return out

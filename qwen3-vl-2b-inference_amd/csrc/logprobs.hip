@@ -168,7 +168,14 @@ template <bool HALF> __device__ __forceinline__ int row_offset(const void *x) {
 // About 15 VALU instructions a value, 4 of them the exponential, against 10
 // bytes a clock that HBM has for a CU.
 template <bool HALF>
-__global__ __launch_bounds__(THREADS) void logprob_scan_kernel(LogprobArgs a, int subs_max) {
+__global__ __launch_bounds__(THREADS) void logprob_scan_kernel(const void *logits_p, int64_t ld_p, const int32_t *tokens_p,
+                                                              int parts_p, int V_p, int subs_max, LogprobArgs args) {
+    LogprobArgs a = args;  // (the leading arguments arrive in registers)
+    a.logits = logits_p;
+    a.ld = ld_p;
+    a.tokens = tokens_p;
+    a.parts = parts_p;
+    a.V = V_p;
     constexpr int VEC = HALF ? 8 : 4, U = 16 / VEC;  // values a load, loads a turn
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts, tid = threadIdx.x, lane = tid & 63;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -431,7 +438,16 @@ __device__ int merge(Best &best, FinishLds &sh, int wid, bool mine) {
 // One block a row: a wave joins the parts' sums; eight others (TOP) find the
 // alternatives.
 template <bool HALF, bool TOP>
-__global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finish_kernel(LogprobArgs a, int subs_max) {
+__global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finish_kernel(
+    const void *logits_p, int64_t ld_p, const float *sub_max_p, const float *part_p, float *logprob_p, int parts_p, int V_p,
+    int k_p, int subs_max, LogprobArgs args) {
+    LogprobArgs a = args;
+    a.logits = logits_p;
+    a.ld = ld_p;
+    a.logprob = logprob_p;
+    a.parts = parts_p;
+    a.V = V_p;
+    a.k = k_p;
     constexpr int VEC = HALF ? 8 : 4, PER = SUB / (64 * VEC);
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -447,7 +463,7 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
             Sums q{-INFINITY, 0.0f, 0.0f};
             int c = 0;
             if (p + lane < a.parts) {
-                const float4_t o = *reinterpret_cast<const float4_t *>(a.part + ((size_t)row * a.parts + p + lane) * 4);
+                const float4_t o = *reinterpret_cast<const float4_t *>(part_p + ((size_t)row * a.parts + p + lane) * 4);
                 q = Sums{o[0], o[1], o[2]};
                 c = __float_as_int(o[3]);
             }
@@ -476,13 +492,16 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
         if (mine)
             for (int c = wid * 64; c < subs; c += 64 * FIN_WAVES) {
                 const int i = c + lane;
-                best.push(i < subs ? key_of(a.sub_max[(size_t)row * subs_max + i], i) : 0, i < subs);
+                best.push(i < subs ? key_of(sub_max_p[(size_t)row * subs_max + i], i) : 0, i < subs);
             }
         const int chunks = merge(best, sh, wid, mine);
         if (mine) {
             // values below the k-th sub-chunk's maximum have k others ahead of them
             const uint64_t bound = chunks == a.k ? sh.out[a.k - 1] & ~0xFFFFFFFFull : 0;
             best = Best{sh.buf[wid], a.k, 0, 0};
+            // (one float comparison a value first: few values pass. -inf: all do)
+            const float least = bound ? value_of(bound) : -INFINITY;
+            const bool all = !(least > -INFINITY);
             constexpr int AHEAD = 4;  // sub-chunks under way
             for (int c = wid; c < chunks; c += AHEAD * FIN_WAVES) {
                 u32x4 raw[AHEAD][PER];
@@ -501,8 +520,10 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
                     for (int u = 0; u < PER; ++u)
 #pragma unroll
                         for (int e = 0; e < VEC; ++e) {
+                            const float v = piece_value<HALF>(raw[g][u], e);
+                            if (!__any(all || v >= least)) continue;
                             const int i = base[g] + (u * 64 + lane) * VEC + e;
-                            const uint64_t key = key_of(piece_value<HALF>(raw[g][u], e), i);
+                            const uint64_t key = key_of(v, i);
                             best.push(key, key >= bound && i >= 0 && i < a.V);
                         }
                 }
@@ -517,21 +538,22 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
     }
 }
 
-hipError_t launch_token_logprobs(const LogprobArgs &a, bool half, hipStream_t st) {
-    const unsigned grid = (unsigned)a.parts * (unsigned)a.M;
+template <bool HALF> static hipError_t launch_half(const LogprobArgs &a, hipStream_t st) {
     const int subs = logprob_subs(a.V);
-    if (half) logprob_scan_kernel<true><<<grid, THREADS, 0, st>>>(a, subs);
-    else logprob_scan_kernel<false><<<grid, THREADS, 0, st>>>(a, subs);
+    logprob_scan_kernel<HALF><<<(unsigned)a.parts * (unsigned)a.M, THREADS, 0, st>>>(a.logits, a.ld, a.tokens, a.parts, a.V, subs, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.k) {
-        if (half) logprob_finish_kernel<true, true><<<a.M, 64 * (FIN_WAVES + 1), 0, st>>>(a, subs);
-        else logprob_finish_kernel<false, true><<<a.M, 64 * (FIN_WAVES + 1), 0, st>>>(a, subs);
-    } else {
-        if (half) logprob_finish_kernel<true, false><<<a.M, 64, 0, st>>>(a, subs);
-        else logprob_finish_kernel<false, false><<<a.M, 64, 0, st>>>(a, subs);
-    }
+    if (a.k)
+        logprob_finish_kernel<HALF, true><<<a.M, 64 * (FIN_WAVES + 1), 0, st>>>(a.logits, a.ld, a.sub_max, a.part, a.logprob,
+                                                                               a.parts, a.V, a.k, subs, a);
+    else
+        logprob_finish_kernel<HALF, false><<<a.M, 64, 0, st>>>(a.logits, a.ld, a.sub_max, a.part, a.logprob, a.parts, a.V, a.k,
+                                                              subs, a);
     return hipGetLastError();
+}
+
+hipError_t launch_token_logprobs(const LogprobArgs &a, bool half, hipStream_t st) {
+    return half ? launch_half<true>(a, st) : launch_half<false>(a, st);
 }
 
 }  // namespace q3vl

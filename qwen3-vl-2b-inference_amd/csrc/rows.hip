@@ -135,7 +135,19 @@ typedef uint16_t h4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint16_t h4_row __attribute__((ext_vector_type(4)));
 
 template <int D, bool HALF, bool AXES3>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkRopeArgs a) {
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(const float *q_p, const float *k_p, const float *v_p,
+                                                           const int32_t *pos_p, const int64_t *slots_p, int heads_p,
+                                                           int kv_heads_p, int gs_p, int rows_p, QkRopeArgs args) {
+    QkRopeArgs a = args;  // (the leading arguments arrive in registers)
+    a.q = q_p;
+    a.k = k_p;
+    a.v = v_p;
+    a.pos = pos_p;
+    a.slots = slots_p;
+    a.heads = heads_p;
+    a.kv_heads = kv_heads_p;
+    a.gs = gs_p;
+    a.rows = rows_p;
     constexpr int Q = D / 16, QH = Q / 2;
     __shared__ __align__(16) float wsh[2][D], ssh[2][D];  // norm weights and their scales, q and k
     const int lane = threadIdx.x & 63, j = lane & 3;
@@ -272,7 +284,7 @@ hipError_t launch_qk_norm_rope(const QkRopeArgs &a, int head_dim, bool half, int
     const int64_t per_row = (a.heads + 2 * a.kv_heads + 15) / 16, blocks = (a.rows * per_row + 3) / 4;
     const unsigned grid = (unsigned)(blocks < 2048 ? blocks : 2048);  // eight a CU, each its share
     auto go = [&](auto kernel) {
-        kernel<<<grid, 256, 0, st>>>(a);
+        kernel<<<grid, 256, 0, st>>>(a.q, a.k, a.v, a.pos, a.slots, a.heads, a.kv_heads, a.gs, (int)a.rows, a);
         return hipGetLastError();
     };
     if (head_dim == 128) {

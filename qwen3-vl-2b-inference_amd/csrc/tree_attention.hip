@@ -214,8 +214,22 @@ __device__ __forceinline__ uint32_t mask_window(const uint64_t *line, int words,
     return i < 0 ? (uint32_t)(v << -i) | ((1u << -i) - 1) : (uint32_t)v;
 }
 
+// (What the first loads need comes as plain leading arguments, which arrive in
+// registers; the rest is read from the struct beside those loads.)
 template <int D, bool HALF, int NR, bool SHARED>
-__global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(TreeAttnArgs a, int tiles, bool paired) {
+__global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(
+    const int32_t *row_start_p, const int32_t *cache_len_p, const void *q_p, int kv_heads_p, int heads_p, int splits_p, int rows_p,
+    int max_rows_p, int max_seq_p, int tiles, int paired, TreeAttnArgs args) {
+    TreeAttnArgs a = args;
+    a.row_start = row_start_p;
+    a.cache_len = cache_len_p;
+    a.q = q_p;
+    a.kv_heads = kv_heads_p;
+    a.heads = heads_p;
+    a.splits = splits_p;
+    a.rows = rows_p;
+    a.max_rows = max_rows_p;
+    a.max_seq = max_seq_p;
     using T = Tile<D, NR, SHARED>;
     constexpr int KS = D / 32, NT = D / 16, NQ = HALF ? 1 : 2;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -651,7 +665,19 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
 
 // Joins a row's splits: one wave a (row, query head), four values a lane, 64 /
 // (D / 4) splits side by side and four such loads under way.
-template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join_kernel(TreeAttnArgs a) {
+template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join_kernel(const int32_t *row_start_p, const int32_t *cache_len_p,
+                                                            const float *part_ml_p, const float *part_o_p, int heads_p,
+                                                            int splits_p, int rows_p, int max_rows_p, int max_seq_p, int batch_p,
+                                                            TreeAttnArgs args) {
+    TreeAttnArgs a = args;
+    a.row_start = row_start_p;
+    a.cache_len = cache_len_p;
+    a.heads = heads_p;
+    a.splits = splits_p;
+    a.rows = rows_p;
+    a.max_rows = max_rows_p;
+    a.max_seq = max_seq_p;
+    a.batch = batch_p;
     constexpr int LANES = D / 4, SIDE = 64 / LANES;
     const int lane = threadIdx.x & 63, d = lane % LANES * 4, side = lane / LANES;
     const int x = blockIdx.x * WAVES + (threadIdx.x >> 6);
@@ -664,8 +690,8 @@ template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join
     if (s.ok) {
         float m = -INFINITY, lw = 0.0f;
         if (lane < a.splits) {
-            m = a.part_ml[(part + lane) * 2];
-            lw = a.part_ml[(part + lane) * 2 + 1];
+            m = part_ml_p[(part + lane) * 2];
+            lw = part_ml_p[(part + lane) * 2 + 1];
         }
         float top = m;
 #pragma unroll
@@ -674,7 +700,7 @@ template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join
         lw *= f;
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) lw += __shfl_xor(lw, k);
-        const float *p = a.part_o + part * D + d;
+        const float *p = part_o_p + part * D + d;
         for (int k = 0; k < a.splits; k += 4 * SIDE) {
             float4_t v[4];
 #pragma unroll
@@ -794,7 +820,8 @@ template <int D, bool HALF, int NR, bool SHARED> static hipError_t launch_tile(c
     const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
     const hipError_t e = allow_lds<&tree_attention_kernel<D, HALF, NR, SHARED>>(T::LDS);
     if (e != hipSuccess) return e;
-    tree_attention_kernel<D, HALF, NR, SHARED><<<grid, THREADS, T::LDS, st>>>(a, tiles, grid <= 512);
+    tree_attention_kernel<D, HALF, NR, SHARED><<<grid, THREADS, T::LDS, st>>>(
+        a.row_start, a.cache_len, a.q, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, grid <= 512, a);
     return hipGetLastError();
 }
 
@@ -806,7 +833,8 @@ template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, in
     else e = launch_tile<D, HALF, 2, true>(a, st);
     if (e != hipSuccess || a.splits == 1) return e;
     const unsigned waves = (unsigned)a.batch * a.max_rows * a.heads;
-    tree_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(a);
+    tree_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(
+        a.row_start, a.cache_len, a.part_ml, a.part_o, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, a.batch, a);
     return hipGetLastError();
 }
 

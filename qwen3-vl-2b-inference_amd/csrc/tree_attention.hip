@@ -312,7 +312,9 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         left = min(left, SHARED ? 64 : 32);
         const rsrc_t r = make_rsrc(p, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
 #pragma unroll
-        for (int t = 0; t < NL; ++t) dma16(r, voff[t], 0, lds + ((SHARED ? wid * NL : 0) + t) * 1024);
+        for (int t = 0; t < NL; ++t)
+            if constexpr (SHARED) dma16(r, voff[t], 0, lds + (wid * NL + t) * 1024);
+            else dma16_nt(r, voff[t], 0, lds + t * 1024);
     };
     const size_t first_at = head_at + (size_t)(j0 + (SHARED ? 0 : wid * 32)) * a.row_stride, turn = (size_t)T::UNIT * a.row_stride;
     const uint16_t *kp = a.k_cache + first_at, *vp = a.v_cache + first_at;  // of the next loads

@@ -137,7 +137,7 @@ int logprob_parts(int M, int V) {
 template <bool HALF> __device__ __forceinline__ u32x4 read_piece(const void *x, int i, int V, bool inside) {
     constexpr int VEC = HALF ? 8 : 4;
     const unsigned char *p = static_cast<const unsigned char *>(x) + (int64_t)i * (HALF ? 2 : 4);
-    if (inside || (i >= 0 && i + VEC <= V)) return *reinterpret_cast<const u32x4 *>(p);
+    if (inside || (i >= 0 && i + VEC <= V)) return __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p));
     u32x4 r;
     if constexpr (HALF) {
 #pragma unroll

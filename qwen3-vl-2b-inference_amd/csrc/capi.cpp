@@ -1609,6 +1609,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     a.max_rows = (size_t)max_rows > rows ? (int)rows : max_rows;
     a.words = mask_words;
     a.splits = plan.splits;
+    a.max_len = max_len && max_len < cache->max_seq ? max_len : cache->max_seq;
     a.scale_log2e = (float)((double)scale * 1.4426950408889634);
     Q3VL_HIP(launch_tree_attention(a, cache->head_dim, half, plan.rows, (hipStream_t)stream), "attention launch");
     return Q3VL_OK;

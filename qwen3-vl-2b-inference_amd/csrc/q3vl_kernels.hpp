@@ -221,6 +221,7 @@ struct TreeAttnArgs {
     float *part_o;         // splits > 1: [rows * heads][splits][head_dim]
     float *part_ml;        //             [rows * heads][splits][2]
     int rows, heads, kv_heads, batch, max_seq, max_rows, words, splits;
+    int max_len;           // the most positions of a sequence, as the caller says
     float scale_log2e;     // scale / ln 2
 };
 struct TreePlan {

@@ -214,12 +214,17 @@ __device__ __forceinline__ uint32_t mask_window(const uint64_t *line, int words,
     return i < 0 ? (uint32_t)(v << -i) | ((1u << -i) - 1) : (uint32_t)v;
 }
 
+enum : int {
+    PAIRED = 1,     // every block has a place at once
+    READ_ONCE = 2,  // shared tiles: no other block reads them, and together they are more than the caches keep
+};
+
 // (What the first loads need comes as plain leading arguments, which arrive in
 // registers; the rest is read from the struct beside those loads.)
 template <int D, bool HALF, int NR, bool SHARED>
 __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(
     const int32_t *row_start_p, const int32_t *cache_len_p, const void *q_p, int kv_heads_p, int heads_p, int splits_p, int rows_p,
-    int max_rows_p, int max_seq_p, int tiles, int paired, TreeAttnArgs args) {
+    int max_rows_p, int max_seq_p, int tiles, int flags, TreeAttnArgs args) {
     TreeAttnArgs a = args;
     a.row_start = row_start_p;
     a.cache_len = cache_len_p;
@@ -245,7 +250,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     // a chain's last rows see most: they go first, and where every block has a
     // place at once (two a CU, the second half of them beside the first), the
     // second half goes the other way round
-    const int tile = paired && 2 * x >= tiles ? x - (tiles + 1) / 2 : tiles - 1 - x;
+    const int tile = (flags & PAIRED) && 2 * x >= tiles ? x - (tiles + 1) / 2 : tiles - 1 - x;
     const Seq s = sequence(a, b);
     const int group = a.heads / a.kv_heads;
     const int n = min(s.n, a.max_rows), nrows = n * group, r0 = tile * T::BM;
@@ -313,8 +318,8 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         const rsrc_t r = make_rsrc(p, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
 #pragma unroll
         for (int t = 0; t < NL; ++t)
-            if constexpr (SHARED) dma16(r, voff[t], 0, lds + (wid * NL + t) * 1024);
-            else dma16_nt(r, voff[t], 0, lds + t * 1024);
+            if (SHARED && !(flags & READ_ONCE)) dma16(r, voff[t], 0, lds + (wid * NL + t) * 1024);
+            else dma16_nt(r, voff[t], 0, lds + ((SHARED ? wid * NL : 0) + t) * 1024);
     };
     const size_t first_at = head_at + (size_t)(j0 + (SHARED ? 0 : wid * 32)) * a.row_stride, turn = (size_t)T::UNIT * a.row_stride;
     const uint16_t *kp = a.k_cache + first_at, *vp = a.v_cache + first_at;  // of the next loads
@@ -822,8 +827,14 @@ template <int D, bool HALF, int NR, bool SHARED> static hipError_t launch_tile(c
     const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
     const hipError_t e = allow_lds<&tree_attention_kernel<D, HALF, NR, SHARED>>(T::LDS);
     if (e != hipSuccess) return e;
+    // Keys and values that one block reads once go past the caches (always with
+    // few rows): 30 trees of 20 over 6000, 369 MB, fp16: 145 us through them, 128
+    // past them; 8 of 40 over 8000, 263 MB: 64.5 and 59.8 (fp32 75.6 and 77.3); but
+    // 1 of 64 over 16000, 66 MB: 28.0 and 30.7.
+    const double held = (double)a.batch * a.kv_heads * a.max_len * D * 4;
+    const int flags = (grid <= 512 ? PAIRED : 0) | (tiles == 1 && held > 192e6 ? READ_ONCE : 0);
     tree_attention_kernel<D, HALF, NR, SHARED><<<grid, THREADS, T::LDS, st>>>(
-        a.row_start, a.cache_len, a.q, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, grid <= 512, a);
+        a.row_start, a.cache_len, a.q, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, flags, a);
     return hipGetLastError();
 }
 

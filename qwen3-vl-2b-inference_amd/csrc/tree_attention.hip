@@ -214,17 +214,13 @@ __device__ __forceinline__ uint32_t mask_window(const uint64_t *line, int words,
     return i < 0 ? (uint32_t)(v << -i) | ((1u << -i) - 1) : (uint32_t)v;
 }
 
-enum : int {
-    PAIRED = 1,     // every block has a place at once
-    READ_ONCE = 2,  // shared tiles: no other block reads them, and together they are more than the caches keep
-};
-
+// ONCE: no other block reads this one's keys and values; they go past the caches.
 // (What the first loads need comes as plain leading arguments, which arrive in
 // registers; the rest is read from the struct beside those loads.)
-template <int D, bool HALF, int NR, bool SHARED>
+template <int D, bool HALF, int NR, bool SHARED, bool ONCE>
 __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel(
     const int32_t *row_start_p, const int32_t *cache_len_p, const void *q_p, int kv_heads_p, int heads_p, int splits_p, int rows_p,
-    int max_rows_p, int max_seq_p, int tiles, int flags, TreeAttnArgs args) {
+    int max_rows_p, int max_seq_p, int tiles, int paired, TreeAttnArgs args) {
     TreeAttnArgs a = args;
     a.row_start = row_start_p;
     a.cache_len = cache_len_p;
@@ -250,7 +246,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
     // a chain's last rows see most: they go first, and where every block has a
     // place at once (two a CU, the second half of them beside the first), the
     // second half goes the other way round
-    const int tile = (flags & PAIRED) && 2 * x >= tiles ? x - (tiles + 1) / 2 : tiles - 1 - x;
+    const int tile = paired && 2 * x >= tiles ? x - (tiles + 1) / 2 : tiles - 1 - x;
     const Seq s = sequence(a, b);
     const int group = a.heads / a.kv_heads;
     const int n = min(s.n, a.max_rows), nrows = n * group, r0 = tile * T::BM;
@@ -317,9 +313,11 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         left = min(left, SHARED ? 64 : 32);
         const rsrc_t r = make_rsrc(p, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
 #pragma unroll
-        for (int t = 0; t < NL; ++t)
-            if (SHARED && !(flags & READ_ONCE)) dma16(r, voff[t], 0, lds + (wid * NL + t) * 1024);
-            else dma16_nt(r, voff[t], 0, lds + ((SHARED ? wid * NL : 0) + t) * 1024);
+        for (int t = 0; t < NL; ++t) {
+            const int at = lds + ((SHARED ? wid * NL : 0) + t) * 1024;
+            if constexpr (ONCE) dma16_nt(r, voff[t], 0, at);
+            else dma16(r, voff[t], 0, at);
+        }
     };
     const size_t first_at = head_at + (size_t)(j0 + (SHARED ? 0 : wid * 32)) * a.row_stride, turn = (size_t)T::UNIT * a.row_stride;
     const uint16_t *kp = a.k_cache + first_at, *vp = a.v_cache + first_at;  // of the next loads
@@ -821,29 +819,29 @@ template <auto Kernel> static hipError_t allow_lds(int bytes) {
     return e;
 }
 
-template <int D, bool HALF, int NR, bool SHARED> static hipError_t launch_tile(const TreeAttnArgs &a, hipStream_t st) {
+template <int D, bool HALF, int NR, bool SHARED, bool ONCE> static hipError_t launch_tile(const TreeAttnArgs &a, int tiles, hipStream_t st) {
     using T = Tile<D, NR, SHARED>;
-    const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + T::BM - 1) / T::BM);
     const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
-    const hipError_t e = allow_lds<&tree_attention_kernel<D, HALF, NR, SHARED>>(T::LDS);
+    const hipError_t e = allow_lds<&tree_attention_kernel<D, HALF, NR, SHARED, ONCE>>(T::LDS);
     if (e != hipSuccess) return e;
-    // Keys and values that one block reads once go past the caches (always with
-    // few rows): 30 trees of 20 over 6000, 369 MB, fp16: 145 us through them, 128
-    // past them; 8 of 40 over 8000, 263 MB: 64.5 and 59.8 (fp32 75.6 and 77.3); but
-    // 1 of 64 over 16000, 66 MB: 28.0 and 30.7.
-    const double held = (double)a.batch * a.kv_heads * a.max_len * D * 4;
-    const int flags = (grid <= 512 ? PAIRED : 0) | (tiles == 1 && held > 192e6 ? READ_ONCE : 0);
-    tree_attention_kernel<D, HALF, NR, SHARED><<<grid, THREADS, T::LDS, st>>>(
-        a.row_start, a.cache_len, a.q, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, flags, a);
+    tree_attention_kernel<D, HALF, NR, SHARED, ONCE><<<grid, THREADS, T::LDS, st>>>(
+        a.row_start, a.cache_len, a.q, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, grid <= 512, a);
     return hipGetLastError();
 }
 
 template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, int bm, hipStream_t st) {
+    const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
+    // Keys and values that one block reads once go past the caches: always with few
+    // rows; of shared tiles where together they are more than the caches keep
+    // (us, through them and past them: 30 trees of 20 over 6000, 369 MB, fp16: 145
+    // and 128; 8 of 40 over 8000, 263 MB: 64 and 59.5, fp32 79.5 and 77.5; but 1 of
+    // 64 over 16000, 66 MB: 28.0 and 30.7).
+    const bool once = tiles == 1 && (double)a.batch * a.kv_heads * a.max_len * D * 4 > 192e6;
     hipError_t e;
-    if (bm == 16) e = launch_tile<D, HALF, 1, false>(a, st);
-    else if (bm == 32) e = launch_tile<D, HALF, 2, false>(a, st);
-    else if (bm == 64) e = launch_tile<D, HALF, 1, true>(a, st);
-    else e = launch_tile<D, HALF, 2, true>(a, st);
+    if (bm == 16) e = launch_tile<D, HALF, 1, false, true>(a, tiles, st);
+    else if (bm == 32) e = launch_tile<D, HALF, 2, false, true>(a, tiles, st);
+    else if (bm == 64) e = once ? launch_tile<D, HALF, 1, true, true>(a, tiles, st) : launch_tile<D, HALF, 1, true, false>(a, tiles, st);
+    else e = once ? launch_tile<D, HALF, 2, true, true>(a, tiles, st) : launch_tile<D, HALF, 2, true, false>(a, tiles, st);
     if (e != hipSuccess || a.splits == 1) return e;
     const unsigned waves = (unsigned)a.batch * a.max_rows * a.heads;
     tree_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(

@@ -40,4 +40,4 @@ def test_attention_reloads_read_slots_only(code):  # noqa: F811
         worst = outstanding(main_loop(ins), is_load)
         assert worst and max(worst) == 0, f"{name}: {worst} reads not waited for"
         seen += 1
-    assert seen == 16  # head sizes, types, four tiles
+    assert seen == 24  # head sizes, types, four tiles, the shared ones through and past the caches

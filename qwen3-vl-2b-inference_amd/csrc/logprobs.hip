@@ -362,13 +362,21 @@ struct Best {
             floor = last > floor ? last : floor;
         }
     }
+    // A sort each time that 32 came after the k kept ones, or else each value
+    // taken up would cost one where k is 64; before that where a push might not fit.
     __device__ __forceinline__ void push(uint64_t key, bool take) {
         take = take && key > floor;
-        const uint64_t m = __ballot(take);
+        uint64_t m = __ballot(take);
         if (!m) return;
+        if (n + __builtin_popcountll(m) > 128) {
+            sort();
+            take = take && key > floor;
+            m = __ballot(take);
+            if (!m) return;
+        }
         if (take) buf[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0))] = key;
         n += __builtin_popcountll(m);
-        if (n > 64 || (n == 64 && k <= 32)) sort();
+        if (n >= 64 && n - k >= 32) sort();
     }
 };
 

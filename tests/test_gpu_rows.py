@@ -539,6 +539,15 @@ def test_logprobs_ties():
     check_logprobs(x.astype(np.float16), [4000, 0, 4, 2501, 0, 64], 64)
 
 
+@pytest.mark.parametrize("k", [1, 31, 32, 33, 40, 63, 64])
+def test_logprobs_rising_rows(k):
+    """Rows whose values rise, so that each one read is among the best so far:
+    the lists of alternatives are full at every turn."""
+    for V, n in ((1500, 1), (9000, 3), (34000, 2)):
+        x = np.stack([np.linspace(-9, 9, V), -np.linspace(-9, 9, V), np.roll(np.linspace(-9, 9, V), V // 2)])[:n].astype(np.float32)
+        check_logprobs(x, [V - 1, 0, V // 3][:n], k)
+
+
 def test_logprobs_ruled_out_values():
     """-inf beside few finite values, a row of nothing else, NaN, +inf, tokens
     outside of the row, the type's lowest value."""

@@ -391,9 +391,13 @@ struct FinishLds {
 };
 
 // The waves' lists as one, in sh.out; how many there are (k at most). The
-// largest of the waves' own k-th keys bounds the answer's from below; a
-// candidate's comparisons are spread over the waves.
-__device__ int merge(Best &best, FinishLds &sh, int wid, bool mine) {
+// largest of the waves' own k-th keys bounds the answer's from below. So does
+// the smallest of their k/8-th keys (rounded up: together they have k that are
+// no smaller), which leaves fewer candidates: `wide`, where every value of a row
+// was one (us a call at k = 64: 67 rows of 32000 86 -> 73, 323 of 3812 70 -> 58;
+// elsewhere few are left anyway and it costs 0.6 to 0.8). A candidate's
+// comparisons are spread over the waves.
+__device__ int merge(Best &best, FinishLds &sh, int wid, bool mine, bool wide) {
     const int lane = __lane_id(), tid = threadIdx.x, k = best.k;
     if (mine) {
         best.sort();
@@ -409,6 +413,17 @@ __device__ int merge(Best &best, FinishLds &sh, int wid, bool mine) {
             bound = other > bound ? other : bound;
         }
         bound = from_lane(bound, 0);
+        if (wide) {
+            const int kk = (k + FIN_WAVES - 1) / FIN_WAVES;
+            uint64_t low = lane >= FIN_WAVES ? ~0ull : sh.count[lane] >= kk ? sh.buf[lane][kk - 1] : 0;
+#pragma unroll
+            for (int o = 1; o < FIN_WAVES; o <<= 1) {
+                const uint64_t other = __shfl_xor((unsigned long long)low, o);
+                low = other < low ? other : low;
+            }
+            low = from_lane(low, 0);
+            bound = low > bound ? low : bound;
+        }
         const bool take = lane < best.n && best.buf[lane] >= bound;
         const uint64_t m = __ballot(take);  // (lists are in order: a leading run)
         int at = 0;
@@ -502,7 +517,7 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
                 const int i = c + lane;
                 best.push(i < subs ? key_of(sub_max_p[(size_t)row * subs_max + i], i) : 0, i < subs);
             }
-        const int chunks = merge(best, sh, wid, mine);
+        const int chunks = merge(best, sh, wid, mine, false);
         if (mine) {
             // values below the k-th sub-chunk's maximum have k others ahead of them
             const uint64_t bound = chunks == a.k ? sh.out[a.k - 1] & ~0xFFFFFFFFull : 0;
@@ -537,7 +552,7 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
                 }
             }
         }
-        merge(best, sh, wid, mine);
+        merge(best, sh, wid, mine, chunks < a.k);
         if (wid == 0 && lane < a.k) {
             const uint64_t key = sh.out[lane];
             a.top_ids[(size_t)row * a.k + lane] = (int32_t)index_of(key);

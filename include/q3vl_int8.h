@@ -381,7 +381,8 @@ typedef struct q3vl_rope {
  * (no token: q3vl_qk_norm_rope leaves it alone). A row that cannot be planned
  * gets an empty mask, position -2 and slot -1 (its query becomes NaN): one
  * whose chain of parents leaves [-1, its own index), one past max_rows or past
- * the cache, and every row of a sequence whose cache_len is negative.
+ * the cache, one whose position is no int32 >= 0, and every row of a sequence
+ * whose cache_len is negative.
  * max_rows: the most rows of one sequence (at most 1024); mask_words at least
  * ceil(max_rows / 64). */
 int q3vl_draft_plan(const int32_t *parents, const int32_t *row_start, const int32_t *cache_len,
@@ -426,7 +427,8 @@ int q3vl_qk_norm_rope(const float *q, size_t ldq, const float *k, size_t ldk, co
  * behind the last sequence, and rows of a sequence past max_rows, are left as
  * they were in `out`. max_rows: the most rows of one sequence. max_len: the
  * most cached positions of one sequence with its rows, used only to choose how
- * far the work is split (0: max_seq). `out` may be q itself, with its stride.
+ * far the work is split (0: max_seq). scale is finite in fp32 times log2 e too
+ * (below 2.3e38). `out` may be q itself, with its stride.
  * Scores of 2^23 and more (in powers of 2), infinities and NaN that a row sees
  * take a slow path of plain fp32. head_dim 64 or 128. Workspace: the bytes for
  * the same rows, heads, max_rows, max_len and cache, any type and mask. */

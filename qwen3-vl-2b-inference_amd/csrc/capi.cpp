@@ -1578,7 +1578,9 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     if (ldq < qn || ldo < qn) return fail(Q3VL_ERR_INVALID_ARGUMENT, "a row stride is shorter than its row");
     if (mask_words < 0 || (mask && mask_words < 1) || mask_words > (1 << 24))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "mask_words=%d", mask_words);
-    if (!(scale > -INFINITY && scale < INFINITY)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "scale is not finite");
+    const float scale_log2e = (float)((double)scale * 1.4426950408889634);
+    if (!(scale_log2e > -INFINITY && scale_log2e < INFINITY))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "scale=%g: not finite, or not times log2 e", (double)scale);
     if (rows == 0 || max_rows == 0) return Q3VL_OK;
     if (!q || !out || !row_start || !cache_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     const bool half = dtype == Q3VL_DTYPE_FP16;
@@ -1610,7 +1612,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     a.words = mask_words;
     a.splits = plan.splits;
     a.max_len = max_len && max_len < cache->max_seq ? max_len : cache->max_seq;
-    a.scale_log2e = (float)((double)scale * 1.4426950408889634);
+    a.scale_log2e = scale_log2e;
     Q3VL_HIP(launch_tree_attention(a, cache->head_dim, half, plan.rows, (hipStream_t)stream), "attention launch");
     return Q3VL_OK;
 }

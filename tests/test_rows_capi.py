@@ -116,6 +116,8 @@ def attn(cache_over={}, **over):
     (dict(max_len=-1), BAD, "max_len"),
     (dict(scale=math.inf), BAD, "scale"),
     (dict(scale=math.nan), BAD, "scale"),
+    (dict(scale=3e38), BAD, "scale"),  # times log2 e it is none in fp32
+    (dict(scale=-3e38), BAD, "scale"),
     (dict(q=None), BAD, "null"),
     (dict(cache_len=None), BAD, "null"),
     (dict(rows=1 << 30), UNS, "too large"),

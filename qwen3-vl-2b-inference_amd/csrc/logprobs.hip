@@ -165,8 +165,9 @@ template <bool HALF> __device__ __forceinline__ int row_offset(const void *x) {
 // A wave takes two sub-chunks a turn, 16 values a lane. The largest of them and
 // of the lane's running maximum wins a tournament whose losers are exactly the
 // values that enter the sum: one more instruction a value than a maximum alone.
-// About 15 VALU instructions a value, 4 of them the exponential, against 10
-// bytes a clock that HBM has for a CU.
+// 208 VALU instructions a turn (13 a value of a lane), 777 rows of 151936 in
+// fp16: active for 43 us of the 50.2 at 2.4 GHz, where the reads need 36.5. 61
+// rows in fp32: 10.8 us, two turns a wave, latency.
 template <bool HALF>
 __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(const void *logits_p, int64_t ld_p, const int32_t *tokens_p,
                                                               int parts_p, int V_p, int subs_max, LogprobArgs args) {

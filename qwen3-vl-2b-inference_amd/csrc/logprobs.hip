@@ -26,8 +26,10 @@ namespace {
 constexpr int SUB = 512;                             // values of a sub-chunk
 constexpr int THREADS = 256, WAVES = THREADS / 64;   // of the scan
 constexpr int FIN_WAVES = 8;                         // of the second kernel, with alternatives
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-constexpr float FAR = -300.0f;    // exponent (base 2) from which 2^x is 0 in fp32
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float FAR = -208.0f;    // x - m from which e^(x - m) is 0 in fp32
+constexpr float TALL = 1e30f;     // a maximum up to which x - m is finite for every finite x (half a step of the
+                                  // largest float is 2^103 = 1.01e31)
 
 // v_max_f32 and v_min_f32 as they are, for operands that are no NaN: no
 // instruction goes to quieting one first.
@@ -50,18 +52,20 @@ __device__ __forceinline__ float vmin(float a, float b) {
 #endif
 }
 
-// (maximum, sum of the rest, weighted sum in base 2) of some values
+// (maximum, sum of the rest, weighted sum) of some values
 struct Sums {
     float m, r, t;
 };
 
-// 2^((lo - m) log2 e) for lo <= m, and its exponent. CUT: the exponent cut off
-// where the weight is 0, which keeps -inf (0 times infinity otherwise) out of t.
+// e^d for d = lo - m, lo <= m. CUT: d cut off where the weight is 0, which
+// keeps -inf (0 times infinity otherwise) out of t. Without it d has to be
+// finite: d log2 e may overflow (d below -2.36e38, as of a mask of the type's
+// lowest value), which makes the weight 0 and leaves d, that t takes, as it is.
 // m is finite here.
-template <bool CUT = true> __device__ __forceinline__ float weight(float lo, float m, float &arg) {
-    arg = (lo - m) * LOG2E;
-    if (CUT) arg = fmaxf(arg, FAR);
-    return __builtin_amdgcn_exp2f(arg);
+template <bool CUT = true> __device__ __forceinline__ float weight(float lo, float m, float &d) {
+    d = lo - m;
+    if (CUT) d = fmaxf(d, FAR);
+    return __builtin_amdgcn_exp2f(d * LOG2E);
 }
 
 __device__ __forceinline__ float lane_swap_max(float v) {
@@ -88,11 +92,11 @@ __device__ __forceinline__ Sums wave_join(Sums s) {
     Sums o;
     o.m = lane_swap_max(s.m);
     const uint64_t top = __ballot(s.m == o.m);
-    float arg;
-    const float w = weight(s.m, fmaxf(o.m, -FLT_MAX), arg);
+    float d;
+    const float w = weight(s.m, fmaxf(o.m, -FLT_MAX), d);
     const bool out = __lane_id() == (uint32_t)__builtin_ctzll(top | 1ull << 63);
     o.r = lane_swap_sum(fmaf(s.r, w, out ? 0.0f : w));
-    o.t = lane_swap_sum(fmaf(fmaf(s.r, arg, s.t), w, out ? 0.0f : w * arg));
+    o.t = lane_swap_sum(fmaf(fmaf(s.r, d, s.t), w, out ? 0.0f : w * d));
     return o;
 }
 
@@ -274,9 +278,9 @@ __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(const void *logit
         lose[15] = vmin(best, s.m);
         const float m = vmax(best, s.m), ref = vmax(m, -FLT_MAX);
         if (__any(best > s.m)) {
-            float arg;
-            const float w = weight(s.m, ref, arg);
-            s.t = fmaf(s.r, arg, s.t) * w;
+            float d;
+            const float w = weight(s.m, ref, d);
+            s.t = fmaf(s.r, d, s.t) * w;
             s.r *= w;
             s.m = m;
         }
@@ -284,14 +288,15 @@ __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(const void *logit
         auto add = [&](auto cut) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float arg;
-                const float w = weight<decltype(cut)::value>(lose[i], ref, arg);
+                float d;
+                const float w = weight<decltype(cut)::value>(lose[i], ref, d);
                 r[i & 1] += w;
-                q[i & 1] = fmaf(w, arg, q[i & 1]);
+                q[i & 1] = fmaf(w, d, q[i & 1]);
             }
         };
-        // (z is finite until a value was not; lose[15] is -inf in the first turn)
-        if (__any(!(__builtin_fabsf(z) < INFINITY) || lose[15] == -INFINITY)) add(std::true_type{});
+        // (z is finite until a value was not; lose[15] is -inf in the first turn;
+        // up to TALL the difference of two finite values is finite)
+        if (__any(!(__builtin_fabsf(z) < INFINITY) || lose[15] == -INFINITY || ref > TALL)) add(std::true_type{});
         else add(std::false_type{});
         s.r += r[0] + r[1];
         s.t += q[0] + q[1];
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(TOP ? 64 * (FIN_WAVES + 1) : 64) void logprob_finis
             whole[1] = logs;
             a.logprob[row] = (xt - s.m) - logs;
             if (a.rank) a.rank[row] = n < 0 ? -1 : n;
-            if (a.entropy) a.entropy[row] = logs - LN2 * s.t / (1.0f + s.r);
+            if (a.entropy) a.entropy[row] = logs - s.t / (1.0f + s.r);
         }
     }
     if constexpr (TOP) {

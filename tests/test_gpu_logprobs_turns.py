@@ -22,8 +22,9 @@ def turns_of(V, off=0):
 
 
 def several_turns(M, V):
-    """A wave gets its second turn from 4 x 4096 turns over all rows on."""
-    assert turns_of(V) * M >= 16384, "every wave has one turn: the case shows nothing"
+    """Waves get a second turn from 4 x 4096 turns over all rows on, in rows of
+    more turns than a block has waves."""
+    assert turns_of(V) > 4 and turns_of(V) * M >= 16384, "every wave has one turn: the case shows nothing"
 
 
 def logits(M, V, half, seed, off=0, pad=0):
@@ -92,3 +93,46 @@ def test_lowest_values_in_later_turns(M, V):
     x[11, 6::7] = LOWEST
     tokens = [(m * 977 + V - 1) % V for m in range(M)]
     check(x, tokens, 5, list(range(12)) + [M - 1])
+
+
+@pytest.mark.parametrize("k", [0, 20, 64])
+@pytest.mark.parametrize("half", [False, True], ids=["fp32", "fp16"])
+@pytest.mark.parametrize("M,V,off,pad", [(120, 151936, 0, 0), (600, 151936, 3, 1), (1200, 32000, 0, 64), (3001, 8191, 1, 0)], ids=str)
+def test_later_turns(M, V, off, pad, half, k):
+    """The maximum in the first, a middle or the last turn, or moving in every
+    one; what is no number, or rules a value out, only from a late turn on;
+    tokens at both ends and in the middle; rows that start anywhere."""
+    x = logits(M, V, half, M + V, off, pad)
+    rise = torch.linspace(-9, 9, V, device="cuda")
+    x[0], x[1] = rise, -rise
+    x[2, 3], x[3, V // 2 + 1], x[4, V - 2] = 25.0, 25.0, 25.0
+    x[5, V - 7] = math.nan
+    x[6, V // 3] = math.inf
+    x[7, V * 3 // 4:] = -math.inf
+    x[8, :V - 40] = -math.inf
+    x[9] = torch.randint(-2, 3, (V,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(k)).to(x.dtype)
+    x[10, V // 2] = math.nan
+    x[10, V // 2 + 1] = -math.inf
+    x[11] = -math.inf
+    x[12, V // 5:V // 4] = float(torch.finfo(x.dtype).min)
+    ends = [0, V - 1, V // 2, 1, V - 2, V // 2 + 1, 1023 % V, 1024 % V]
+    tokens = [ends[m % 8] for m in range(M)]
+    tokens[3], tokens[4], tokens[7], tokens[8], tokens[9], tokens[12] = V // 2 + 1, V - 2, V - 1, V - 3, V - 4, V // 5 + 3
+    tokens[13], tokens[14] = -1, V
+    check(x, tokens, k, list(range(16)) + [M // 2, M - 2, M - 1])
+
+
+def test_row_counts_agree():
+    """The same row gives the same ids and rank however many others there are,
+    with one turn a wave and with several."""
+    V, k = 151936, 20
+    x = logits(600, V, False, 7)
+    tokens = torch.arange(0, 600 * 250, 250, dtype=torch.int32, device="cuda")
+    want = q.token_logprobs(x, tokens, top_k=k)
+    for M in (1, 109, 110, 223, 599):
+        r = q.token_logprobs(x[:M], tokens[:M], top_k=k)
+        assert torch.equal(r.rank, want.rank[:M]) and torch.equal(r.top_ids, want.top_ids[:M])
+        # both are off by at most the bound that `check` derives
+        e = 21 * 2.0 ** -23 + V ** 0.5 * 2.0 ** -22
+        assert ((r.logprob - want.logprob[:M]).abs().double() <= 2 * (e + 30 * 2.0 ** -22)).all()
+        assert ((r.entropy - want.entropy[:M]).abs().double() <= 2 * 4 * e * want.entropy[:M].double()).all()

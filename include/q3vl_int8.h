@@ -448,7 +448,8 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
  * -inf. rank, entropy and, for top_k 0, the top arrays may be NULL. A logit of
  * -inf has probability 0. A row with a NaN or +inf, or with nothing but -inf,
  * has NaN log probabilities and entropy; its ids and rank stand. A token
- * outside of [0, V) gives NaN and rank -1. */
+ * outside of [0, V) gives NaN and rank -1. Workspace: the bytes for M rows of V
+ * values serve any call of no more rows and values. */
 size_t q3vl_token_logprobs_workspace_bytes(size_t M, size_t V);
 int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t *tokens,
                         size_t M, size_t V, int top_k, float *logprob, int32_t *rank,

@@ -1619,7 +1619,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
 
 size_t q3vl_token_logprobs_workspace_bytes(size_t M, size_t V) {
     if (M == 0 || V == 0 || V > kLogprobMaxV || M > kLogprobMaxM) return 0;
-    return align256(M * (size_t)logprob_parts((int)M, (int)V) * 16) + align256(M * (size_t)logprob_subs((int)V) * 4);
+    return align256((size_t)logprob_parts_most((int)M, (int)V) * 16) + align256(M * (size_t)logprob_subs((int)V) * 4);
 }
 
 int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t *tokens, size_t M,
@@ -1637,8 +1637,10 @@ int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t 
     if (!logits || !tokens || !logprob || (top_k && (!top_ids || !top_logprobs)))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     if ((uintptr_t)logits % (dtype == Q3VL_DTYPE_FP16 ? 2 : 4)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned logits");
+    const int parts = logprob_parts((int)M, (int)V);
+    const size_t part_bytes = align256(M * (size_t)parts * 16);
     char *w = nullptr;
-    const int rc = resolve_ws(workspace, workspace_bytes, q3vl_token_logprobs_workspace_bytes(M, V), &w);
+    const int rc = resolve_ws(workspace, workspace_bytes, part_bytes + align256(M * (size_t)logprob_subs((int)V) * 4), &w);
     if (rc) return rc;
     LogprobArgs a{};
     a.logits = logits;
@@ -1647,9 +1649,9 @@ int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t 
     a.M = (int)M;
     a.V = (int)V;
     a.k = top_k;
-    a.parts = logprob_parts((int)M, (int)V);
+    a.parts = parts;
     a.part = reinterpret_cast<float *>(w);
-    a.sub_max = reinterpret_cast<float *>(w + align256(M * (size_t)a.parts * 16));
+    a.sub_max = reinterpret_cast<float *>(w + part_bytes);
     a.logprob = logprob;
     a.rank = rank;
     a.entropy = entropy;

@@ -136,6 +136,13 @@ int logprob_parts(int M, int V) {
     return (int)(p < kLogprobParts ? p : kLogprobParts);
 }
 
+// No fewer than m * logprob_parts(m, v) for any m <= M, v <= V: turns * m < WAVES
+// 4096 each, so m * (turns / (WAVES each) + 1) stays below 4096 + m.
+int64_t logprob_parts_most(int M, int V) {
+    const int64_t all = (int64_t)M * logprob_parts(1, V), few = 4096 + (int64_t)M;
+    return all < few ? all : few;
+}
+
 // A lane's 16 bytes of a row, values [i, i + VEC), -inf outside of [0, V);
 // inside: the whole wave's piece lies in the row.
 template <bool HALF> __device__ __forceinline__ u32x4 read_piece(const void *x, int i, int V, bool inside) {

@@ -248,6 +248,7 @@ constexpr int kLogprobTop = 64;     // most alternatives
 constexpr int kLogprobParts = 256;  // most parts of a row
 int logprob_subs(int V);
 int logprob_parts(int M, int V);
+int64_t logprob_parts_most(int M, int V);  // parts of all rows, for up to M rows of up to V values
 hipError_t launch_token_logprobs(const LogprobArgs &a, bool half, hipStream_t st);
 
 }  // namespace q3vl

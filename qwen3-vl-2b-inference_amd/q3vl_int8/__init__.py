@@ -296,7 +296,7 @@ class TokenLogprobs(NamedTuple):
 
 
 def alloc_token_logprobs_workspace(M, V, device="cuda"):
-    """Device workspace for token_logprobs over [M, V] logits."""
+    """Device workspace for token_logprobs over up to M rows of up to V logits."""
     torch = _torch()
     return torch.empty(max(256, lib().q3vl_token_logprobs_workspace_bytes(M, V)), dtype=torch.uint8, device=device)
 

@@ -136,3 +136,17 @@ def test_row_counts_agree():
         e = 21 * 2.0 ** -23 + V ** 0.5 * 2.0 ** -22
         assert ((r.logprob - want.logprob[:M]).abs().double() <= 2 * (e + 30 * 2.0 ** -22)).all()
         assert ((r.entropy - want.entropy[:M]).abs().double() <= 2 * 4 * e * want.entropy[:M].double()).all()
+
+
+@pytest.mark.parametrize("most,V", [(333, 151936), (777, 151936), (512, 32000)], ids=str)
+def test_one_workspace_for_fewer_rows(most, V):
+    """A workspace for the largest batch serves the smaller ones, those that
+    are split into more parts among them."""
+    x = logits(most, V, True, 11)
+    tokens = torch.arange(most, dtype=torch.int32, device="cuda")
+    ws = q.alloc_token_logprobs_workspace(most, V)
+    for M in sorted({1, 109, 110, 322, 329, 426, 511, 768, 769, most}):
+        if M <= most:
+            r = q.token_logprobs(x[:M], tokens[:M], top_k=3, workspace=ws)
+            own = q.token_logprobs(x[:M], tokens[:M], top_k=3, workspace=q.alloc_token_logprobs_workspace(M, V))
+            assert all(torch.equal(a, b) for a, b in zip(r, own)), M

@@ -187,3 +187,14 @@ def test_bindings_refuse_host_tensors():
         qa.KVCache(x.half().reshape(1, 1, 2, 128), x.half().reshape(1, 1, 2, 128))
     with pytest.raises(ValueError, match="device tensor"):
         qa.draft_plan(i, i, i, 10, 3)
+
+
+@pytest.mark.parametrize("V", [1, 1000, 4096, 32000, 151936, 1 << 20, 1 << 30])
+def test_logprobs_workspace_serves_fewer_rows(V):
+    """A workspace for M rows holds what fewer rows, and shorter ones, need: the
+    size asked for never falls with M or V."""
+    size = q.lib().q3vl_token_logprobs_workspace_bytes
+    rows = sorted({*range(1, 1200), *(1 << i for i in range(23)), *((1 << i) - 1 for i in range(11, 23))})
+    sizes = [size(M, V) for M in rows]
+    assert all(0 < a <= b for a, b in zip(sizes, sizes[1:]))
+    assert all(size(M, max(1, V - 1)) <= size(M, V) and size(M, V // 2 + 1) <= size(M, V) for M in rows)

@@ -607,6 +607,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
         }
     };
     if constexpr (SHARED) {
+        lds_barrier();  // one lane alone may have set a row's flag, and its other three read it
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
             if (live[nr] && !flag[row[nr] - r0])

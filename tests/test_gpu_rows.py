@@ -582,3 +582,27 @@ def test_logprobs_of_the_certain_token():
             # |x - m| 2^-23 and the exponential's 2^-23, V half steps
             assert abs(float(r.logprob[m]) - want) <= abs(want) * (45 + V) * 2.0 ** -23
             assert r.top_ids[m, 0] == 1234 and r.rank[m] == 0 and r.top_logprobs[m, 0] == r.logprob[m]
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["fp32", "fp16"])
+@pytest.mark.parametrize("T,ctx", [(7, 30), (40, 30), (150, 64), (40, 5000)], ids=str)
+def test_attention_redone_rows_in_place(T, ctx, half):
+    """A row whose result one lane alone finds not finite (an infinity in a
+    single column of an unseen draft) is done again from its query: with out
+    over q no lane of it may write before that. Unsplit and split tiles, few
+    rows and many; the answer is that without the infinity."""
+    B = Batch(T + ctx + 1, [T, 3], [ctx, 9], 4, 2, 128, half, True)
+    for col in (0, 37, 126):
+        clean = B.run()
+        kept = B.v.copy()
+        B.v[0, :, ctx + T - 1, col] = np.inf  # the last draft: no other row sees it
+        x = dev(B.q)
+        got = B.run(q=x, out=x)
+        unseen = [r for r in range(T - 1)]
+        assert np.isfinite(got[unseen]).all()
+        B.check(got, only=lambda b, t: b == 1 or t < T - 1)
+        g = got[T - 1].reshape(4, 128)
+        assert (g[:, col] == np.inf).all() and np.isfinite(np.delete(g, col, 1)).all()
+        np.testing.assert_array_equal(got, B.run())
+        B.v = kept
+        np.testing.assert_array_equal(B.run(), clean)

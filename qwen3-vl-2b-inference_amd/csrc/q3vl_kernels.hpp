@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 namespace q3vl {
 
 // ---------------------------------------------------------------- quantizer
@@ -187,6 +189,21 @@ hipError_t launch_gemm_wide(const float *A, const int8_t *W, const float *S, flo
                             float *part_val, int32_t *part_idx, int cus, hipStream_t st);
 
 // ------------------------------------------- rows of tokens over the caches
+// Raises a kernel's LDS limit to the most it asks for, once a device: `bytes` is
+// the same at every call, or one call would lower it for another thread's.
+template <auto Kernel> inline hipError_t allow_lds(int bytes) {
+    if (bytes <= 64 * 1024) return hipSuccess;
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e != hipSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    e = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 constexpr int kDraftRows = 1024;  // most rows of one sequence that a plan's LDS holds
 hipError_t launch_draft_plan(const int32_t *parents, const int32_t *row_start, const int32_t *cache_len,
                              const int32_t *pos_delta, int batch, int rows, int max_rows, int max_seq, uint64_t *mask,

@@ -104,10 +104,10 @@ hipError_t launch_draft_plan(const int32_t *parents, const int32_t *row_start, c
                              int words, int32_t *pos, int64_t *slots, hipStream_t st) {
     const int n = max_rows < rows ? max_rows : rows;
     const size_t lds = (size_t)n * ((n + 63) / 64) * 8 + (size_t)n * 4;
-    static_assert(kDraftRows * (kDraftRows / 64) * 8 + kDraftRows * 4 <= 160 * 1024, "LDS");
+    constexpr int most = kDraftRows * (kDraftRows / 64) * 8 + kDraftRows * 4;
+    static_assert(most <= 160 * 1024, "LDS");
     if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(draft_plan_kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        const hipError_t e = allow_lds<&draft_plan_kernel>(most);
         if (e != hipSuccess) return e;
     }
     const int threads = n <= 64 ? 64 : n <= 256 ? 256 : 1024;

@@ -1,8 +1,6 @@
 // tree_attention.hip -- attention of several rows a sequence over its cache:
 // one token of each sequence of a batch, a prompt's chunk, or a tree of
 // drafted tokens. gfx950.
-#include <atomic>
-
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 #include "q3vl_mfma.hpp"
@@ -807,20 +805,6 @@ TreePlan tree_attention_plan(int64_t rows, int heads, int kv_heads, int batch, i
 
 bool tree_attention_fits(int64_t kv_rows, int kv_heads, int batch, int max_rows, int heads) {
     return (kv_rows + 15) / 16 * batch <= kBlocks / kv_heads && (int64_t)batch * max_rows <= kBlocks * WAVES / heads;
-}
-
-// Raises the kernel's LDS limit, once a device.
-template <auto Kernel> static hipError_t allow_lds(int bytes) {
-    if (bytes <= 64 * 1024) return hipSuccess;
-    static std::atomic<uint64_t> done{0};
-    int dev = 0;
-    hipError_t e = hipGetDevice(&dev);
-    if (e != hipSuccess) return e;
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (done.load(std::memory_order_relaxed) & bit) return hipSuccess;
-    e = hipFuncSetAttribute(reinterpret_cast<const void *>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == hipSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-    return e;
 }
 
 template <int D, bool HALF, int NR, bool SHARED, bool ONCE> static hipError_t launch_tile(const TreeAttnArgs &a, int tiles, hipStream_t st) {

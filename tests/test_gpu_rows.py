@@ -606,3 +606,33 @@ def test_attention_redone_rows_in_place(T, ctx, half):
         np.testing.assert_array_equal(got, B.run())
         B.v = kept
         np.testing.assert_array_equal(B.run(), clean)
+
+
+def test_plans_of_two_threads():
+    """Plans of different sizes, both past 64 KiB of LDS, from two threads at
+    once: neither call changes what the other's launch may use."""
+    import threading
+    wrong = []
+
+    def plans(T):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                par = random_parents(np.random.default_rng(T), [T, T])
+                args = i32(par), i32([0, T, 2 * T]), i32([5, 70]), 2 * T, T
+                want = ref.plan(par, [0, T, 2 * T], [5, 70], 2 * T, T, -(-T // 64))
+                got = [qa.draft_plan(*args) for _ in range(100)]
+                stream.synchronize()
+                for mask, pos, slots in got:
+                    np.testing.assert_array_equal(mask.cpu().numpy().view(np.uint64), want[0])
+                    np.testing.assert_array_equal(pos.cpu().numpy(), want[1])
+                    np.testing.assert_array_equal(slots.cpu().numpy(), want[2])
+        except BaseException as e:  # noqa: BLE001  (for the main thread)
+            wrong.append((T, e))
+
+    threads = [threading.Thread(target=plans, args=(T,)) for T in (1024, 750)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong

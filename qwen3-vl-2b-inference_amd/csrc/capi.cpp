@@ -1576,6 +1576,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
         return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
     const size_t qn = (size_t)heads * cache->head_dim;
     if (ldq < qn || ldo < qn) return fail(Q3VL_ERR_INVALID_ARGUMENT, "a row stride is shorter than its row");
+    if (out == q && ldo != ldq && rows > 1) return fail(Q3VL_ERR_INVALID_ARGUMENT, "out over q needs q's stride");
     if (mask_words < 0 || (mask && mask_words < 1) || mask_words > (1 << 24))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "mask_words=%d", mask_words);
     const float scale_log2e = (float)((double)scale * 1.4426950408889634);

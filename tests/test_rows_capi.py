@@ -198,3 +198,10 @@ def test_logprobs_workspace_serves_fewer_rows(V):
     sizes = [size(M, V) for M in rows]
     assert all(0 < a <= b for a, b in zip(sizes, sizes[1:]))
     assert all(size(M, max(1, V - 1)) <= size(M, V) and size(M, V // 2 + 1) <= size(M, V) for M in rows)
+
+
+@pytest.mark.parametrize("over", [dict(out=P, ldo=600), dict(out=P, ldq=640)], ids=str)
+def test_tree_attention_in_place_needs_one_stride(over):
+    """out over q with another stride: its rows would lie over other rows'
+    queries."""
+    refused(attn(**over), BAD, "over q")

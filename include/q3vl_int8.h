@@ -49,9 +49,10 @@
  * reads). Calls sharing one workspace must be ordered on one stream, and so
  * must calls that pass NULL and use the library's buffer: every call of more
  * than 8 rows or K > 8192, the MLP block, the argmax calls, the decode step,
- * and products of 5..8 rows with a weight of N * K >= 2^26 at group_size 64.
- * The other linears of up to 8 rows keep nothing in it, and may run on several
- * streams without a workspace.
+ * products of 5..8 rows with a weight of N * K >= 2^26 at group_size 64,
+ * q3vl_tree_attention where its workspace is not 0 bytes, and
+ * q3vl_token_logprobs. The other linears of up to 8 rows keep nothing in it,
+ * and may run on several streams without a workspace.
  */
 #ifndef Q3VL_INT8_H
 #define Q3VL_INT8_H
@@ -331,7 +332,8 @@ int q3vl_quantize_groupwise(const float *x, size_t count, size_t group, int8_t *
  * cached before this step) live in device memory, so that a captured call
  * replays with other lengths. Rows behind the last sequence hold no token.
  * Values there are clamped to the arrays: no row_start or cache_len makes a
- * call read or write outside of its buffers. */
+ * call read or write outside of its buffers. A captured call that needs a
+ * workspace is refused without one. */
 
 /* One layer's caches of a batch, fp16. Row r of kv head h of sequence b is the
  * head_dim values at b * seq_stride + h * head_stride + r * row_stride

@@ -1419,6 +1419,18 @@ int q3vl_quantize_groupwise(const float *x, size_t count, size_t group, int8_t *
 
 // ---- rows of tokens over the caches
 
+// The workspace of these calls. A graph would keep the address of the library's
+// buffer, which a later call may free to grow it: a captured call brings its own.
+static int resolve_ws_rows(void *user, size_t user_bytes, size_t need, hipStream_t st, char **out) {
+    if (!user && st) {  // (the null stream is never captured)
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        Q3VL_HIP(hipStreamIsCapturing(st, &capture), "hipStreamIsCapturing");
+        if (capture != hipStreamCaptureStatusNone)
+            return fail(Q3VL_ERR_INVALID_ARGUMENT, "a captured call needs a workspace of its own (%zu bytes)", need);
+    }
+    return resolve_ws(user, user_bytes, need, out);
+}
+
 static int check_cache(const q3vl_kv_cache *c) {
     if (!c || !c->k || !c->v) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null cache");
     if (c->batch < 1 || c->kv_heads < 1 || c->max_seq < 1)
@@ -1588,7 +1600,7 @@ int q3vl_tree_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     size_t need = 0;
     const TreePlan plan = plan_tree_attention(rows, heads, max_rows, max_len, cache, half, !mask, &need);
     char *w = nullptr;
-    if (need && (rc = resolve_ws(workspace, workspace_bytes, need, &w))) return rc;
+    if (need && (rc = resolve_ws_rows(workspace, workspace_bytes, need, (hipStream_t)stream, &w))) return rc;
     TreeAttnArgs a{};
     a.q = q;
     a.out = out;
@@ -1641,7 +1653,8 @@ int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t 
     const int parts = logprob_parts((int)M, (int)V);
     const size_t part_bytes = align256(M * (size_t)parts * 16);
     char *w = nullptr;
-    const int rc = resolve_ws(workspace, workspace_bytes, part_bytes + align256(M * (size_t)logprob_subs((int)V) * 4), &w);
+    const int rc = resolve_ws_rows(workspace, workspace_bytes, part_bytes + align256(M * (size_t)logprob_subs((int)V) * 4),
+                                   (hipStream_t)stream, &w);
     if (rc) return rc;
     LogprobArgs a{};
     a.logits = logits;

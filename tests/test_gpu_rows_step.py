@@ -239,3 +239,32 @@ def test_bindings_refuse_what_does_not_fit():
         qa.qk_norm_rope(st["q"], st["k"][:, :128], st["v"], st["cache"], st["tokens"].long(), st["tokens"], st["norm"], st["rope"])
     with pytest.raises(q.Q3VLError, match="top_k=65"):
         q.token_logprobs(st["logits"], st["tokens"], top_k=65)
+
+
+def test_captured_calls_need_their_own_workspace():
+    """The library's buffer may be freed to grow it, and a graph would keep its
+    address: refused, while the capture goes on; a call that needs none is
+    captured."""
+    st = make_step(11)
+    attn = lambda cache, rows, **kw: qa.tree_attention(st["q"], cache, st["row_start"], st["cache_len"], rows, **kw)  # noqa: E731
+    ws = st["ws"]
+    assert ws.numel() > 256  # the attention of this step is split
+    want = [x.clone() for x in run_step(st)]
+    st["ws"] = st["lws"] = None
+    run_step(st)  # the library's buffer is large enough
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(q.Q3VLError, match="needs a workspace of its own"):
+            attn(st["cache"], st["T"], max_len=st["S"])
+        with pytest.raises(q.Q3VLError, match="needs a workspace of its own"):
+            q.token_logprobs(st["logits"], st["tokens"], top_k=3)
+        unsplit = attn(st["cache"], st["T"], max_len=1)
+        split = attn(st["cache"], st["T"], max_len=st["S"], workspace=ws)
+    eager = attn(st["cache"], st["T"], max_len=1).clone(), attn(st["cache"], st["T"], max_len=st["S"], workspace=ws).clone()
+    for _ in range(3):
+        unsplit.zero_(), split.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(unsplit, eager[0]) and torch.equal(split, eager[1])
+    assert same(run_step(st), want)

@@ -306,7 +306,7 @@ def token_logprobs(logits, tokens, top_k=0, workspace=None, stream=None):
     the top_k best alternatives, from logits [M, V] (fp32 or fp16, rows may be
     views of wider ones): a TokenLogprobs. Larger values come first, equal ones
     by index; a token outside of [0, V) gives NaN and rank -1."""
-    from .attention import _device, _empty, _raw_stream, _rows, _vec
+    from .attention import _device, _empty, _raw_stream, _rows, _vec, _workspace
     torch, dev = _device()
     f32, i32 = torch.float32, torch.int32
     ld = _rows(logits, (f32, torch.float16), "logits", dev)
@@ -319,7 +319,7 @@ def token_logprobs(logits, tokens, top_k=0, workspace=None, stream=None):
     else:
         lp, ent, top = (_empty(tokens, stream, *n, dtype=f32) for n in ((M,), (M,), (M, k)))
         rank, ids = _empty(tokens, stream, M), _empty(tokens, stream, M, k)
-    wp, wb = _ws(workspace)
+    wp, wb = _workspace(workspace, dev)
     rc = lib().q3vl_token_logprobs(logits.data_ptr(), ld, FP32 if logits.dtype is f32 else FP16, tokens.data_ptr(), M, V, top_k,
                                    lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), wp, wb,
                                    _raw_stream(stream, torch, dev))

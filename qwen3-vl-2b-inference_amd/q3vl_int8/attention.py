@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import FP16, FP32, _check, _need, _ptr, _torch, _ws, lib
+from . import FP16, FP32, _check, _need, _ptr, _torch, lib
 
 _sz = ctypes.c_size_t
 _vp = ctypes.c_void_p
@@ -125,6 +125,15 @@ def _mask_words(mask, rows, dev):
     if n != rows:
         raise ValueError("mask must have a line for each row")
     return words
+
+
+def _workspace(t, dev):
+    """(address, bytes) of a call's workspace; none: the library's own."""
+    if t is None:
+        return None, 0
+    if not (isinstance(t, _torch().Tensor) and t.get_device() == dev and t.is_contiguous()):
+        raise ValueError("workspace must be a contiguous tensor on the current device")
+    return t.data_ptr(), t.numel() * t.element_size()
 
 
 def _empty(like, stream, *shape, dtype=None):
@@ -329,7 +338,7 @@ def tree_attention(q, cache, row_start, cache_len, max_rows, mask=None, max_len=
     _vec(row_start, torch.int32, batch + 1, "row_start", dev)
     _vec(cache_len, torch.int32, batch, "cache_len", dev)
     words = 0 if mask is None else _mask_words(mask, rows, dev)
-    wp, wb = _ws(workspace)
+    wp, wb = _workspace(workspace, dev)
     rc = (_attn_fn or _L().q3vl_tree_attention)(
         q.data_ptr(), ldq, out.data_ptr(), ldo, FP16 if q.dtype is torch.float16 else FP32, rows, qn // D, cache.ref,
         row_start.data_ptr(), cache_len.data_ptr(), _ptr(mask), words, max_rows, max_len or 0,

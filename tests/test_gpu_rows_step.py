@@ -268,3 +268,15 @@ def test_captured_calls_need_their_own_workspace():
         torch.cuda.synchronize()
         assert torch.equal(unsplit, eager[0]) and torch.equal(split, eager[1])
     assert same(run_step(st), want)
+
+
+def test_workspaces_that_no_kernel_may_write():
+    """A host tensor, or every other byte of one: refused before the launch."""
+    st = make_step(12)
+    n = st["ws"].numel()
+    for ws in (torch.empty(n, dtype=torch.uint8), torch.empty(n, dtype=torch.uint8).pin_memory(),
+               torch.empty((n, 2), dtype=torch.uint8, device="cuda")[:, 0], 4096):
+        with pytest.raises(ValueError, match="workspace must be"):
+            qa.tree_attention(st["q"], st["cache"], st["row_start"], st["cache_len"], st["T"], max_len=st["S"], workspace=ws)
+        with pytest.raises(ValueError, match="workspace must be"):
+            q.token_logprobs(st["logits"], st["tokens"], workspace=ws)

@@ -424,7 +424,8 @@ int q3vl_qk_norm_rope(const float *q, size_t ldq, const float *k, size_t ldk, co
  * strides ldq and ldo; heads a multiple of cache->kv_heads, query head h reads
  * kv head h / (heads / kv_heads). Products in fp16 matrix instructions with
  * fp32 sums: fp32 queries and their probabilities as two fp16 terms each
- * (relative 2^-21), fp16 ones as one. The rows of a sequence with cache_len[b]
+ * (relative 2^-21), fp16 ones as one; no probability finer than 2^-31 of the
+ * row's largest. The rows of a sequence with cache_len[b]
  * < 0 or cache_len[b] + its rows > max_seq give NaN, reading nothing. Rows
  * behind the last sequence, and rows of a sequence past max_rows, are left as
  * they were in `out`. max_rows: the most rows of one sequence. max_len: the

@@ -145,8 +145,10 @@ template <bool HALF> __device__ __forceinline__ void put(void *out, int64_t at, 
 // when the bias was last set: a score that passes it by up to GROW stays under
 // fp16's 2^16, so the accumulators are rescaled in the first step and seldom
 // after (with every new maximum, some row of 32 had one in most steps: 267 VALU
-// instructions a step). 2^-20 of the largest p is still a normal number, and of
-// fp32's two terms the smaller keeps 2^-31 of it. A row's results are its O and
+// instructions a step). 2^-20 of the largest p is still a normal number; no p
+// is held finer than 2^-31 of it, of two terms either, and below that it counts
+// for nothing (BASE 12 and GROW 3 would hold 2^-37: the tree's case below 62.8
+// us a call for 61.2, the prompt's 52.3 for 51.4). A row's results are its O and
 // l with weights 2^(-bias). l is summed by the matrix cores too, as V's column
 // of ones: a product a step instead of an addition a score.
 //

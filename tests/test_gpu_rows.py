@@ -636,3 +636,25 @@ def test_plans_of_two_threads():
     for t in threads:
         t.join()
     assert not wrong, wrong
+
+
+@pytest.mark.parametrize("half", [False, True], ids=["fp32", "fp16"])
+@pytest.mark.parametrize("T,ctx", [(1, 3000), (40, 900)], ids=str)
+@pytest.mark.parametrize("gap", [5.0, 12.0, 17.0, 21.0, 25.0])
+def test_attention_small_probabilities(gap, T, ctx, half):
+    """One cached key ahead of all others by e^gap, its value 0: the answer is
+    made of the others' probabilities, which are held no finer than 2^-31 of
+    the row's largest (fp16 subnormals' half step, 2^-25, where the largest is
+    2^6 at least). Over the values: 2^-31 sum |v|, beside the general bound."""
+    B = Batch(T, [T], [ctx], 4, 2, 128, half, False)
+    B.k[:] = 0
+    B.k[0, :, 0, 0] = 8.0
+    B.v[0, :, 0] = 0
+    B.q[:, 0::128] = gap / 8.0 / 128 ** -0.5
+    got = B.run()
+    for t in {0, T // 2, T - 1}:
+        seen = ref.seen_by(t, T, ctx, None)
+        want, absv, qk = ref.attention(B.q[t].reshape(4, 128), B.k[0], B.v[0], seen, 128 ** -0.5)
+        sums = np.repeat(np.abs(B.v[0][:, seen].astype(np.float64)).sum(1), 2, axis=0)
+        tol = ref.attention_tolerance(absv, qk, 128, len(seen), half) + 2.0 ** -31 * 1.01 * sums
+        within(got[t].reshape(4, 128), want, tol, f"row {t}")

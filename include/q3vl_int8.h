@@ -384,7 +384,9 @@ typedef struct q3vl_rope {
  * gets an empty mask, position -2 and slot -1 (its query becomes NaN): one
  * whose chain of parents leaves [-1, its own index), one past max_rows or past
  * the cache, one whose position is no int32 >= 0, and every row of a sequence
- * whose cache_len is negative.
+ * whose cache_len is negative. Positions alone do not end a chain: with cache_len
+ * + pos_delta below 0 deeper rows can be planned, and their masks name ancestors
+ * that store no keys in this step.
  * max_rows: the most rows of one sequence (at most 1024); mask_words at least
  * ceil(max_rows / 64). */
 int q3vl_draft_plan(const int32_t *parents, const int32_t *row_start, const int32_t *cache_len,

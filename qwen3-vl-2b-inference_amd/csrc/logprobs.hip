@@ -126,8 +126,10 @@ __device__ __forceinline__ bool ahead(float x, int i, float xt, int t) { return 
 // Sub-chunks lie on 16-byte boundaries, so a row may touch one more than its size asks for.
 int logprob_subs(int V) { return (V + 7 + SUB - 1) / SUB; }
 
-// Blocks a row: about 4096 over all rows, every wave with the same number of
-// turns but the last (a turn is two sub-chunks).
+// Blocks a row. A turn of a wave is two sub-chunks; every wave but the last has
+// as many turns as keep all rows' blocks to about 4096 or fewer (110 rows of
+// 151936: 2 turns, 2090 blocks; 777: 8, 3885). With fewer than 4 x 4096 turns over
+// all rows a wave has one (1 row 38 blocks, 61 rows 2318).
 int logprob_parts(int M, int V) {
     const int64_t turns = (V + 7 + 2 * SUB - 1) / (2 * SUB);
     int64_t each = (turns * M + 2 * WAVES * 2048) / (WAVES * 4096);
@@ -176,9 +178,10 @@ template <bool HALF> __device__ __forceinline__ int row_offset(const void *x) {
 // A wave takes two sub-chunks a turn, 16 values a lane. The largest of them and
 // of the lane's running maximum wins a tournament whose losers are exactly the
 // values that enter the sum: one more instruction a value than a maximum alone.
-// 208 VALU instructions a turn (13 a value of a lane), 777 rows of 151936 in
-// fp16: active for 43 us of the 50.2 at 2.4 GHz, where the reads need 36.5. 61
-// rows in fp32: 10.8 us, two turns a wave, latency.
+// 209 VALU instructions a turn (13 a value of a lane): 777 rows of 151936 in fp16
+// hold the VALU for 99 of 100 busy cycles, 48.9 us, where the reads need 36.5. 61
+// rows in fp32: 10.6 us for 5.7 of reads, one turn a wave: 2318 blocks that each
+// pay the token's load, two joins across lanes and a barrier for 16 values a lane.
 template <bool HALF>
 __global__ __launch_bounds__(THREADS) void logprob_scan_kernel(const void *logits_p, int64_t ld_p, const int32_t *tokens_p,
                                                               int parts_p, int V_p, int subs_max, LogprobArgs args) {

@@ -127,8 +127,8 @@ hipError_t launch_draft_plan(const int32_t *parents, const int32_t *row_start, c
 // same four chains, exchange their values and run all of them.
 //
 // Bound by HBM: 8 D bytes a query head in and out, 6 D a key or value head.
-// 4999 rows of 16 + 8 + 8 heads with three positions: 29.2 us again and again,
-// 37.7 a call on other data each time; pairs of two values a lane (32-byte
+// 4999 rows of 16 + 8 + 8 heads with three positions: 29.3 us again and again,
+// 37.8 a call on other data each time; pairs of two values a lane (32-byte
 // pieces, no exchange) took 65.8 where this took 28.4.
 #define Q3VL_QUADP(v, ctrl) \
     __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xF, 0xF, true))

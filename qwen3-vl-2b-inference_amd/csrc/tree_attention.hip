@@ -129,11 +129,15 @@ template <bool HALF> __device__ __forceinline__ void put(void *out, int64_t at, 
 // Two forms. Few rows (at most 32 of a kv head's): each wave walks its own 32
 // keys of every 128 with all rows, in a private ring of two stages, no barrier;
 // the four waves' results are joined in LDS at the end. Bound by the cache's
-// reads: one token each of 24 sequences of up to 6000, 67.6 us, 6.4 TB/s, the
+// reads: one token each of 24 sequences of up to 6000, 67.1 us, 6.5 TB/s, the
 // rate of a plain read here. Many rows: a wave has 16 or 32 rows of its own, the
-// block shares 64-key tiles in two buffers, one barrier a tile. Bound by matrix
-// and vector instructions, which add up on a SIMD: three trees of up to 61 rows
-// over 16000 in fp32 56.7 us, 2000 rows behind 1200 in fp16 54.1.
+// block shares 64-key tiles in two buffers, one barrier a tile. Two waves a SIMD,
+// each a chain of scores, softmax and values: three trees of up to 61 rows over
+// 16000 in fp32 55.2 us, 2000 rows behind 1200 in fp16 51.8. Of the shader
+// engines' busy cycles the matrix cores work in 45 and 35 of 100 and other vector
+// instructions run in 31 and 27, a SIMD's mean; even laid end to end they leave 24
+// and 38 to waits (for the chain's own results, LDS reads, the next tile and its
+// barrier) and to SIMDs without a block.
 //
 // fp32 queries are two fp16 terms, hi + lo, relative to the row's largest value
 // (a power of two, undone in the score's factor sc), and so are their
@@ -156,7 +160,11 @@ template <bool HALF> __device__ __forceinline__ void put(void *out, int64_t at, 
 // keys are replaced by -inf before the maximum. An unseen V row of another
 // row's draft can still hold an infinity or NaN, and 0 times it is NaN: a row
 // whose O or l is not finite is done again by row_attention; so is one whose
-// scores pass 2^23, where the rounding of M sc alone moves p by bits.
+// scores pass 2^23, where the rounding of M sc alone moves p by bits. Such rows
+// go one after the other through their block's part of the cache, and a NaN in
+// a draft that no row sees brings every row of the sequence there: 8 drafts
+// over 1000 in fp32 370 us for 10.3, three trees of up to 61 over 16000 17.2 ms
+// for 57 us.
 template <int D, int NR, bool SHARED> struct Tile {
     static constexpr int RB = 2 * D;             // bytes of a cached row
     static constexpr int RI = D / 32;            // loads of 1 KiB for 16 rows
@@ -751,24 +759,28 @@ constexpr int64_t kBlocks = (1 << 24) - 1;  // of 256 threads in a launch
 //
 // Up to 32 rows a kv head: blocks of 16 or 32 rows whose waves walk their own
 // keys, one to a CU, bound by its reads; as many splits as fill the chip once.
-// us over splits (16 / 8 heads of 128, fp32): one token at 32000, 8 blocks
-// unsplit: 184 at 1, 28.3 at 32; two trees of 16 rows over 16000, 16 blocks: 151
-// at 1, 29.1 at 16, 38 at 21. Where that leaves part of the chip idle, a few
-// rounds of smaller blocks: 24 sequences of 6000, 192 blocks: 88.5 at 1, 83.7 at
-// 4; 40 of 3000, 320 blocks: 74 at 1, 68 at 3. Not below 128 positions a split
-// (one token at 1024: 12.3 at 1, 10.5 at 8).
+// us over splits (16 / 8 heads of 128, fp32; call after call on one state, all
+// sides in turn): one token at 32000, 8 blocks unsplit: 281 at 1, 30.8 at 16,
+// 25.8 at 32; two trees of 16 rows over 16000, 16 blocks: 154 at 1, 32.4 at 16,
+// 44.5 at 21. Where that leaves part of the chip idle, a few rounds of smaller
+// blocks: 24 sequences of 3000 to 6000, 192 blocks: 80.0 at 1, 73.4 at 4, 74.6 at
+// the rule's 5 (all of 6000: 91.5, 94.0 and 94.2, which the lengths, known only
+// to the device, cannot tell apart); 40 of 1500 to 3000, 320 blocks: 68.5 at 1,
+// 62.6 at 3. Not below 128 positions a split (one token at 1024: 11.7 at 1, 9.7
+// at 8).
 //
-// More rows: blocks of 64 or 128, two to a CU. A turn of 64 positions takes 0.78
-// us at 64 rows in fp16, 1.1 in fp32, 1.18 and 1.9 at 128, times the blocks on
-// the CU (a second block hides little of the first's time), a quarter more for
-// a block alone; three and more wait for a place. (A tree's rows are few and
-// its cache long: that two tiles read it costs 8 %.) A
-// split call writes and reads its partial results (4 TB/s) and has one launch
-// more (2.5 us). Both sides measured: 2000 rows behind 1200, fp16: 64 rows 57.5,
-// 128 rows 67 unsplit, 63 split; 4000 rows: 91 and 88; three trees of 61 over
-// 16000, fp32: 64 rows 72 at 5 splits, 65 at 10, 128 rows 72 at 10, 66 at 21; 16
-// trees of 64 over 500: 15.2 at 1 split, 28 at 2; 8 trees of 40 over 8000: 64
-// rows 66, 128 rows 56.
+// More rows: blocks of 64 or 128, two to a CU. The model's constants, a turn of
+// 64 positions at 0.78 us for 64 rows in fp16, 1.1 in fp32, 1.18 and 1.9 for 128,
+// times the blocks on the CU, a quarter more for a block alone, 8 % for a tree's
+// cache that two tiles read, were fitted to an earlier form of the kernel; a block
+// alone now takes 0.77, 1.10, 1.15 and 1.81 a turn. A split call writes and reads
+// its partial results (4 TB/s) and has one launch more (2.5 us). Both sides with
+// the present kernel, the rule's choice first: 2000 rows behind 1200, fp16: 64
+// rows unsplit 51.8, split 65.8, 128 rows 65.2 and 59.2 (fp32 74.1, 87.2, 102.5
+// and 83.0); 4000 rows, fp16: 128 rows 84.2, 64 rows 87.9; 16 trees of 64 over
+// 500: 14.3 unsplit, 24.2 in two; 8 trees of 40 over 8000: 128 rows 55.8, 64 rows
+// 56.3 (fp32 74.0 and 78.3); three trees of 61 over 16000: 128 rows at 21 splits
+// 52.0, where 64 rows at 10 take 46.7 (fp32 64.9 and 62.2).
 TreePlan tree_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim,
                              bool half, bool chain) {
     const int64_t kv_rows = (int64_t)max_rows * (heads / kv_heads), most = ((int64_t)max_len + 127) / 128;
@@ -823,9 +835,10 @@ template <int D, bool HALF> static hipError_t launch_d(const TreeAttnArgs &a, in
     const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
     // Keys and values that one block reads once go past the caches: always with few
     // rows; of shared tiles where together they are more than the caches keep
-    // (us, through them and past them: 30 trees of 20 over 6000, 369 MB, fp16: 145
-    // and 128; 8 of 40 over 8000, 263 MB: 64 and 59.5, fp32 79.5 and 77.5; but 1 of
-    // 64 over 16000, 66 MB: 28.0 and 30.7).
+    // (us through them and past them, call after call on one state: 30 trees of 20
+    // over 6000, 369 MB, fp16 138 and 118, fp32 145 and 123; 8 of 40 over 8000, 263
+    // MB, 55 and 57, 76 and 76; but 1 of 64 over 16000, 66 MB: 25.7 and 28.6, 32.9
+    // and 34.5).
     const bool once = tiles == 1 && (double)a.batch * a.kv_heads * a.max_len * D * 4 > 192e6;
     hipError_t e;
     if (bm == 16) e = launch_tile<D, HALF, 1, false, true>(a, tiles, st);

@@ -50,8 +50,8 @@
  * must calls that pass NULL and use the library's buffer: every call of more
  * than 8 rows or K > 8192, the MLP block, the argmax calls, the decode step,
  * products of 5..8 rows with a weight of N * K >= 2^26 at group_size 64,
- * q3vl_tree_attention where its workspace is not 0 bytes, and
- * q3vl_token_logprobs. The other linears of up to 8 rows keep nothing in it,
+ * q3vl_tree_attention and q3vl_long_attention where their workspace is not 0
+ * bytes, q3vl_token_logprobs and q3vl_verify_drafts. The other linears of up to 8 rows keep nothing in it,
  * and may run on several streams without a workspace.
  */
 #ifndef Q3VL_INT8_H
@@ -460,6 +460,108 @@ int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t 
                         size_t M, size_t V, int top_k, float *logprob, int32_t *rank,
                         float *entropy, int32_t *top_ids, float *top_logprobs, void *workspace,
                         size_t workspace_bytes, q3vl_stream stream);
+
+/* ---- long contexts: a cache whose whole blocks of 32 positions are held in 8
+ * bits, and attention through a window. No counterpart in the reference.
+ *
+ * A sequence's positions are packed_len[b] in 8-bit blocks (a multiple of 32)
+ * and, behind them, the rows of a q3vl_kv_cache: cache_len[b] of them and the
+ * step's own. New rows are written there in fp16 as ever (q3vl_draft_plan with
+ * pos_delta = packed_len, q3vl_qk_norm_rope) and stay so until they are no
+ * drafts any more and their block of 32 is whole; q3vl_kv_pack then rounds
+ * them once. In a step: q3vl_long_attention in place of q3vl_tree_attention;
+ * after the layers, the accepted drafts moved and cache_len raised,
+ * q3vl_kv_pack for each layer and q3vl_kv_advance once. Both lengths are int32
+ * [batch] in device memory. */
+
+/* One layer's 8-bit blocks: k, v [batch][kv_heads][blocks][32 * head_dim],
+ * 16-byte aligned, and one scale a block [batch][kv_heads][blocks]. A value is
+ * int8 * scale, |int8| <= 127. Within a block (the order in which the matrix
+ * instructions take it): key position 16 a + i, value 64 c + 32 s + 8 g + e at
+ * [a][c][g][i][s][e]; value position 16 a + 4 g + e, value 32 c + 16 s + i at
+ * [c][g][i][s][a][e] (a, s < 2; g < 4; i < 16; e < 8 and 4). */
+typedef struct q3vl_kv_blocks {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int batch, kv_heads, blocks, head_dim;
+} q3vl_kv_blocks;
+
+/* Packs the first cache_len[b] / 32 blocks of 32 rows of each sequence of
+ * `cache` behind its packed_len[b] positions, and moves the cache_len[b] % 32
+ * rows left to the front of the cache. Per block and kv head, keys and values
+ * apart: scale = max|x| / 127, int8 = x / scale rounded half to even (0 for a
+ * block of zeros). A block that holds an infinity or NaN gets a NaN scale. The
+ * lengths stay as they are: q3vl_kv_advance sets them to what they then are,
+ * packed_len[b] + cache_len[b] / 32 * 32 and cache_len[b] % 32. Both leave
+ * alone a sequence whose lengths are out of range (cache_len[b] outside of [0,
+ * cache->max_seq], packed_len[b] not a multiple of 32 in [0, 32 *
+ * blocks->blocks]), that has no whole block, or whose whole blocks do not all
+ * fit. */
+int q3vl_kv_pack(const q3vl_kv_cache *cache, const q3vl_kv_blocks *blocks, const int32_t *cache_len,
+                 const int32_t *packed_len, q3vl_stream stream);
+int q3vl_kv_advance(const q3vl_kv_cache *cache, const q3vl_kv_blocks *blocks, int32_t *cache_len,
+                    int32_t *packed_len, q3vl_stream stream);
+
+/* Packed positions first[b] .. first[b] + count - 1 (first NULL: from 0), as
+ * far as they are below packed_len[b], to rows 0 .. count - 1 of `cache`,
+ * rounded to fp16. Other rows are left as they were. A sequence whose
+ * packed_len is past its blocks counts up to their end, one whose first[b] is
+ * negative not at all. count: at most cache->max_seq. */
+int q3vl_kv_unpack(const q3vl_kv_blocks *blocks, const int32_t *packed_len, const int32_t *first,
+                   const q3vl_kv_cache *cache, int count, q3vl_stream stream);
+
+/* q3vl_tree_attention over the positions of `blocks` (packed_len[b] of them;
+ * blocks and packed_len NULL: none), then those of `cache`, and through a
+ * window: of the positions that a row would see, in their order, it sees the
+ * first `sinks` and the last `window` (window 0: all). A window over a mask is
+ * at least max_rows. Arguments, types and results are otherwise
+ * q3vl_tree_attention's; max_len counts packed positions too, and 0 stands for
+ * all that the cache and the blocks can hold. A sequence also gives NaN where packed_len[b] is not a
+ * multiple of 32 in [0, 32 * blocks->blocks]. A row that sees a position of a
+ * block with a NaN scale gives NaN. */
+size_t q3vl_long_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
+                                           int window, int sinks, const q3vl_kv_cache *cache,
+                                           const q3vl_kv_blocks *blocks);
+int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,
+                        int heads, const q3vl_kv_cache *cache, const int32_t *row_start,
+                        const int32_t *cache_len, const q3vl_kv_blocks *blocks,
+                        const int32_t *packed_len, const uint64_t *mask, int mask_words,
+                        int max_rows, int max_len, int window, int sinks, float scale,
+                        void *workspace, size_t workspace_bytes, q3vl_stream stream);
+
+/* Judges drafted tokens by rejection sampling: which of a sequence's rows stay,
+ * and the token after them, distributed as if the target alone had drawn them.
+ * rows, parents and row_start as for q3vl_draft_plan; row 0 of a sequence is
+ * the token chosen last and always stays, other rows with parent -1 are not
+ * reached. logits [rows, V] (fp32 or fp16, row stride ld): the target's, after
+ * each row; p = softmax(logits / temperature). draft_probs [rows, V] fp32 (row
+ * stride ldp) or NULL: the probabilities that each row's children were drawn
+ * from, independently (what is negative or NaN counts as 0). accept_u and
+ * sample_u [rows] in [0, 1): one number for a row's own test, one for the token
+ * after it.
+ *
+ * From a row, over its children in order of their index, with c = 0 at first
+ * and Z = sum_i max(p_i - c q_i, 0): the child with token t stays if
+ * accept_u[child] q_t Z < max(p_t - c q_t, 0), else c += Z. If none stays, the
+ * next token is the first i with w_0 + .. + w_i > sample_u[row] sum w, w_i =
+ * max(p_i - c q_i, 0) (p_i where all of these are 0). With draft_probs NULL the
+ * next token is drawn from p at once, and its first child that has it stays.
+ * All in 64 bits; a p below e^-700 of the row's largest counts as 0.
+ *
+ * accepted[b]: rows that stay, the first among them (0: the sequence has none);
+ * path [batch, max_rows]: their indexes in the sequence, ascending, then -1;
+ * next[b]: the token after the last (-1: no rows). A row with a NaN or +inf, or
+ * with nothing but -inf, ends the path, with next -1. A row whose parent is no
+ * earlier row, or whose token is outside of [0, V), does not stay. Rows past
+ * max_rows (at most 1024) do not count. temperature is positive (greedy drafts
+ * are judged by q3vl_token_logprobs' ranks). Workspace: the bytes for as many
+ * rows and values serve any call of no more. */
+size_t q3vl_verify_drafts_workspace_bytes(size_t rows, size_t V);
+int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *draft_probs, size_t ldp,
+                       const int32_t *tokens, const int32_t *parents, const int32_t *row_start,
+                       const float *accept_u, const float *sample_u, int batch, size_t rows,
+                       size_t V, int max_rows, double temperature, int32_t *accepted, int32_t *path,
+                       int32_t *next, void *workspace, size_t workspace_bytes, q3vl_stream stream);
 
 /* ---- weight registry for host-pointer callers (the drop-in linear()).
  * The reference hands linear() mmapped host pointers to weights and scales

@@ -53,6 +53,8 @@ inline bool aligned16(const void *p) { return ((uintptr_t)p & 15u) == 0; }
 
 constexpr size_t kMaxGemvParts = 8192;  // >= grid of any GEMV launch
 constexpr size_t kLogprobMaxM = 1 << 22, kLogprobMaxV = 1 << 30;  // blocks of a launch, indexes of a row
+constexpr int kMaxBlocks = 1 << 25;     // 8-bit blocks of a kv head: 2^30 positions
+constexpr int64_t kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads in a launch
 constexpr int kGemmArgmaxParts = 64;    // argmax partials per row after a GEMM
 
 bool gs_ok_gemv(size_t gs) { return gs == 16 || gs == 32 || gs == 64 || gs == 128 || gs == 256; }
@@ -1672,6 +1674,229 @@ int q3vl_token_logprobs(const void *logits, size_t ld, int dtype, const int32_t 
     a.top_ids = top_ids;
     a.top_logprobs = top_logprobs;
     Q3VL_HIP(launch_token_logprobs(a, dtype == Q3VL_DTYPE_FP16, (hipStream_t)stream), "log probability launch");
+    return Q3VL_OK;
+}
+
+// ---- long contexts
+
+static int check_blocks(const q3vl_kv_blocks *p, const q3vl_kv_cache *c) {
+    if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null blocks");
+    if (p->batch != c->batch || p->kv_heads != c->kv_heads || p->head_dim != c->head_dim)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "blocks of %d x %d heads of %d for a cache of %d x %d of %d", p->batch, p->kv_heads,
+                    p->head_dim, c->batch, c->kv_heads, c->head_dim);
+    if (p->blocks < 1 || p->blocks > kMaxBlocks) return fail(Q3VL_ERR_INVALID_ARGUMENT, "blocks=%d: 1 to %d", p->blocks, kMaxBlocks);
+    if (!aligned16(p->k) || !aligned16(p->v)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "blocks must be 16-byte aligned");
+    if ((uintptr_t)p->k_scale % 4 || (uintptr_t)p->v_scale % 4) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned scales");
+    return Q3VL_OK;
+}
+
+// Whether `per` workgroups for each (sequence, kv head) are a launch.
+static bool blocks_fit(const q3vl_kv_cache *c, int64_t per) {
+    return per <= kMaxGrid && per * c->kv_heads <= kMaxGrid && per * c->kv_heads <= kMaxGrid / c->batch;
+}
+
+int q3vl_kv_pack(const q3vl_kv_cache *cache, const q3vl_kv_blocks *blocks, const int32_t *cache_len,
+                 const int32_t *packed_len, q3vl_stream stream) {
+    int rc = check_cache(cache);
+    if (rc || (rc = check_blocks(blocks, cache))) return rc;
+    if (!cache_len || !packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    if (!blocks_fit(cache, cache->max_seq / 32))
+        return fail(Q3VL_ERR_UNSUPPORTED, "cache too large: batch=%d kv_heads=%d max_seq=%d", cache->batch, cache->kv_heads, cache->max_seq);
+    KvPackArgs a{};
+    a.k = cache->k;
+    a.v = cache->v;
+    a.seq_stride = cache->seq_stride;
+    a.head_stride = cache->head_stride;
+    a.row_stride = cache->row_stride;
+    a.k8 = blocks->k;
+    a.v8 = blocks->v;
+    a.k_scale = blocks->k_scale;
+    a.v_scale = blocks->v_scale;
+    a.cache_len = cache_len;
+    a.packed_len = packed_len;
+    a.batch = cache->batch;
+    a.kv_heads = cache->kv_heads;
+    a.max_seq = cache->max_seq;
+    a.blocks = blocks->blocks;
+    Q3VL_HIP(launch_kv_pack(a, cache->head_dim, (hipStream_t)stream), "cache packing launch");
+    return Q3VL_OK;
+}
+
+int q3vl_kv_advance(const q3vl_kv_cache *cache, const q3vl_kv_blocks *blocks, int32_t *cache_len,
+                    int32_t *packed_len, q3vl_stream stream) {
+    int rc = check_cache(cache);
+    if (rc || (rc = check_blocks(blocks, cache))) return rc;
+    if (!cache_len || !packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    if (cache_len == packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "cache_len and packed_len are one array");
+    Q3VL_HIP(launch_kv_advance(cache_len, packed_len, cache->batch, cache->max_seq, blocks->blocks, (hipStream_t)stream),
+             "cache lengths launch");
+    return Q3VL_OK;
+}
+
+int q3vl_kv_unpack(const q3vl_kv_blocks *blocks, const int32_t *packed_len, const int32_t *first,
+                   const q3vl_kv_cache *cache, int count, q3vl_stream stream) {
+    int rc = check_cache(cache);
+    if (rc || (rc = check_blocks(blocks, cache))) return rc;
+    if (count < 0 || count > cache->max_seq)
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "count=%d: 0 to the cache's max_seq=%d", count, cache->max_seq);
+    if (count == 0) return Q3VL_OK;
+    if (!packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    if (!blocks_fit(cache, (int64_t)count / 32 + 2))
+        return fail(Q3VL_ERR_UNSUPPORTED, "cache too large: batch=%d kv_heads=%d count=%d", cache->batch, cache->kv_heads, count);
+    KvUnpackArgs a{};
+    a.k8 = blocks->k;
+    a.v8 = blocks->v;
+    a.k_scale = blocks->k_scale;
+    a.v_scale = blocks->v_scale;
+    a.packed_len = packed_len;
+    a.first = first;
+    a.k = cache->k;
+    a.v = cache->v;
+    a.seq_stride = cache->seq_stride;
+    a.head_stride = cache->head_stride;
+    a.row_stride = cache->row_stride;
+    a.batch = cache->batch;
+    a.kv_heads = cache->kv_heads;
+    a.blocks = blocks->blocks;
+    a.count = count;
+    Q3VL_HIP(launch_kv_unpack(a, cache->head_dim, (hipStream_t)stream), "cache unpacking launch");
+    return Q3VL_OK;
+}
+
+static int check_long_attention(size_t rows, int heads, int max_rows, int max_len, int window, int sinks, const q3vl_kv_cache *c,
+                                const q3vl_kv_blocks *p) {
+    int rc = check_tree_attention(rows, heads, max_rows, max_len, c);
+    if (rc || (p && (rc = check_blocks(p, c)))) return rc;
+    if (window < 0 || sinks < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "window=%d sinks=%d", window, sinks);
+    if (sinks && !window) return fail(Q3VL_ERR_INVALID_ARGUMENT, "sinks=%d without a window", sinks);
+    return Q3VL_OK;
+}
+
+size_t q3vl_long_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
+                                           int window, int sinks, const q3vl_kv_cache *cache,
+                                           const q3vl_kv_blocks *blocks) {
+    if (check_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks)) return 0;
+    return 0;
+}
+
+int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,
+                        int heads, const q3vl_kv_cache *cache, const int32_t *row_start,
+                        const int32_t *cache_len, const q3vl_kv_blocks *blocks,
+                        const int32_t *packed_len, const uint64_t *mask, int mask_words,
+                        int max_rows, int max_len, int window, int sinks, float scale,
+                        void *workspace, size_t workspace_bytes, q3vl_stream stream) {
+    int rc = check_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks);
+    if (rc) return rc;
+    if (dtype != Q3VL_DTYPE_FP32 && dtype != Q3VL_DTYPE_FP16)
+        return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
+    const size_t qn = (size_t)heads * cache->head_dim;
+    if (ldq < qn || ldo < qn) return fail(Q3VL_ERR_INVALID_ARGUMENT, "a row stride is shorter than its row");
+    if (out == q && ldo != ldq && rows > 1) return fail(Q3VL_ERR_INVALID_ARGUMENT, "out over q needs q's stride");
+    if (mask_words < 0 || (mask && mask_words < 1) || mask_words > (1 << 24))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "mask_words=%d", mask_words);
+    if (window && mask && window < max_rows)
+        return fail(Q3VL_ERR_UNSUPPORTED, "window=%d over masks of up to %d rows: at least as many are served", window, max_rows);
+    if (!blocks != !packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "blocks and packed_len come together");
+    const float scale_log2e = (float)((double)scale * 1.4426950408889634);
+    if (!(scale_log2e > -INFINITY && scale_log2e < INFINITY))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "scale=%g: not finite, or not times log2 e", (double)scale);
+    if (rows == 0 || max_rows == 0) return Q3VL_OK;
+    if (!q || !out || !row_start || !cache_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    const bool half = dtype == Q3VL_DTYPE_FP16;
+    LongAttnArgs a{};
+    a.q = q;
+    a.out = out;
+    a.ldq = (int64_t)ldq;
+    a.ldo = (int64_t)ldo;
+    a.k_cache = cache->k;
+    a.v_cache = cache->v;
+    a.seq_stride = cache->seq_stride;
+    a.head_stride = cache->head_stride;
+    a.row_stride = cache->row_stride;
+    a.row_start = row_start;
+    a.cache_len = cache_len;
+    a.mask = mask;
+    a.rows = (int)rows;
+    a.heads = heads;
+    a.kv_heads = cache->kv_heads;
+    a.batch = cache->batch;
+    a.max_seq = cache->max_seq;
+    a.max_rows = (size_t)max_rows > rows ? (int)rows : max_rows;
+    a.words = mask_words;
+    a.splits = 1;
+    a.scale_log2e = scale_log2e;
+    if (blocks) {
+        a.k8 = blocks->k;
+        a.v8 = blocks->v;
+        a.k_scale = blocks->k_scale;
+        a.v_scale = blocks->v_scale;
+        a.packed_len = packed_len;
+        a.blocks = blocks->blocks;
+    }
+    a.window = window;
+    a.sinks = sinks;
+    (void)workspace;
+    (void)workspace_bytes;
+    Q3VL_HIP(launch_long_attention(a, cache->head_dim, half, (hipStream_t)stream), "attention launch");
+    return Q3VL_OK;
+}
+
+// ---- drafts judged
+
+size_t q3vl_verify_drafts_workspace_bytes(size_t rows, size_t V) {
+    if (rows == 0 || V == 0 || V > kLogprobMaxV || rows > kLogprobMaxM) return 0;
+    return 2 * align256(rows * 4);
+}
+
+int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *draft_probs, size_t ldp,
+                       const int32_t *tokens, const int32_t *parents, const int32_t *row_start,
+                       const float *accept_u, const float *sample_u, int batch, size_t rows,
+                       size_t V, int max_rows, double temperature, int32_t *accepted, int32_t *path,
+                       int32_t *next, void *workspace, size_t workspace_bytes, q3vl_stream stream) {
+    if (dtype != Q3VL_DTYPE_FP32 && dtype != Q3VL_DTYPE_FP16)
+        return fail(Q3VL_ERR_UNSUPPORTED, "dtype=%d: fp32 or fp16 are served", dtype);
+    if (V == 0 || ld < V || ld > (SIZE_MAX >> 32) || (draft_probs && (ldp < V || ldp > (SIZE_MAX >> 32))))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape V=%zu ld=%zu ldp=%zu", V, ld, ldp);
+    if (batch < 0 || max_rows < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape batch=%d max_rows=%d", batch, max_rows);
+    if (max_rows > kDraftRows)
+        return fail(Q3VL_ERR_UNSUPPORTED, "max_rows=%d: at most %d rows a sequence", max_rows, kDraftRows);
+    const double inv_t = 1.0 / temperature;
+    if (!(temperature > 0.0 && inv_t > 0.0 && inv_t < INFINITY))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "temperature=%g: positive and finite, its reciprocal too", temperature);
+    if (batch == 0) return Q3VL_OK;
+    if (rows > kLogprobMaxM || V > kLogprobMaxV || batch > (1 << 22))
+        return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu V=%zu batch=%d)", rows, V, batch);
+    if (!row_start || !accepted || !next || (max_rows && !path) ||
+        (rows && (!logits || !tokens || !parents || !accept_u || !sample_u)))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
+    if ((uintptr_t)logits % (dtype == Q3VL_DTYPE_FP16 ? 2 : 4)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned logits");
+    if ((uintptr_t)draft_probs % 4) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned draft_probs");
+    char *w = nullptr;
+    if (rows) {
+        const int rc = resolve_ws_rows(workspace, workspace_bytes, q3vl_verify_drafts_workspace_bytes(rows, V), (hipStream_t)stream, &w);
+        if (rc) return rc;
+    }
+    VerifyArgs a{};
+    a.logits = logits;
+    a.ld = (int64_t)ld;
+    a.draft = draft_probs;
+    a.ldp = (int64_t)ldp;
+    a.tokens = tokens;
+    a.parents = parents;
+    a.row_start = row_start;
+    a.accept_u = accept_u;
+    a.sample_u = sample_u;
+    a.batch = batch;
+    a.rows = (int)rows;
+    a.V = (int)V;
+    a.max_rows = max_rows;
+    a.inv_t = inv_t;
+    a.accepted = accepted;
+    a.path = path;
+    a.next = next;
+    a.pick = reinterpret_cast<int32_t *>(w);
+    a.taken = reinterpret_cast<int32_t *>(w + align256(rows * 4));
+    Q3VL_HIP(launch_verify_drafts(a, dtype == Q3VL_DTYPE_FP16, (hipStream_t)stream), "draft judging launch");
     return Q3VL_OK;
 }
 

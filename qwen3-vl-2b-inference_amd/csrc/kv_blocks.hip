@@ -1,0 +1,168 @@
+// kv_blocks.hip -- a cache's whole blocks of 32 positions in 8 bits: written
+// from the fp16 rows, and read back. gfx950.
+#include "q3vl_device.hpp"
+#include "q3vl_kernels.hpp"
+#include "q3vl_kv_blocks.hpp"
+
+namespace q3vl {
+
+namespace {
+
+constexpr int THREADS = 256;
+
+typedef _Float16 half8_row __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+}  // namespace
+
+// Scale and integers of one block: s = max |x| / 127, n = rne(x / s), both
+// divisions correctly rounded, so that the integers are those of their
+// definition in fp32 and no value is further than s / 2 from its own.
+//
+// One workgroup a (sequence, kv head, block): two waves take the keys, two the
+// values. The rows come in whole, 16 bytes a lane; the maximum of the fp16 bits
+// without their sign tells infinities and NaN apart from the rest. The block is
+// put into its order in LDS and leaves in pieces of 16 bytes.
+//
+// The workgroup of a sequence's first block also moves the rows behind the last
+// whole one to the front: fewer than 32, which no other workgroup reads, to
+// rows that this one alone reads, before it writes them.
+template <int D> __global__ __launch_bounds__(THREADS) void kv_pack_kernel(KvPackArgs a, int most) {
+    constexpr int HALF = THREADS / 2, PIECES = BLOCK * D / 8 / HALF;  // pieces of 8 values a thread
+    __shared__ __align__(16) unsigned char tile[2][BLOCK * D];
+    __shared__ int red[THREADS / 64];
+    int x = blockIdx.x;
+    const int j = x % most;
+    x /= most;
+    const int h = x % a.kv_heads, b = x / a.kv_heads;
+    const Fill f = filled(a.cache_len[b], a.packed_len[b], a.max_seq, a.blocks);
+    if (j >= f.whole) return;
+    const int tid = threadIdx.x, part = tid / HALF, t = tid % HALF;  // part 0: keys, 1: values
+    uint16_t *rows = (part ? a.v : a.k) + (size_t)b * a.seq_stride + (size_t)h * a.head_stride;
+    half8_row v[PIECES];
+    int top = 0;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int at = t + p * HALF, r = at / (D / 8), c = at % (D / 8);
+        v[p] = *reinterpret_cast<const half8_row *>(rows + (size_t)(j * BLOCK + r) * a.row_stride + c * 8);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, (int)(__builtin_bit_cast(uint16_t, (_Float16)v[p][e]) & 0x7FFF));
+    }
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) top = max(top, __shfl_xor(top, k));
+    if ((tid & 63) == 0) red[tid >> 6] = top;
+    __syncthreads();
+    top = max(red[2 * part], red[2 * part + 1]);
+    const bool fine = top < 0x7C00;
+    const float s = fine ? h2f((uint16_t)top) / 127.0f : __builtin_nanf("");
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int at = t + p * HALF, r = at / (D / 8), c = at % (D / 8);
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int n = fine && top ? (int)__builtin_rintf((float)v[p][e] / s) : 0;
+            w[e >> 2] |= (uint32_t)(n & 255) << (8 * (e & 3));
+        }
+        if (part == 0) {
+            *reinterpret_cast<u32x2 *>(tile[0] + key_at<D>(r, 8 * c)) = u32x2{w[0], w[1]};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tile[1][value_at<D>(r, 8 * c + e)] = (unsigned char)(w[e >> 2] >> (8 * (e & 3)));
+        }
+    }
+    const size_t to = ((size_t)b * a.kv_heads + h) * a.blocks + f.first + j;
+    if (t == 0) (part ? a.v_scale : a.k_scale)[to] = s;
+    __syncthreads();
+    int8_t *out = (part ? a.v8 : a.k8) + to * (BLOCK * D);
+#pragma unroll
+    for (int p = 0; p < PIECES / 2; ++p) {
+        const int at = (t + p * HALF) * 16;
+        *reinterpret_cast<u32x4 *>(out + at) = *reinterpret_cast<const u32x4 *>(tile[part] + at);
+    }
+    if (j) return;
+    const int rest = f.rest;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+        const int at = t + p * HALF, r = at / (D / 8), c = at % (D / 8);
+        if (r >= rest) continue;
+        const half8_row y = *reinterpret_cast<const half8_row *>(rows + (size_t)(f.whole * BLOCK + r) * a.row_stride + c * 8);
+        *reinterpret_cast<half8_row *>(rows + (size_t)r * a.row_stride + c * 8) = y;
+    }
+}
+
+__global__ __launch_bounds__(THREADS) void kv_advance_kernel(int32_t *cache_len, int32_t *packed_len, int batch, int max_seq, int blocks) {
+    for (int b = blockIdx.x * THREADS + threadIdx.x; b < batch; b += gridDim.x * THREADS) {
+        const Fill f = filled(cache_len[b], packed_len[b], max_seq, blocks);
+        if (!f.whole) continue;
+        packed_len[b] += f.whole * BLOCK;
+        cache_len[b] = f.rest;
+    }
+}
+
+// One workgroup a (sequence, kv head, block that holds a wanted position).
+template <int D> __global__ __launch_bounds__(THREADS) void kv_unpack_kernel(KvUnpackArgs a, int most) {
+    __shared__ __align__(16) unsigned char tile[2][BLOCK * D];
+    int x = blockIdx.x;
+    const int j = x % most;
+    x /= most;
+    const int h = x % a.kv_heads, b = x / a.kv_heads, tid = threadIdx.x;
+    const int first = a.first ? a.first[b] : 0;
+    if (first < 0) return;
+    const int64_t have = min((int64_t)a.packed_len[b], (int64_t)a.blocks * BLOCK);
+    const int64_t end = min((int64_t)first + a.count, have);  // of the positions wanted
+    const int64_t blk = first / BLOCK + j, p0 = blk * BLOCK;
+    if (p0 >= end) return;
+    const size_t from = ((size_t)b * a.kv_heads + h) * a.blocks + blk;
+    constexpr int PIECES = BLOCK * D / 16;  // of one part
+    for (int i = tid; i < 2 * PIECES; i += THREADS) {
+        const int part = i / PIECES, at = i % PIECES * 16;
+        *reinterpret_cast<u32x4 *>(tile[part] + at) = *reinterpret_cast<const u32x4 *>((part ? a.v8 : a.k8) + from * (BLOCK * D) + at);
+    }
+    const float s[2] = {a.k_scale[from], a.v_scale[from]};
+    __syncthreads();
+    for (int i = tid; i < 2 * BLOCK * (D / 8); i += THREADS) {
+        const int part = i / (BLOCK * (D / 8)), r = i / (D / 8) % BLOCK, c = i % (D / 8);
+        const int64_t p = p0 + r;
+        if (p < first || p >= end) continue;
+        uint16_t o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int at = part ? value_at<D>(r, 8 * c + e) : key_at<D>(r, 8 * c + e);
+            o[e] = f2h((float)(int8_t)tile[part][at] * s[part]);
+        }
+        uint16_t *to = (part ? a.v : a.k) + (size_t)b * a.seq_stride + (size_t)h * a.head_stride + (size_t)(p - first) * a.row_stride + 8 * c;
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = o[2 * e] | (uint32_t)o[2 * e + 1] << 16;
+        *reinterpret_cast<u32x4 *>(to) = w;
+    }
+}
+
+hipError_t launch_kv_pack(const KvPackArgs &a, int head_dim, hipStream_t st) {
+    const int64_t most = a.max_seq / BLOCK;
+    if (most == 0) return hipSuccess;  // no whole block fits the cache
+    const unsigned grid = (unsigned)(most * a.kv_heads * a.batch);
+    if (head_dim == 128) kv_pack_kernel<128><<<grid, THREADS, 0, st>>>(a, (int)most);
+    else kv_pack_kernel<64><<<grid, THREADS, 0, st>>>(a, (int)most);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_advance(int32_t *cache_len, int32_t *packed_len, int batch, int max_seq, int blocks, hipStream_t st) {
+    const int grid = (batch + THREADS - 1) / THREADS;
+    kv_advance_kernel<<<grid < 1024 ? grid : 1024, THREADS, 0, st>>>(cache_len, packed_len, batch, max_seq, blocks);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_unpack(const KvUnpackArgs &a, int head_dim, hipStream_t st) {
+    // blocks that `count` positions from anywhere on can touch
+    const int64_t touched = ((int64_t)a.count + BLOCK - 1) / BLOCK + (a.first ? 1 : 0);
+    const int64_t most = touched < a.blocks ? touched : a.blocks;
+    const unsigned grid = (unsigned)(most * a.kv_heads * a.batch);
+    if (head_dim == 128) kv_unpack_kernel<128><<<grid, THREADS, 0, st>>>(a, (int)most);
+    else kv_unpack_kernel<64><<<grid, THREADS, 0, st>>>(a, (int)most);
+    return hipGetLastError();
+}
+
+}  // namespace q3vl

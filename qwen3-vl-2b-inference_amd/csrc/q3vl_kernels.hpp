@@ -268,4 +268,49 @@ int logprob_parts(int M, int V);
 int64_t logprob_parts_most(int M, int V);  // parts of all rows, for up to M rows of up to V values
 hipError_t launch_token_logprobs(const LogprobArgs &a, bool half, hipStream_t st);
 
+// -------------------------------------------------------------- long contexts
+struct KvPackArgs {
+    uint16_t *k, *v;  // fp16 rows
+    size_t seq_stride, head_stride, row_stride;
+    int8_t *k8, *v8;
+    float *k_scale, *v_scale;
+    const int32_t *cache_len, *packed_len;
+    int batch, kv_heads, max_seq, blocks;
+};
+hipError_t launch_kv_pack(const KvPackArgs &a, int head_dim, hipStream_t st);
+hipError_t launch_kv_advance(int32_t *cache_len, int32_t *packed_len, int batch, int max_seq, int blocks, hipStream_t st);
+
+struct KvUnpackArgs {
+    const int8_t *k8, *v8;
+    const float *k_scale, *v_scale;
+    const int32_t *packed_len, *first;  // first may be null
+    uint16_t *k, *v;
+    size_t seq_stride, head_stride, row_stride;
+    int batch, kv_heads, blocks, count;
+};
+hipError_t launch_kv_unpack(const KvUnpackArgs &a, int head_dim, hipStream_t st);
+
+struct LongAttnArgs : TreeAttnArgs {
+    const int8_t *k8, *v8;
+    const float *k_scale, *v_scale;
+    const int32_t *packed_len;  // null: no blocks
+    int blocks;                 // of a kv head
+    int window, sinks;          // window 0: none
+};
+hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, hipStream_t st);
+
+struct VerifyArgs {
+    const void *logits;
+    int64_t ld;
+    const float *draft;  // or null
+    int64_t ldp;
+    const int32_t *tokens, *parents, *row_start;
+    const float *accept_u, *sample_u;
+    int batch, rows, V, max_rows;
+    double inv_t;
+    int32_t *accepted, *path, *next;
+    int32_t *pick, *taken;  // [rows]
+};
+hipError_t launch_verify_drafts(const VerifyArgs &a, bool half, hipStream_t st);
+
 }  // namespace q3vl

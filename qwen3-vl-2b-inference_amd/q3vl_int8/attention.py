@@ -1,12 +1,19 @@
 """Rows of tokens over the caches: the plan of a step's drafts, the head norms
 with the rotary position, and attention of several rows a sequence (a prompt,
-one token of each sequence of a batch, a tree of drafted tokens).
+one token of each sequence of a batch, a tree of drafted tokens); the drafts
+judged; a cache whose whole blocks of 32 positions are held in 8 bits, and
+attention over it or through a window.
 
 The order in a step: draft_plan once; in each layer linear_i8_multi (q, k, v),
 qk_norm_rope, tree_attention, linear_i8 (o); token_logprobs over the logits.
-After a tree is judged, the caller moves the accepted rows' keys and values to
-the positions they now have (their slots are those of their rows) and adds
-their number to cache_len.
+After a tree is judged (verify_drafts, or the ranks of token_logprobs), the
+caller moves the accepted rows' keys and values to the positions they now have
+(their slots are those of their rows) and adds their number to cache_len.
+
+Over 8-bit blocks (PackedKV) the KVCache holds the newest rows alone:
+draft_plan's pos_delta is packed_len, long_attention takes tree_attention's
+place, and at a step's end kv_pack for each layer and kv_advance once move what
+fills whole blocks. kv_unpack brings positions back to an fp16 cache.
 
 KVCache, QKNorm and Rope hold one layer's caches, norm weights and the rotary
 tables with their C descriptions; a program builds them once. The tensors stay
@@ -16,6 +23,7 @@ Every tensor of a call has to be on the current device.
 from __future__ import annotations
 
 import ctypes
+from typing import NamedTuple
 
 from . import FP16, FP32, _check, _need, _ptr, _torch, lib
 
@@ -29,6 +37,11 @@ class _CacheC(ctypes.Structure):
                 ("seq_stride", _sz), ("head_stride", _sz), ("row_stride", _sz)]
 
 
+class _BlocksC(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("batch", _i), ("kv_heads", _i), ("blocks", _i),
+                ("head_dim", _i)]
+
+
 class _NormC(ctypes.Structure):
     _fields_ = [("q_w", _vp), ("q_s", _vp), ("k_w", _vp), ("k_s", _vp), ("group_size", _i), ("eps", ctypes.c_float)]
 
@@ -37,11 +50,11 @@ class _RopeC(ctypes.Structure):
     _fields_ = [("cos", _vp), ("sin", _vp), ("rows", _i), ("axes", _i), ("sections", _i * 3), ("interleaved", _i)]
 
 
-_lib = _plan_fn = _rope_fn = _attn_fn = None
+_lib = _plan_fn = _rope_fn = _attn_fn = _long_fn = _verify_fn = None
 
 
 def _L():
-    global _lib, _plan_fn, _rope_fn, _attn_fn
+    global _lib, _plan_fn, _rope_fn, _attn_fn, _long_fn, _verify_fn
     if _lib is None:
         L = lib()
         sigs = {
@@ -50,11 +63,21 @@ def _L():
             "q3vl_tree_attention_workspace_bytes": (_sz, [_sz, _i, _i, _i, _vp]),
             "q3vl_tree_attention": (_i, [_vp, _sz, _vp, _sz, _i, _sz, _i, _vp, _vp, _vp, _vp, _i, _i, _i, ctypes.c_float,
                                          _vp, _sz, _vp]),
+            "q3vl_kv_pack": (_i, [_vp, _vp, _vp, _vp, _vp]),
+            "q3vl_kv_advance": (_i, [_vp, _vp, _vp, _vp, _vp]),
+            "q3vl_kv_unpack": (_i, [_vp, _vp, _vp, _vp, _i, _vp]),
+            "q3vl_long_attention_workspace_bytes": (_sz, [_sz, _i, _i, _i, _i, _i, _vp, _vp]),
+            "q3vl_long_attention": (_i, [_vp, _sz, _vp, _sz, _i, _sz, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i,
+                                         ctypes.c_float, _vp, _sz, _vp]),
+            "q3vl_verify_drafts_workspace_bytes": (_sz, [_sz, _sz]),
+            "q3vl_verify_drafts": (_i, [_vp, _sz, _i, _vp, _sz, _vp, _vp, _vp, _vp, _vp, _i, _sz, _sz, _i, ctypes.c_double, _vp, _vp,
+                                        _vp, _vp, _sz, _vp]),
         }
         for name, (res, args) in sigs.items():
             fn = getattr(L, name)
             fn.restype, fn.argtypes = res, args
         _plan_fn, _rope_fn, _attn_fn = L.q3vl_draft_plan, L.q3vl_qk_norm_rope, L.q3vl_tree_attention
+        _long_fn, _verify_fn = L.q3vl_long_attention, L.q3vl_verify_drafts
         _lib = L
     return _lib
 
@@ -171,6 +194,39 @@ class KVCache:
         self.c = _CacheC(k.data_ptr(), v.data_ptr(), B, H, S, D, *st)
         self.ref = ctypes.byref(self.c)
         self.device, self.dev = k.device, k.get_device()
+
+
+class PackedKV:
+    """One layer's positions in 8 bits, in blocks of 32: k, v int8 [batch,
+    kv_heads, blocks, 32 * head_dim], k_scale, v_scale fp32 [batch, kv_heads,
+    blocks], contiguous (alloc_packed_kv makes them). kv_pack fills them; the
+    order of a block's values is told in include/q3vl_int8.h."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        torch = _torch()
+        for t, n in ((k, "k"), (v, "v")):
+            _need(t, torch.int8, n, 4)
+        for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            _need(t, torch.float32, n, 3)
+        B, H, N, E = k.shape
+        if v.shape != k.shape or k_scale.shape != (B, H, N) or v_scale.shape != (B, H, N) or E % 32:
+            raise ValueError("k and v must be [batch, kv_heads, blocks, 32 * head_dim] and their scales [batch, kv_heads, blocks]")
+        if len({t.get_device() for t in (k, v, k_scale, v_scale)}) > 1:
+            raise ValueError("the blocks' tensors must be on one device")
+        if k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise ValueError("blocks must be 16-byte aligned")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.c = _BlocksC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), B, H, N, E // 32)
+        self.ref = ctypes.byref(self.c)
+        self.device, self.dev = k.device, k.get_device()
+
+
+def alloc_packed_kv(batch, kv_heads, positions, head_dim, device="cuda"):
+    """A PackedKV for up to `positions` positions of each sequence."""
+    torch = _torch()
+    n = -(-positions // 32)
+    k, v = (torch.zeros((batch, kv_heads, n, 32 * head_dim), dtype=torch.int8, device=device) for _ in range(2))
+    return PackedKV(k, v, *(torch.zeros((batch, kv_heads, n), device=device) for _ in range(2)))
 
 
 class QKNorm:
@@ -346,3 +402,153 @@ def tree_attention(q, cache, row_start, cache_len, max_rows, mask=None, max_len=
     if rc:
         _check(rc)
     return out
+
+
+def _both(cache, packed, dev):
+    if not cache.dev == packed.dev == dev:
+        raise ValueError("cache and packed must be on the current device")
+
+
+def kv_pack(cache, packed, cache_len, packed_len, stream=None):
+    """Packs the whole blocks of 32 among the first cache_len[b] rows of each
+    sequence of the cache behind its packed_len[b] packed positions, and moves
+    the rows left to the cache's front. The lengths (int32 [batch]) stay: they
+    are the same for every layer, and kv_advance moves them on."""
+    torch, dev = _device()
+    _both(cache, packed, dev)
+    _vec(cache_len, torch.int32, cache.c.batch, "cache_len", dev)
+    _vec(packed_len, torch.int32, cache.c.batch, "packed_len", dev)
+    _check(_L().q3vl_kv_pack(cache.ref, packed.ref, cache_len.data_ptr(), packed_len.data_ptr(), _raw_stream(stream, torch, dev)))
+
+
+def kv_advance(cache, packed, cache_len, packed_len, stream=None):
+    """The lengths after kv_pack, in place: whole blocks of cache_len go over to
+    packed_len."""
+    torch, dev = _device()
+    _both(cache, packed, dev)
+    _vec(cache_len, torch.int32, cache.c.batch, "cache_len", dev)
+    _vec(packed_len, torch.int32, cache.c.batch, "packed_len", dev)
+    _check(_L().q3vl_kv_advance(cache.ref, packed.ref, cache_len.data_ptr(), packed_len.data_ptr(), _raw_stream(stream, torch, dev)))
+
+
+def kv_unpack(packed, packed_len, cache, first=None, count=None, stream=None):
+    """Packed positions first[b] .. first[b] + count - 1 below packed_len[b] (int32
+    [batch]; first None: from 0) to the cache's rows 0 .. count - 1 as fp16.
+    count: default what the packed blocks hold, at most the cache's rows."""
+    torch, dev = _device()
+    _both(cache, packed, dev)
+    c = cache.c
+    _vec(packed_len, torch.int32, c.batch, "packed_len", dev)
+    if first is not None:
+        _vec(first, torch.int32, c.batch, "first", dev)
+    if count is None:
+        count = min(32 * packed.c.blocks, c.max_seq)
+    _check(_L().q3vl_kv_unpack(packed.ref, packed_len.data_ptr(), _ptr(first), cache.ref, count, _raw_stream(stream, torch, dev)))
+
+
+def long_attention_workspace_bytes(cache, rows, heads, max_rows, max_len=None, packed=None, window=0, sinks=0) -> int:
+    return _L().q3vl_long_attention_workspace_bytes(rows, heads, max_rows, max_len or 0, window, sinks, cache.ref,
+                                                    None if packed is None else packed.ref)
+
+
+def alloc_long_attention_workspace(cache, rows, heads, max_rows, max_len=None, packed=None, window=0, sinks=0):
+    """Device workspace for long_attention at these sizes."""
+    n = long_attention_workspace_bytes(cache, rows, heads, max_rows, max_len, packed, window, sinks)
+    return _torch().empty(max(n, 256), dtype=_torch().uint8, device=cache.device)
+
+
+def long_attention(q, cache, row_start, cache_len, max_rows, packed=None, packed_len=None, window=0, sinks=0, mask=None, max_len=None,
+                   scale=None, out=None, workspace=None, stream=None):
+    """tree_attention over the packed_len[b] positions of `packed` and, behind
+    them, those of the cache; through a window where one is given: of what a row
+    would see it sees the first `sinks` positions and the last `window` (with a
+    mask at least max_rows). packed None: the cache alone. max_len counts packed
+    positions too. The rest as tree_attention. workspace:
+    alloc_long_attention_workspace with the same packed, max_rows, max_len,
+    window and sinks."""
+    torch, dev = _device()
+    ldq = _rows(q, (torch.float32, torch.float16), "q", dev)
+    c = cache.c
+    D, batch = c.head_dim, c.batch
+    rows, qn = q.shape
+    if qn % D:
+        raise ValueError("q's rows must be whole heads of the cache's head_dim")
+    if cache.dev != dev:
+        raise ValueError("cache must be on the current device")
+    if (packed is None) != (packed_len is None):
+        raise ValueError("packed and packed_len come together")
+    if out is None:
+        out = _empty(q, stream, rows, qn)
+        ldo = qn
+    else:
+        ldo = _rows(out, (q.dtype,), "out", dev)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    _vec(row_start, torch.int32, batch + 1, "row_start", dev)
+    _vec(cache_len, torch.int32, batch, "cache_len", dev)
+    pref = plen = None
+    if packed is not None:
+        if packed.dev != dev:
+            raise ValueError("packed must be on the current device")
+        _vec(packed_len, torch.int32, batch, "packed_len", dev)
+        pref, plen = packed.ref, packed_len.data_ptr()
+    words = 0 if mask is None else _mask_words(mask, rows, dev)
+    wp, wb = _workspace(workspace, dev)
+    rc = (_long_fn or _L().q3vl_long_attention)(
+        q.data_ptr(), ldq, out.data_ptr(), ldo, FP16 if q.dtype is torch.float16 else FP32, rows, qn // D, cache.ref,
+        row_start.data_ptr(), cache_len.data_ptr(), pref, plen, _ptr(mask), words, max_rows, max_len or 0, window, sinks,
+        D ** -0.5 if scale is None else scale, wp, wb, _raw_stream(stream, torch, dev))
+    if rc:
+        _check(rc)
+    return out
+
+
+class VerifiedDrafts(NamedTuple):
+    accepted: object  # int32 [batch]: rows that stay, the first among them
+    path: object      # int32 [batch, max_rows]: their indexes in the sequence, then -1
+    next: object      # int32 [batch]: the token after the last of them
+
+
+def alloc_verify_drafts_workspace(rows, V, device="cuda"):
+    """Device workspace for verify_drafts over up to `rows` rows of up to V logits."""
+    torch = _torch()
+    return torch.empty(max(256, _L().q3vl_verify_drafts_workspace_bytes(rows, V)), dtype=torch.uint8, device=device)
+
+
+def verify_drafts(logits, tokens, parents, row_start, accept_u, sample_u, max_rows, draft_probs=None, temperature=1.0, workspace=None,
+                  stream=None):
+    """Rejection sampling of drafted tokens (int32 [rows], parents and row_start
+    as for draft_plan; row 0 of a sequence is the token chosen last) against
+    softmax(logits / temperature), logits [rows, V] fp32 or fp16: which rows
+    stay and the token after them, a VerifiedDrafts. draft_probs fp32 [rows, V]:
+    what each row's children were drawn from (None: the draft is certain of
+    them). accept_u, sample_u fp32 [rows], uniform in [0, 1). max_rows: the most
+    rows of one sequence, at most 1024."""
+    torch, dev = _device()
+    f32, i32 = torch.float32, torch.int32
+    ld = _rows(logits, (f32, torch.float16), "logits", dev)
+    rows, V = logits.shape
+    ldp = 0
+    if draft_probs is not None:
+        ldp = _rows(draft_probs, (f32,), "draft_probs", dev)
+        if draft_probs.shape != logits.shape:
+            raise ValueError("draft_probs must have the logits' shape")
+    _vec(row_start, i32, None, "row_start", dev)
+    batch = row_start.numel() - 1
+    if batch < 0:
+        raise ValueError("row_start must hold at least one value")
+    _vec(tokens, i32, rows, "tokens", dev)
+    _vec(parents, i32, rows, "parents", dev)
+    _vec(accept_u, f32, rows, "accept_u", dev)
+    _vec(sample_u, f32, rows, "sample_u", dev)
+    if max_rows < 0:
+        raise ValueError("max_rows must not be negative")
+    accepted, path, nxt = _empty(tokens, stream, batch), _empty(tokens, stream, batch, max_rows), _empty(tokens, stream, batch)
+    wp, wb = _workspace(workspace, dev)
+    rc = (_verify_fn or _L().q3vl_verify_drafts)(
+        logits.data_ptr(), ld, FP16 if logits.dtype is torch.float16 else FP32, _ptr(draft_probs), ldp, tokens.data_ptr(),
+        parents.data_ptr(), row_start.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), batch, rows, V, max_rows, temperature,
+        accepted.data_ptr(), path.data_ptr(), nxt.data_ptr(), wp, wb, _raw_stream(stream, torch, dev))
+    if rc:
+        _check(rc)
+    return VerifiedDrafts(accepted, path, nxt)

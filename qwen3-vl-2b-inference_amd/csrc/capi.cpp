@@ -1772,11 +1772,32 @@ static int check_long_attention(size_t rows, int heads, int max_rows, int max_le
     return Q3VL_OK;
 }
 
+// A call's tile and splits, and its workspace bytes. Through a window a
+// workgroup's rows see its positions, the first ones and their own.
+static TreePlan plan_long_attention(size_t rows, int heads, int max_rows, int max_len, int window, int sinks, const q3vl_kv_cache *c,
+                                    const q3vl_kv_blocks *p, bool half, bool chain, size_t *bytes) {
+    if ((size_t)max_rows > rows) max_rows = (int)rows;
+    const int64_t room = (int64_t)c->max_seq + (p ? (int64_t)p->blocks * 32 : 0);
+    int64_t len = max_len && max_len < room ? max_len : room;
+    if (window && (int64_t)window + sinks + max_rows < len) len = (int64_t)window + sinks + max_rows;
+    if (len > INT32_MAX - 256) len = INT32_MAX - 256;
+    const TreePlan t = tree_attention_plan((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, (int)len, c->head_dim, half, chain);
+    const size_t parts = rows * (size_t)heads * (size_t)t.splits;
+    *bytes = t.splits > 1 ? align256(parts * (size_t)c->head_dim * 4) + align256(parts * 8) : 0;
+    return t;
+}
+
 size_t q3vl_long_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
                                            int window, int sinks, const q3vl_kv_cache *cache,
                                            const q3vl_kv_blocks *blocks) {
     if (check_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks)) return 0;
-    return 0;
+    size_t most = 0;
+    for (int i = 0; i < 4; ++i) {  // types, chains and trees
+        size_t bytes = 0;
+        plan_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks, i & 1, i >> 1, &bytes);
+        most = bytes > most ? bytes : most;
+    }
+    return most;
 }
 
 int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dtype, size_t rows,
@@ -1803,6 +1824,10 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     if (rows == 0 || max_rows == 0) return Q3VL_OK;
     if (!q || !out || !row_start || !cache_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     const bool half = dtype == Q3VL_DTYPE_FP16;
+    size_t need = 0;
+    const TreePlan plan = plan_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks, half, !mask, &need);
+    char *w = nullptr;
+    if (need && (rc = resolve_ws_rows(workspace, workspace_bytes, need, (hipStream_t)stream, &w))) return rc;
     LongAttnArgs a{};
     a.q = q;
     a.out = out;
@@ -1823,7 +1848,9 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     a.max_seq = cache->max_seq;
     a.max_rows = (size_t)max_rows > rows ? (int)rows : max_rows;
     a.words = mask_words;
-    a.splits = 1;
+    a.part_o = reinterpret_cast<float *>(w);
+    a.part_ml = need ? reinterpret_cast<float *>(w + align256(rows * (size_t)heads * plan.splits * cache->head_dim * 4)) : nullptr;
+    a.splits = plan.splits;
     a.scale_log2e = scale_log2e;
     if (blocks) {
         a.k8 = blocks->k;
@@ -1835,9 +1862,7 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     }
     a.window = window;
     a.sinks = sinks;
-    (void)workspace;
-    (void)workspace_bytes;
-    Q3VL_HIP(launch_long_attention(a, cache->head_dim, half, (hipStream_t)stream), "attention launch");
+    Q3VL_HIP(launch_long_attention(a, cache->head_dim, half, plan.rows, (hipStream_t)stream), "attention launch");
     return Q3VL_OK;
 }
 

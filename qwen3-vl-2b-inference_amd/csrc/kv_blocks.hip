@@ -12,7 +12,6 @@ constexpr int THREADS = 256;
 
 typedef _Float16 half8_row __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 }  // namespace
 

@@ -1,9 +1,14 @@
 // long_attention.hip -- attention over long contexts: positions in 8-bit blocks
 // and the fp16 rows behind them, all of them or a window of them with a few
 // first ones. gfx950.
+#include "q3vl_attention.hpp"
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 #include "q3vl_kv_blocks.hpp"
+#include "q3vl_mfma.hpp"
+
+#include <type_traits>
+#include <utility>
 
 namespace q3vl {
 
@@ -175,43 +180,806 @@ __device__ void long_row(const LongAttnArgs &a, const LongSeq &s, int b, int t, 
     }
 }
 
-template <bool HALF> __device__ __forceinline__ void put(void *out, int64_t at, float v) {
-    if (HALF) static_cast<uint16_t *>(out)[at] = f2h(v);
-    else static_cast<float *>(out)[at] = v;
-}
-
 }  // namespace
 
-// One workgroup a row and query head.
-template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void long_row_kernel(LongAttnArgs a) {
-    __shared__ LongScratch sh;
-    int x = blockIdx.x;
-    const int head = x % a.heads;
-    x /= a.heads;
-    const int t = x % a.max_rows, b = x / a.max_rows, tid = threadIdx.x;
+// ------------------------------------------------------------ the kernel
+template <int D, int NR, bool SHARED, bool PACKED> struct LongTile {
+    static constexpr int RB = 2 * D;                           // bytes of an fp16 row
+    static constexpr int NS = SHARED ? 2 : PACKED ? 128 / D : 256 / D;  // stages of fp16 rows
+    static constexpr int STAGE = (SHARED ? 64 : 32) * RB * 2;  // K, then V
+    static constexpr int RING = (SHARED ? 1 : WAVES) * NS * STAGE;
+    static constexpr int BM = 16 * NR * (SHARED ? WAVES : 1);  // query rows of a workgroup
+    static constexpr int OS = D + 4;                           // floats of a joined row (spread over the banks)
+    static constexpr int JOIN = SHARED ? 0 : WAVES * BM * OS * 4;
+    static constexpr int ML = RING > JOIN ? RING : JOIN;       // (M, l) of each wave's rows
+    static constexpr int FLAG = ML + (SHARED ? 0 : WAVES * BM * 8);
+    static constexpr int LDS = FLAG + (BM + 1) * 4;
+    static constexpr int UNIT = SHARED ? 64 : 32 * WAVES;      // positions of a turn
+    static_assert(LDS <= 160 * 1024 && sizeof(LongScratch) <= (size_t)RING, "LDS");
+};
+
+// A block of 32 packed positions on its way to the operands.
+template <int D> struct PackedBlock {
+    u32x4 k[2 * D / 64], v[D / 32];
+    float ks, vs;
+};
+
+template <int D, bool HALF, int NR, bool SHARED, bool PACKED>
+__global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) void long_attention_kernel(
+    const int32_t *row_start_p, const int32_t *cache_len_p, const void *q_p, const int32_t *packed_len_p, int kv_heads_p, int heads_p,
+    int splits_p, int rows_p, int max_rows_p, int max_seq_p, int tiles, int paired, LongAttnArgs args) {
+    LongAttnArgs a = args;  // (the leading arguments arrive in registers)
+    a.row_start = row_start_p;
+    a.cache_len = cache_len_p;
+    a.q = q_p;
+    a.packed_len = PACKED ? packed_len_p : nullptr;
+    a.kv_heads = kv_heads_p;
+    a.heads = heads_p;
+    a.splits = splits_p;
+    a.rows = rows_p;
+    a.max_rows = max_rows_p;
+    a.max_seq = max_seq_p;
+    using T = LongTile<D, NR, SHARED, PACKED>;
+    constexpr int KS = D / 32, NT = D / 16, NQ = HALF ? 1 : 2, UNIT = T::UNIT;
+    extern __shared__ __align__(16) unsigned char smem[];
+    // (loads with an LDS destination take its offset: 0, as the kernel has no other LDS)
+    const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
+    int x = blockIdx.x;  // kv head, split, tile, sequence
+    const int h = x % a.kv_heads;
+    x /= a.kv_heads;
+    const int split = x % a.splits;
+    x /= a.splits;
+    const int b = x / tiles;
+    x -= b * tiles;
+    // a chain's last rows see most: they go first, and where every workgroup has
+    // a place at once, the second half goes the other way round
+    const int tile = paired && 2 * x >= tiles ? x - (tiles + 1) / 2 : tiles - 1 - x;
     const LongSeq s = long_sequence(a, b);
-    if (t >= s.n) return;
-    const int64_t at = (int64_t)(s.start + t) * a.ldo + (int64_t)head * D + tid;
+    const int group = a.heads / a.kv_heads;
+    const int n = min(s.n, a.max_rows), nrows = n * group, r0 = tile * T::BM;
+    if (r0 >= nrows) return;
+
+    int row[NR], tok[NR], head[NR];  // of column i: its row, token, query head
+    bool live[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        row[nr] = r0 + (SHARED ? wid * 16 * NR : 0) + nr * 16 + i;
+        live[nr] = row[nr] < nrows;
+        tok[nr] = live[nr] ? row[nr] / group : 0;
+        head[nr] = h * group + (live[nr] ? row[nr] - tok[nr] * group : 0);
+    }
     if (!s.ok) {
-        if (tid < D) put<HALF>(a.out, at, __builtin_nanf(""));
+        if (a.splits == 1)
+            for (int e = tid; e < min(T::BM, nrows - r0) * D; e += THREADS) {
+                const int r = r0 + e / D, t = r / group;
+                put<HALF>(a.out, (int64_t)(s.start + t) * a.ldo + (int64_t)(h * group + r - t * group) * D + e % D, __builtin_nanf(""));
+            }
         return;
     }
-    const Turns<THREADS> turns = turns_of<THREADS>(a, s, s.len + (a.mask ? s.n : t + 1), window_from(a, s, t));
-    float o, m, l;
-    long_row<D, HALF, THREADS>(a, s, b, t, head, turns, 0, turns.count, sh, o, m, l);
-    if (tid < D) put<HALF>(a.out, at, m == -INFINITY ? 0.0f : o / l);
+
+    // ---- this workgroup's turns
+    const int before = s.packed + s.len;  // positions before the step's
+    const int first_tok = (r0 + (SHARED ? wid * 16 * NR : 0)) / group;  // of this wave's rows
+    const int tile_tok = r0 / group, last_tok = min((r0 + T::BM - 1) / group, n - 1);
+    const int total = s.len + (a.mask ? s.n : last_tok + 1);  // fp16 rows that some row sees
+    const Turns<UNIT> turns = turns_of<UNIT>(a, s, total, (int64_t)before + (a.mask ? 0 : tile_tok + 1) - a.window);
+    const int u0 = (int)((int64_t)turns.count * split / a.splits), u1 = (int)((int64_t)turns.count * (split + 1) / a.splits);
+
+    int tp = u0;  // turns [u0, tp) are of packed positions (turns.at rises: they come first)
+    if constexpr (PACKED) {
+        const int end = turns.first < turns.packed ? max(turns.first, turns.packed - turns.skip) : turns.packed;
+        tp = min(max(end, u0), u1);
+    }
+
+    // ---- queries (the first tiles' loads go out behind theirs, before they are used)
+    half8_any qh[NR][KS];
+    float4_any qs[NR][KS][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        const int64_t at = (int64_t)(s.start + tok[nr]) * a.ldq + (int64_t)head[nr] * D + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if constexpr (HALF) {
+                qh[nr][ks] = *reinterpret_cast<const half8_any *>(static_cast<const _Float16 *>(a.q) + at + 32 * ks);
+            } else {
+                const float *p = static_cast<const float *>(a.q) + at + 32 * ks;
+                qs[nr][ks][0] = *reinterpret_cast<const float4_any *>(p);
+                qs[nr][ks][1] = *reinterpret_cast<const float4_any *>(p + 4);
+            }
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- loads of fp16 rows: a lane's place in 16 rows of the cache, and of LDS
+    const size_t head_at = (size_t)b * a.seq_stride + (size_t)h * a.head_stride;
+    const int rsb = (int)(a.row_stride * 2);
+    constexpr int NL = (SHARED ? 1 : 2) * (D / 32);  // loads of a K or V part
+    int voff[NL];
+#pragma unroll
+    for (int t = 0; t < NL; ++t) {
+        const int r = (t * 64 + lane) / (D / 8), c = lane % (D / 8);
+        voff[t] = (r + (SHARED ? wid * 16 : 0)) * rsb + (c ^ swizzle<D>(r)) * 16;
+    }
+    // rows from p on, `left` of them there: 32 to this wave's own stage, or its
+    // 16 of a tile's 64. Rows past the end read as zeros by the buffer's bounds.
+    auto load_rows = [&](const uint16_t *p, int left, int lds) {
+        left = min(left, SHARED ? 64 : 32);
+        const rsrc_t r = make_rsrc(p, left > 0 ? (uint32_t)((left - 1) * rsb + 2 * D) : 0);
+#pragma unroll
+        for (int t = 0; t < NL; ++t) {
+            const int at = lds + ((SHARED ? wid * NL : 0) + t) * 1024;
+            if constexpr (!SHARED) dma16_nt(r, voff[t], 0, at);
+            else dma16(r, voff[t], 0, at);
+        }
+    };
+    const size_t head_blocks = ((size_t)b * a.kv_heads + h) * a.blocks;
+    const int held = s.packed / BLOCK;
+    // (SHARED) turn u's fp16 rows to LDS at `lds`
+    auto load_tile = [&](int u, int lds) {
+        const int first = (u - turns.packed) * UNIT;
+        const size_t at = head_at + (size_t)first * a.row_stride;
+        load_rows(a.k_cache + at, total - first, lds);
+        load_rows(a.v_cache + at, total - first, lds + 64 * T::RB);
+    };
+    // ... its two packed blocks: this wave's quarter of the keys and of the values
+    // to registers, and from there, widened, to LDS, in the operands' order
+    constexpr int PER = SHARED && PACKED ? 2 * BLOCK * D / 1024 / WAVES : 1;  // KiB of int8
+    u32x4 nk[PER], nv[PER];
+    auto fetch_tile = [&](int u) {
+        const int left = min(held - u * 2, 2) * (BLOCK * D);  // bytes of a part
+        const size_t at = (head_blocks + u * 2) * (BLOCK * D);
+        const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.k8 + at), 0, left, 0x00020000);
+        const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.v8 + at), 0, left, 0x00020000);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) nk[k] = __builtin_amdgcn_raw_buffer_load_b128(rk, (wid * PER + k) * 1024 + lane * 16, 0, 0);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) nv[k] = __builtin_amdgcn_raw_buffer_load_b128(rv, (wid * PER + k) * 1024 + lane * 16, 0, 0);
+    };
+    auto widen_tile = [&](int lds) {
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+            unsigned char *p = smem + lds + (wid * PER + k) * 2048 + lane * 16;
+            *reinterpret_cast<half8_t *>(p) = widen8_plain(nk[k][0], nk[k][1]);
+            *reinterpret_cast<half8_t *>(p + 1024) = widen8_plain(nk[k][2], nk[k][3]);
+            *reinterpret_cast<half8_t *>(p + 64 * T::RB) = widen8_plain(nv[k][0], nv[k][1]);
+            *reinterpret_cast<half8_t *>(p + 64 * T::RB + 1024) = widen8_plain(nv[k][2], nv[k][3]);
+        }
+    };
+
+    // ---- operand registers, the score's factor
+    half8_t qf[NR][NQ][KS];
+    float sc[NR];
+    auto queries = [&] {
+        const float sign = a.scale_log2e < 0.0f ? -1.0f : a.scale_log2e == 0.0f ? 0.0f : 1.0f;
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            sc[nr] = sign == 0.0f ? 1.0f : fabsf(a.scale_log2e);
+            if constexpr (HALF) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) qf[nr][0][ks][e] = live[nr] ? (_Float16)(qh[nr][ks][e] * (_Float16)sign) : (_Float16)0.0f;
+            } else {
+                float v[KS][8], top = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        v[ks][e] = live[nr] ? qs[nr][ks][e >> 2][e & 3] * sign : 0.0f;
+                        top = fmaxf(top, fabsf(v[ks][e]));
+                    }
+                top = column_max(top);
+                // the largest value to [2^13, 2^14)
+                const int shift = top > 0.0f && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+                sc[nr] = ldexpf(sc[nr], -shift);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float y = ldexpf(v[ks][e], shift);
+                        qf[nr][0][ks][e] = (_Float16)y;
+                        qf[nr][1][ks][e] = (_Float16)(y - (float)qf[nr][0][ks][e]);
+                    }
+            }
+        }
+    };
+
+    // ---- what a row's window holds: positions from lo[] on, and below `sinks`
+    int lo[NR], lo_most = INT_MIN;  // (lo_most: of this wave's rows)
+    const bool windowed = a.window != 0;
+    if (windowed) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) lo[nr] = (int)max(window_from(a, s, tok[nr]), (int64_t)INT_MIN);
+        const int last = min((r0 + (SHARED ? (wid + 1) * 16 * NR : T::BM) - 1) / group, n - 1);
+        const int64_t most = (int64_t)before + (a.mask ? min((int64_t)0, (int64_t)s.n - a.window) : (int64_t)last + 1 - a.window);
+        lo_most = (int)max(most, (int64_t)INT_MIN);
+    }
+    // whether all of this wave's rows see positions j .. j + 31, as far as the window goes
+    auto inside = [&](int j) { return !windowed || j >= lo_most || j + 32 <= a.sinks; };
+    auto window_bits = [&](int nr, int j) {
+        auto from = [](int k) { return k <= 0 ? 0xFFFFFFFFu : k >= 32 ? 0u : 0xFFFFFFFFu << k; };  // bits from k on
+        return from(lo[nr] - j) | ~from(a.sinks - j);
+    };
+    // fp16 rows below this are seen by all of this wave's rows, as far as the mask goes
+    const int clear = min(s.len + (a.mask ? 0 : min(first_tok, n - 1) + 1), total);
+
+    // ---- one step: 32 positions
+    int kaddr[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kaddr[ks] = i * T::RB + ((ks * 4 + g) ^ swizzle<D>(i)) * 16;
+    const int vr = 4 * g + (i >> 2);  // row of a 16-position tile this lane's transposing read starts from
+    const int vaddr = vr * T::RB + (((i & 3) >> 1) ^ swizzle<D>(vr)) * 16 + (i & 1) * 8;
+    float M[NR], bias[NR], limit[NR], room[NR];  // limit: the score from which M is set anew, M + room
+    float4_t O[NT][NR], L[NR];  // L: the sum of p, in each register and lane of the column,
+    float lsum[NR];             // and of packed positions, this lane's share
+    bool any[NR];
+    auto clear_rows = [&] {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            M[nr] = limit[nr] = -INFINITY;
+            room[nr] = GROW / sc[nr];
+            bias[nr] = lsum[nr] = 0.0f;
+            any[nr] = false;
+            L[nr] = float4_t{0, 0, 0, 0};
+#pragma unroll
+            for (int dt = 0; dt < NT; ++dt) O[dt][nr] = float4_t{0, 0, 0, 0};
+        }
+    };
+    float4_t S[2][NR];
+    half8_t P[NR][NQ];
+    auto zero_scores = [&](int kb) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) S[kb][nr] = float4_t{0, 0, 0, 0};
+    };
+    auto score = [&](half8_t f, int kb, int ks) {
+#pragma unroll
+        for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) S[kb][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, qf[nr][q][ks], S[kb][nr], 0, 0, 0);
+    };
+    auto value = [&](half8_t f, int dt) {
+#pragma unroll
+        for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) O[dt][nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, P[nr][q], O[dt][nr], 0, 0, 0);
+    };
+    auto masked = [&](int nr, uint32_t w) {  // scores of positions whose bit is not set
+        any[nr] = any[nr] || w;
+        w >>= 4 * g;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(w >> (16 * kb + e) & 1)) S[kb][nr][e] = -INFINITY;
+    };
+    // probabilities of scores ks S; those of packed positions times the values' scale
+    auto softmax = [&](float ks, float vs, auto packed) {
+        float top[NR];  // of this lane's positions
+        bool grow = false;
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            top[nr] = S[0][nr][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top[nr] = fmaxf(top[nr], S[e >> 2][nr][e & 3]);
+            if constexpr (packed) top[nr] *= ks;
+            grow = grow || top[nr] > limit[nr];
+        }
+        if (__any(grow)) {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                const float m = fmaxf(M[nr], column_max(top[nr]));
+                const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], BASE);
+                const float f = M[nr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(nb - bias[nr]);
+                M[nr] = m;
+                limit[nr] = m + room[nr];
+                bias[nr] = nb;
+                L[nr] *= f;
+                if constexpr (PACKED) lsum[nr] *= f;
+#pragma unroll
+                for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= f;
+            }
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            const float c = packed ? sc[nr] * ks : sc[nr];
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(S[e >> 2][nr][e & 3], c, bias[nr]));
+            if constexpr (packed) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) lsum[nr] += p[e];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] *= vs;
+                    // (the product as it is rounded here: fused into the conversion below, the
+                    // first term would now and then be another than the one the rest is of)
+                    asm("" : "+v"(p[e]));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                P[nr][0][e] = (_Float16)p[e];
+                if constexpr (!HALF) P[nr][1][e] = (_Float16)(p[e] - (float)P[nr][0][e]);
+            }
+        }
+    };
+    constexpr std::integral_constant<bool, true> kPacked{};
+    constexpr std::integral_constant<bool, false> kRows{};
+
+    // Values of packed positions come out in units of U, a power of two that the
+    // largest scale of values so far fits.
+    float U = 0.0f, to_units = 0.0f;
+    auto new_units = [&](float vs) {
+        if (vs > U) {  // (uniform)
+            const int e = __builtin_amdgcn_frexp_expf(vs);
+            const float r = U > 0.0f ? ldexpf(U, -e) : 0.0f;
+            U = ldexpf(1.0f, e);
+            to_units = ldexpf(1.0f, -e);
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= r;
+        }
+    };
+    auto packed_softmax = [&](float ks, float vs, int j) {
+        if (inside(j)) {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) any[nr] = true;
+        } else {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) masked(nr, window_bits(nr, j));
+        }
+        softmax(ks, vs * to_units, kPacked);
+    };
+    // 32 packed positions from j on, out of registers
+    auto packed_step = [&](const PackedBlock<D> &f, int j) {
+        new_units(f.vs);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            zero_scores(kb);
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) {
+                const u32x4 w = f.k[kb * (D / 64) + c];
+                score(widen8_plain(w[0], w[1]), kb, 2 * c);
+                score(widen8_plain(w[2], w[3]), kb, 2 * c + 1);
+            }
+        }
+        packed_softmax(f.ks, f.vs, j);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+            const u32x4 w = f.v[c];
+            value(widen8_plain(w[0], w[1]), 2 * c);
+            value(widen8_plain(w[2], w[3]), 2 * c + 1);
+        }
+    };
+    auto leave_units = [&] {  // O in the values' own units
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= U;
+    };
+
+    // 32 fp16 rows from row j on, K and V at LDS offsets. Operand reads, half a
+    // step's at a time: the next half is on its way while the matrix cores work on
+    // this one.
+    const half8_t ones = {(_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1, (_Float16)1};
+    half8_t ka[KS], kb[KS], va[NT / 2], vb[NT / 2];
+    auto read_k = [&](half8_t (&f)[KS], int klds, int t) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) f[ks] = *reinterpret_cast<const half8_t *>(smem + klds + kaddr[ks] + t * 16 * T::RB);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto read_v = [&](half8_t (&f)[NT / 2], int vlds, int part) {
+#pragma unroll
+        for (int t = 0; t < NT / 2; ++t) {
+            const int dt = part * (NT / 2) + t;
+            const half4_t low = read_transposed(smem + vlds + (vaddr ^ (dt * 32)));
+            const half4_t high = read_transposed(smem + vlds + (vaddr ^ (dt * 32)) + 16 * T::RB);
+            f[t] = __builtin_shufflevector(low, high, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto scores = [&](const half8_t (&f)[KS], int t) {
+        zero_scores(t);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) score(f[ks], t, ks);
+    };
+    auto values = [&](const half8_t (&f)[NT / 2], int part) {
+#pragma unroll
+        for (int t = 0; t < NT / 2; ++t) value(f[t], part * (NT / 2) + t);
+    };
+    auto rows_softmax = [&](int j) {
+        const bool in = inside(s.packed + j);
+        if (j + 32 > clear || !in) {  // some positions are not for every row
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                uint32_t w;
+                if (a.mask) {
+                    w = mask_window(a.mask + (size_t)(s.start + tok[nr]) * a.words, a.words, s.n, j - s.len);
+                } else {
+                    const int left = s.len + tok[nr] + 1 - j;
+                    w = left >= 32 ? 0xFFFFFFFFu : left > 0 ? (1u << left) - 1 : 0;
+                }
+                if (total - j < 32) w &= total > j ? (1u << (total - j)) - 1 : 0;
+                if (!in) {
+                    uint32_t win = window_bits(nr, s.packed + j);
+                    if (a.mask && j + 32 > s.len) win |= j >= s.len ? 0xFFFFFFFFu : 0xFFFFFFFFu << (s.len - j);  // (the step's own rows)
+                    w &= win;
+                }
+                masked(nr, w);
+            }
+        } else {
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) any[nr] = true;
+        }
+        softmax(1.0f, 1.0f, kRows);
+    };
+    auto sums = [&] {
+#pragma unroll
+        for (int q = NQ - 1; q >= 0; --q)
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) L[nr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, P[nr][q], L[nr], 0, 0, 0);
+    };
+
+    if constexpr (SHARED) {
+        int lds = 0;
+        if constexpr (PACKED) {
+            if (u0 < tp) {
+                fetch_tile(turns.at(u0));
+                widen_tile(0);
+                if (u0 + 1 < tp) fetch_tile(turns.at(u0 + 1));
+            }
+        }
+        if (u0 >= tp && u0 < u1) load_tile(turns.at(u0), 0);
+        queries();
+        clear_rows();
+        if constexpr (PACKED) {
+            for (int t = u0; t < tp; ++t, lds = T::STAGE - lds) {
+                const int u = turns.at(t);
+                lds_barrier();  // the tile is there, and every wave is done with the other buffer
+                if (t + 1 < tp) {
+                    widen_tile(T::STAGE - lds);
+                    if (t + 2 < tp) fetch_tile(turns.at(t + 2));
+                } else if (t + 1 < u1) {
+                    load_tile(turns.at(t + 1), T::STAGE - lds);
+                }
+                const int end = min(held - u * 2, 2);
+#pragma unroll 1
+                for (int k = 0; k < end; ++k) {
+                    const int blk = u * 2 + k;
+                    const float ks = a.k_scale[head_blocks + blk], vs = a.v_scale[head_blocks + blk];
+                    const unsigned char *p = smem + lds + k * 64 * D + lane * 16;
+                    auto keys = [&](half8_t (&f)[KS], int kb) {
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) f[i] = *reinterpret_cast<const half8_t *>(p + (kb * KS + i) * 1024);
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    auto vals = [&](half8_t (&f)[NT / 2], int part) {
+#pragma unroll
+                        for (int i = 0; i < NT / 2; ++i)
+                            f[i] = *reinterpret_cast<const half8_t *>(p + 64 * T::RB + (part * (NT / 2) + i) * 1024);
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    keys(ka, 0);
+                    keys(kb, 1);
+                    new_units(vs);
+                    scores(ka, 0);
+                    scores(kb, 1);
+                    vals(va, 0);
+                    packed_softmax(ks, vs, blk * BLOCK);
+                    vals(vb, 1);
+                    values(va, 0);
+                    values(vb, 1);
+                }
+            }
+            if (U > 0.0f) leave_units();
+        }
+        for (int t = tp; t < u1; ++t, lds = T::STAGE - lds) {
+            const int j = (turns.at(t) - turns.packed) * UNIT;
+            dma_wait<0>();
+            lds_barrier();
+            if (t + 1 < u1) load_tile(turns.at(t + 1), T::STAGE - lds);
+            read_k(ka, lds, 0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int klds = lds + k * 32 * T::RB, vlds = klds + 64 * T::RB;
+                read_k(kb, klds, 1);
+                scores(ka, 0);
+                scores(kb, 1);
+                read_v(va, vlds, 0);
+                rows_softmax(j + k * 32);
+                read_v(vb, vlds, 1);
+                sums();
+                values(va, 0);
+                if (k == 0) read_k(ka, klds + 32 * T::RB, 0);
+                values(vb, 1);
+            }
+        }
+    } else {
+        const int mine = wid * T::NS * T::STAGE;  // this wave's ring
+        // fp16 rows, a wave's 32 of each turn
+        int ahead = tp;  // the next turn to load
+        auto load_turn = [&](int slot) {
+            const int first = ahead < u1 ? (turns.at(ahead) - turns.packed) * UNIT + wid * 32 : 0;
+            const size_t at = head_at + (size_t)first * a.row_stride;
+            return std::pair<size_t, int>{at, ahead < u1 ? total - first : 0};
+        };
+#pragma unroll
+        for (int k = 0; k < T::NS; ++k) {
+            const auto [at, left] = load_turn(k);
+            load_rows(a.k_cache + at, left, mine + k * T::STAGE);
+            load_rows(a.v_cache + at, left, mine + k * T::STAGE + 32 * T::RB);
+            ++ahead;
+        }
+        if constexpr (PACKED) {
+            PackedBlock<D> f[2];
+            auto fetch = [&](PackedBlock<D> &to, int t) {
+                const int blk = turns.at(min(t, tp - 1)) * WAVES + wid;
+                const bool there = t < tp && blk < held;
+                const size_t at = head_blocks + (there ? blk : 0);
+                const int bytes = there ? BLOCK * D : 0;
+                const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.k8 + at * (BLOCK * D)), 0, bytes, 0x00020000);
+                const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.v8 + at * (BLOCK * D)), 0, bytes, 0x00020000);
+#pragma unroll
+                for (int c = 0; c < 2 * D / 64; ++c) to.k[c] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane * 16 + c * 1024, 0, 2);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) to.v[c] = __builtin_amdgcn_raw_buffer_load_b128(rv, lane * 16 + c * 1024, 0, 2);
+                to.ks = a.k_scale[at];
+                to.vs = a.v_scale[at];
+            };
+            if (u0 < tp) {
+                fetch(f[0], u0);
+                fetch(f[1], u0 + 1);
+            }
+            queries();
+            clear_rows();
+            auto step = [&](PackedBlock<D> &now, int t) {
+                const int blk = turns.at(t) * WAVES + wid;
+                if (blk < held) packed_step(now, blk * BLOCK);
+                fetch(now, t + 2);
+            };
+            for (int t = u0; t < tp; t += 2) {
+                step(f[0], t);
+                if (t + 1 < tp) step(f[1], t + 1);
+            }
+            if (U > 0.0f) leave_units();
+        } else {
+            queries();
+            clear_rows();
+        }
+        // loads younger than the K or V part waited for
+        constexpr int YOUNGER = NL + (T::NS - 1) * 2 * NL;
+        int lds = mine;
+        for (int t = tp; t < u1; ++t) {
+            const int j = (turns.at(t) - turns.packed) * UNIT + wid * 32;
+            const auto [at, left] = load_turn(0);
+            dma_wait<YOUNGER>();
+            read_k(ka, lds, 0);
+            read_k(kb, lds, 1);
+            scores(ka, 0);
+            scores(kb, 1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the slot is refilled
+            load_rows(a.k_cache + at, left, lds);
+            rows_softmax(j);
+            dma_wait<YOUNGER>();
+            read_v(va, lds + 32 * T::RB, 0);
+            read_v(vb, lds + 32 * T::RB, 1);
+            sums();
+            values(va, 0);
+            values(vb, 1);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            load_rows(a.v_cache + at, left, lds + 32 * T::RB);
+            ++ahead;
+            lds += T::STAGE;
+            if (lds == mine + T::NS * T::STAGE) lds = mine;
+        }
+    }
+    dma_wait<0>();
+    lds_barrier();  // the ring is free
+
+    // ---- results: whole rows, what is not finite again
+    int *flag = reinterpret_cast<int *>(smem + T::FLAG);
+    for (int e = tid; e <= T::BM; e += THREADS) flag[e] = 0;
+    lds_barrier();
+    bool redo[NR];
+    float l[NR];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        l[nr] = L[nr][0];
+        if constexpr (PACKED) l[nr] += column_sum(lsum[nr]);
+        float z = l[nr] * 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < NT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) z = fmaf(O[dt][nr][e], 0.0f, z);
+        // (the largest score's p is 2^BASE at least if its product with sc rounds to within a bit)
+        redo[nr] = live[nr] && (z != 0.0f || (any[nr] && !(l[nr] >= 32.0f)));
+        if (redo[nr]) flag[row[nr] - r0] = flag[T::BM] = 1;
+    }
+    auto emit = [&](int t, int hd, int d, float4_t o, float m, float sum) {
+        const int64_t r = s.start + t;
+        if (a.splits == 1) {
+            const float inv = m == -INFINITY ? 0.0f : 1.0f / sum;
+            o *= inv;
+            const int64_t at = r * a.ldo + (int64_t)hd * D + d;
+            if constexpr (HALF)
+                *reinterpret_cast<half4_bits *>(static_cast<uint16_t *>(a.out) + at) = half4_bits{f2h(o[0]), f2h(o[1]), f2h(o[2]), f2h(o[3])};
+            else
+                *reinterpret_cast<float4_any *>(static_cast<float *>(a.out) + at) = o;
+        } else {
+            const int64_t part = (r * a.heads + hd) * a.splits + split;
+            *reinterpret_cast<float4_t *>(a.part_o + part * D + d) = o;
+            if (d == 0) {
+                a.part_ml[part * 2] = m;
+                a.part_ml[part * 2 + 1] = sum;
+            }
+        }
+    };
+    if constexpr (SHARED) {
+        lds_barrier();  // one lane alone may have set a row's flag, and its other three read it
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+            if (live[nr] && !flag[row[nr] - r0])
+#pragma unroll
+                for (int dt = 0; dt < NT; ++dt)
+                    emit(tok[nr], head[nr], dt * 16 + 4 * g, O[dt][nr], M[nr] == -INFINITY ? -INFINITY : -bias[nr], l[nr]);
+        lds_barrier();
+    } else {
+        float *join = reinterpret_cast<float *>(smem);
+        float *ml = reinterpret_cast<float *>(smem + T::ML);
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            const int at = wid * T::BM + nr * 16 + i;
+#pragma unroll
+            for (int dt = 0; dt < NT; ++dt) *reinterpret_cast<float4_t *>(join + at * T::OS + dt * 16 + 4 * g) = O[dt][nr];
+            if (g == 0) {
+                ml[at * 2] = M[nr] == -INFINITY ? -INFINITY : -bias[nr];
+                ml[at * 2 + 1] = l[nr];
+            }
+        }
+        lds_barrier();
+        for (int e = tid; e < T::BM * (D / 4); e += THREADS) {
+            const int k = e / (D / 4), d = e % (D / 4) * 4, r = r0 + k;
+            if (r >= nrows || flag[k]) continue;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, ml[(w * T::BM + k) * 2]);
+            float4_t o = {0, 0, 0, 0};
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float mw = ml[(w * T::BM + k) * 2];
+                const float f = mw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mw - m);
+                sum = fmaf(ml[(w * T::BM + k) * 2 + 1], f, sum);
+                o += *reinterpret_cast<const float4_t *>(join + (w * T::BM + k) * T::OS + d) * f;
+            }
+            const int t = r / group;
+            emit(t, h * group + r - t * group, d, o, m, sum);
+        }
+        lds_barrier();
+    }
+    if (!flag[T::BM]) return;
+    LongScratch &sh = *reinterpret_cast<LongScratch *>(smem);
+    for (int k = 0; k < T::BM; ++k) {
+        if (!flag[k]) continue;  // (uniform)
+        const int t = (r0 + k) / group, hd = h * group + r0 + k - t * group;
+        float o, m, sum;
+        long_row<D, HALF, UNIT>(a, s, b, t, hd, turns, u0, u1, sh, o, m, sum);
+        if (tid < D) {
+            const int64_t r = s.start + t;
+            if (a.splits == 1) {
+                put<HALF>(a.out, r * a.ldo + (int64_t)hd * D + tid, m == -INFINITY ? 0.0f : o / sum);
+            } else {
+                const int64_t part = (r * a.heads + hd) * a.splits + split;
+                a.part_o[part * D + tid] = o;
+                if (tid == 0) {
+                    a.part_ml[part * 2] = m;
+                    a.part_ml[part * 2 + 1] = sum;
+                }
+            }
+        }
+    }
 }
 
-hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, hipStream_t st) {
-    const unsigned grid = (unsigned)a.batch * a.max_rows * a.heads;
-    if (head_dim == 128) {
-        if (half) long_row_kernel<128, true><<<grid, THREADS, 0, st>>>(a);
-        else long_row_kernel<128, false><<<grid, THREADS, 0, st>>>(a);
+// Joins a row's splits: one wave a (row, query head), four values a lane, 64 /
+// (D / 4) splits side by side and four such loads under way.
+template <int D, bool HALF>
+__global__ __launch_bounds__(THREADS) void long_join_kernel(const int32_t *row_start_p, const int32_t *cache_len_p, const float *part_ml_p,
+                                                            const float *part_o_p, int heads_p, int splits_p, int rows_p, int max_rows_p,
+                                                            LongAttnArgs args) {
+    LongAttnArgs a = args;
+    a.row_start = row_start_p;
+    a.cache_len = cache_len_p;
+    a.heads = heads_p;
+    a.splits = splits_p;
+    a.rows = rows_p;
+    a.max_rows = max_rows_p;
+    constexpr int LANES = D / 4, SIDE = 64 / LANES;
+    const int lane = threadIdx.x & 63, d = lane % LANES * 4, side = lane / LANES;
+    const int x = blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const int hd = x % a.heads, bt = x / a.heads, t = bt % a.max_rows, b = bt / a.max_rows;
+    if (b >= a.batch) return;
+    const LongSeq s = long_sequence(a, b);
+    if (t >= s.n) return;
+    const int64_t r = s.start + t, part = (r * a.heads + hd) * a.splits;
+    float4_t o = {0, 0, 0, 0};
+    if (s.ok) {
+        float m = -INFINITY, lw = 0.0f;
+        if (lane < a.splits) {
+            m = part_ml_p[(part + lane) * 2];
+            lw = part_ml_p[(part + lane) * 2 + 1];
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);  // (nothing seen there: o = l = 0)
+        lw *= f;
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) lw += __shfl_xor(lw, k);
+        const float *p = part_o_p + part * D + d;
+        for (int k = 0; k < a.splits; k += 4 * SIDE) {
+            float4_t v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int at = k + u * SIDE + side;
+                v[u] = at < a.splits ? *reinterpret_cast<const float4_t *>(p + (size_t)at * D) : float4_t{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float fk = __shfl(f, min(k + u * SIDE + side, 63));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = fmaf(v[u][e], fk, o[e]);
+            }
+        }
+#pragma unroll
+        for (int k = LANES; k < 64; k <<= 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k);
+        const float inv = top == -INFINITY ? 0.0f : 1.0f / lw;
+        o *= inv;
     } else {
-        if (half) long_row_kernel<64, true><<<grid, THREADS, 0, st>>>(a);
-        else long_row_kernel<64, false><<<grid, THREADS, 0, st>>>(a);
+        const float nan = __builtin_nanf("");
+        o = float4_t{nan, nan, nan, nan};
     }
+    if (side) return;
+    const int64_t at = r * a.ldo + (int64_t)hd * D + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put<HALF>(a.out, at + e, o[e]);
+}
+
+template <int D, bool HALF, int NR, bool SHARED, bool PACKED> static hipError_t launch_tile(const LongAttnArgs &a, int tiles, hipStream_t st) {
+    using T = LongTile<D, NR, SHARED, PACKED>;
+    const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
+    const hipError_t e = allow_lds<&long_attention_kernel<D, HALF, NR, SHARED, PACKED>>(T::LDS);
+    if (e != hipSuccess) return e;
+    long_attention_kernel<D, HALF, NR, SHARED, PACKED><<<grid, THREADS, T::LDS, st>>>(
+        a.row_start, a.cache_len, a.q, a.packed_len, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, grid <= 512, a);
     return hipGetLastError();
+}
+
+template <int D, bool HALF, bool PACKED> static hipError_t launch_d(const LongAttnArgs &a, int bm, hipStream_t st) {
+    const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
+    hipError_t e;
+    if (bm == 16) e = launch_tile<D, HALF, 1, false, PACKED>(a, tiles, st);
+    else if (bm == 32) e = launch_tile<D, HALF, 2, false, PACKED>(a, tiles, st);
+    else if (bm == 64) e = launch_tile<D, HALF, 1, true, PACKED>(a, tiles, st);
+    else e = launch_tile<D, HALF, 2, true, PACKED>(a, tiles, st);
+    if (e != hipSuccess || a.splits == 1) return e;
+    const unsigned waves = (unsigned)a.batch * a.max_rows * a.heads;
+    long_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(a.row_start, a.cache_len, a.part_ml, a.part_o, a.heads,
+                                                                             a.splits, a.rows, a.max_rows, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st) {
+    const bool packed = a.packed_len != nullptr;
+    auto go = [&](auto d, auto h) {
+        return packed ? launch_d<d, h, true>(a, block_rows, st) : launch_d<d, h, false>(a, block_rows, st);
+    };
+    using std::integral_constant;
+    if (head_dim == 128)
+        return half ? go(integral_constant<int, 128>{}, std::true_type{}) : go(integral_constant<int, 128>{}, std::false_type{});
+    return half ? go(integral_constant<int, 64>{}, std::true_type{}) : go(integral_constant<int, 64>{}, std::false_type{});
 }
 
 }  // namespace q3vl

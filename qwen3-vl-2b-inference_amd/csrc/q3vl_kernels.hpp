@@ -297,7 +297,7 @@ struct LongAttnArgs : TreeAttnArgs {
     int blocks;                 // of a kv head
     int window, sinks;          // window 0: none
 };
-hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, hipStream_t st);
+hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st);
 
 struct VerifyArgs {
     const void *logits;

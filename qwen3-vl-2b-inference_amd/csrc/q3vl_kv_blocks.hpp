@@ -3,6 +3,7 @@
 #pragma once
 
 #include "q3vl_device.hpp"
+#include "q3vl_mfma.hpp"
 
 namespace q3vl {
 
@@ -20,6 +21,25 @@ template <int D> __host__ __device__ __forceinline__ constexpr int key_at(int p,
 }
 template <int D> __host__ __device__ __forceinline__ constexpr int value_at(int p, int d) {
     return ((d / 32 * 4 + p % 16 / 4) * 16 + d % 16) * 16 + d % 32 / 16 * 8 + p / 16 * 4 + p % 4;
+}
+
+// Eight int8 as fp16, exactly: a byte u under the byte 0x64 is the half 1024 + u,
+// so x ^ 0x80 gives 1152 + x. (widen4's conversions in asm are not for operands
+// that a matrix instruction has just read: written over too early there, two of
+// eight products came out wrong.)
+Q3VL_INLINE half8_t widen8_plain(uint32_t x, uint32_t y) {
+    typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+    const half2_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    x ^= 0x80808080u;
+    y ^= 0x80808080u;
+    auto part = [&](uint32_t v, uint32_t sel) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        return __builtin_bit_cast(uint32_t, (half2_t)(__builtin_bit_cast(half2_t, __builtin_amdgcn_perm(0x64646464u, v, sel)) + off));
+#else
+        return v;
+#endif
+    };
+    return __builtin_bit_cast(half8_t, (u32x4){part(x, 0x04010400u), part(x, 0x04030402u), part(y, 0x04010400u), part(y, 0x04030402u)});
 }
 
 // What of a sequence can be packed: all of its whole blocks or nothing.

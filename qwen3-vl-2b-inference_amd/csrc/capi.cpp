@@ -1775,13 +1775,14 @@ static int check_long_attention(size_t rows, int heads, int max_rows, int max_le
 // A call's tile and splits, and its workspace bytes. Through a window a
 // workgroup's rows see its positions, the first ones and their own.
 static TreePlan plan_long_attention(size_t rows, int heads, int max_rows, int max_len, int window, int sinks, const q3vl_kv_cache *c,
-                                    const q3vl_kv_blocks *p, bool half, bool chain, size_t *bytes) {
+                                    const q3vl_kv_blocks *p, bool half, bool chain, size_t *bytes, int *most = nullptr) {
     if ((size_t)max_rows > rows) max_rows = (int)rows;
     const int64_t room = (int64_t)c->max_seq + (p ? (int64_t)p->blocks * 32 : 0);
     int64_t len = max_len && max_len < room ? max_len : room;
     if (window && (int64_t)window + sinks + max_rows < len) len = (int64_t)window + sinks + max_rows;
     if (len > INT32_MAX - 256) len = INT32_MAX - 256;
-    const TreePlan t = tree_attention_plan((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, (int)len, c->head_dim, half, chain);
+    if (most) *most = (int)len;
+    const TreePlan t = long_attention_plan((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, (int)len, c->head_dim, half, chain, p);
     const size_t parts = rows * (size_t)heads * (size_t)t.splits;
     *bytes = t.splits > 1 ? align256(parts * (size_t)c->head_dim * 4) + align256(parts * 8) : 0;
     return t;
@@ -1825,10 +1826,10 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     if (!q || !out || !row_start || !cache_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     const bool half = dtype == Q3VL_DTYPE_FP16;
     size_t need = 0;
-    const TreePlan plan = plan_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks, half, !mask, &need);
+    LongAttnArgs a{};
+    const TreePlan plan = plan_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks, half, !mask, &need, &a.max_len);
     char *w = nullptr;
     if (need && (rc = resolve_ws_rows(workspace, workspace_bytes, need, (hipStream_t)stream, &w))) return rc;
-    LongAttnArgs a{};
     a.q = q;
     a.out = out;
     a.ldq = (int64_t)ldq;

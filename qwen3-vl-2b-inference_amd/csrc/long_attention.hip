@@ -204,8 +204,9 @@ template <int D> struct PackedBlock {
     float ks, vs;
 };
 
-template <int D, bool HALF, int NR, bool SHARED, bool PACKED>
-__global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) void long_attention_kernel(
+// ONCE: no other workgroup reads this one's keys and values; they go past the caches.
+template <int D, bool HALF, int NR, bool SHARED, bool PACKED, bool ONCE>
+__global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attention_kernel(
     const int32_t *row_start_p, const int32_t *cache_len_p, const void *q_p, const int32_t *packed_len_p, int kv_heads_p, int heads_p,
     int splits_p, int rows_p, int max_rows_p, int max_seq_p, int tiles, int paired, LongAttnArgs args) {
     LongAttnArgs a = args;  // (the leading arguments arrive in registers)
@@ -221,6 +222,7 @@ __global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) voi
     a.max_seq = max_seq_p;
     using T = LongTile<D, NR, SHARED, PACKED>;
     constexpr int KS = D / 32, NT = D / 16, NQ = HALF ? 1 : 2, UNIT = T::UNIT;
+    constexpr int NT_BIT = ONCE ? 2 : 0;  // (a buffer load's non-temporal bit)
     extern __shared__ __align__(16) unsigned char smem[];
     // (loads with an LDS destination take its offset: 0, as the kernel has no other LDS)
     const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, i = lane & 15, g = lane >> 4;
@@ -308,7 +310,7 @@ __global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) voi
 #pragma unroll
         for (int t = 0; t < NL; ++t) {
             const int at = lds + ((SHARED ? wid * NL : 0) + t) * 1024;
-            if constexpr (!SHARED) dma16_nt(r, voff[t], 0, at);
+            if constexpr (ONCE) dma16_nt(r, voff[t], 0, at);
             else dma16(r, voff[t], 0, at);
         }
     };
@@ -331,9 +333,9 @@ __global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) voi
         const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.k8 + at), 0, left, 0x00020000);
         const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.v8 + at), 0, left, 0x00020000);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) nk[k] = __builtin_amdgcn_raw_buffer_load_b128(rk, (wid * PER + k) * 1024 + lane * 16, 0, 0);
+        for (int k = 0; k < PER; ++k) nk[k] = __builtin_amdgcn_raw_buffer_load_b128(rk, (wid * PER + k) * 1024 + lane * 16, 0, NT_BIT);
 #pragma unroll
-        for (int k = 0; k < PER; ++k) nv[k] = __builtin_amdgcn_raw_buffer_load_b128(rv, (wid * PER + k) * 1024 + lane * 16, 0, 0);
+        for (int k = 0; k < PER; ++k) nv[k] = __builtin_amdgcn_raw_buffer_load_b128(rv, (wid * PER + k) * 1024 + lane * 16, 0, NT_BIT);
     };
     auto widen_tile = [&](int lds) {
 #pragma unroll
@@ -531,9 +533,11 @@ __global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) voi
         }
         softmax(ks, vs * to_units, kPacked);
     };
-    // 32 packed positions from j on, out of registers
-    auto packed_step = [&](const PackedBlock<D> &f, int j) {
-        new_units(f.vs);
+    // 32 packed positions from j on, out of registers; more_k and more_v: the keys'
+    // and the values' registers are free
+    auto packed_step = [&](const PackedBlock<D> &f, int j, auto more_k, auto more_v) {
+        const float ks = f.ks, vs = f.vs;
+        new_units(vs);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             zero_scores(kb);
@@ -544,13 +548,15 @@ __global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) voi
                 score(widen8_plain(w[2], w[3]), kb, 2 * c + 1);
             }
         }
-        packed_softmax(f.ks, f.vs, j);
+        more_k();
+        packed_softmax(ks, vs, j);
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
             const u32x4 w = f.v[c];
             value(widen8_plain(w[0], w[1]), 2 * c);
             value(widen8_plain(w[2], w[3]), 2 * c + 1);
         }
+        more_v();
     };
     auto leave_units = [&] {  // O in the values' own units
 #pragma unroll
@@ -712,31 +718,45 @@ __global__ __launch_bounds__(THREADS, SHARED || (PACKED && NR == 1) ? 2 : 1) voi
             ++ahead;
         }
         if constexpr (PACKED) {
-            PackedBlock<D> f[2];
-            auto fetch = [&](PackedBlock<D> &to, int t) {
-                const int blk = turns.at(min(t, tp - 1)) * WAVES + wid;
-                const bool there = t < tp && blk < held;
+            PackedBlock<D> f[2];  // on their way
+            auto block_of = [&](int t) {  // this wave's of turn t; past the last: -1
+                if (t >= tp) return -1;
+                const int blk = turns.at(t) * WAVES + wid;
+                return blk < held ? blk : -1;
+            };
+            auto fetch = [&](PackedBlock<D> &to, int t, bool keys) {
+                const int blk = block_of(t);
+                const bool there = blk >= 0;
                 const size_t at = head_blocks + (there ? blk : 0);
                 const int bytes = there ? BLOCK * D : 0;
-                const auto rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.k8 + at * (BLOCK * D)), 0, bytes, 0x00020000);
-                const auto rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>(a.v8 + at * (BLOCK * D)), 0, bytes, 0x00020000);
+                const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<int8_t *>((keys ? a.k8 : a.v8) + at * (BLOCK * D)), 0, bytes, 0x00020000);
+                if (keys) {
 #pragma unroll
-                for (int c = 0; c < 2 * D / 64; ++c) to.k[c] = __builtin_amdgcn_raw_buffer_load_b128(rk, lane * 16 + c * 1024, 0, 2);
+                    for (int c = 0; c < 2 * D / 64; ++c) to.k[c] = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16 + c * 1024, 0, NT_BIT);
+                    to.ks = a.k_scale[at];
+                    to.vs = a.v_scale[at];
+                } else {
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) to.v[c] = __builtin_amdgcn_raw_buffer_load_b128(rv, lane * 16 + c * 1024, 0, 2);
-                to.ks = a.k_scale[at];
-                to.vs = a.v_scale[at];
+                    for (int c = 0; c < D / 32; ++c) to.v[c] = __builtin_amdgcn_raw_buffer_load_b128(r, lane * 16 + c * 1024, 0, NT_BIT);
+                }
             };
             if (u0 < tp) {
-                fetch(f[0], u0);
-                fetch(f[1], u0 + 1);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    fetch(f[k], u0 + k, true);
+                    fetch(f[k], u0 + k, false);
+                }
             }
             queries();
             clear_rows();
             auto step = [&](PackedBlock<D> &now, int t) {
-                const int blk = turns.at(t) * WAVES + wid;
-                if (blk < held) packed_step(now, blk * BLOCK);
-                fetch(now, t + 2);
+                const int blk = block_of(t);
+                if (blk < 0) {
+                    fetch(now, t + 2, true);
+                    fetch(now, t + 2, false);
+                    return;
+                }
+                packed_step(now, blk * BLOCK, [&] { fetch(now, t + 2, true); }, [&] { fetch(now, t + 2, false); });
             };
             for (int t = u0; t < tp; t += 2) {
                 step(f[0], t);
@@ -947,23 +967,66 @@ __global__ __launch_bounds__(THREADS) void long_join_kernel(const int32_t *row_s
     for (int e = 0; e < 4; ++e) put<HALF>(a.out, at + e, o[e]);
 }
 
-template <int D, bool HALF, int NR, bool SHARED, bool PACKED> static hipError_t launch_tile(const LongAttnArgs &a, int tiles, hipStream_t st) {
+// Rows of a workgroup and splits.
+//
+// Over packed blocks up to 64 rows of a kv head go in tiles of 16, each of which
+// reads and widens for itself what its neighbours read too (out of the caches):
+// two workgroups fit a CU, where 32 rows' registers leave room for one. us
+// (16 / 8 heads of 128, fp32, lengths from half to all, each at its best split):
+// 24 trees of 12 rows over 8000 75 in tiles of 16, 103 with 32 rows a workgroup,
+// 119 in shared tiles of 64; of 20 rows 94 and 131 shared; of 32 139 and 140; of
+// 40 146 and 146, 6 of 40 53 and 51.
+// As many splits as fill whole rounds of 512 workgroups to nine tenths (the rule's
+// choice first): one token of 4 sequences of 16000 24.9 at 16, 27.6 at 8; of 8 of
+// 12000 32.6 at 8, 39.3 at 4; of 12 47.1 at 5, 58.2 at 2; of 24 86.9 at 5, 95.6 at
+// 2, 85.3 at 8; of 40 of 3000 43.7 at 3, 46.4 at 1. Below 512 positions a split one
+// round of 256: one token of 8 of 3000 17.2 at 4, 17.9 at 8; of 2 of 8000 15.0 at
+// 16, 16.8 at 32; 6 trees of 20 over 1000 15.1 at 1, 16.7 at 4. (All of one length:
+// 32 of 8192 90.8 at 2, 87.6 at 1, which the host cannot tell apart.)
+//
+// Else as tree_attention_plan says, whose kernels these are.
+TreePlan long_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim, bool half,
+                             bool chain, bool packed) {
+    const int64_t kv_rows = (int64_t)max_rows * (heads / kv_heads), tiles = (kv_rows + 15) / 16;
+    if (!packed || tiles > 4) return tree_attention_plan(rows, heads, kv_heads, batch, max_rows, max_len, head_dim, half, chain);
+    const int64_t base = (int64_t)batch * kv_heads * tiles, most = ((int64_t)max_len + 127) / 128;
+    if (base < 1) return {16, 1};
+    int64_t k = 256 / base;
+    for (int i = 1; i <= 16 && base <= 4096; ++i) {
+        const int64_t blocks = base * i, rounds = (blocks + 511) / 512;
+        if (blocks * 10 < rounds * 512 * 9) continue;
+        if (max_len / i >= 512) k = i;
+        break;
+    }
+    k = k < most ? k : most;
+    return {16, (int)(k < 1 ? 1 : k < 32 ? k : 32)};
+}
+
+template <int D, bool HALF, int NR, bool SHARED, bool PACKED, bool ONCE>
+static hipError_t launch_tile(const LongAttnArgs &a, int tiles, hipStream_t st) {
     using T = LongTile<D, NR, SHARED, PACKED>;
     const unsigned grid = (unsigned)tiles * a.splits * a.batch * a.kv_heads;
-    const hipError_t e = allow_lds<&long_attention_kernel<D, HALF, NR, SHARED, PACKED>>(T::LDS);
+    const hipError_t e = allow_lds<&long_attention_kernel<D, HALF, NR, SHARED, PACKED, ONCE>>(T::LDS);
     if (e != hipSuccess) return e;
-    long_attention_kernel<D, HALF, NR, SHARED, PACKED><<<grid, THREADS, T::LDS, st>>>(
+    long_attention_kernel<D, HALF, NR, SHARED, PACKED, ONCE><<<grid, THREADS, T::LDS, st>>>(
         a.row_start, a.cache_len, a.q, a.packed_len, a.kv_heads, a.heads, a.splits, a.rows, a.max_rows, a.max_seq, tiles, grid <= 512, a);
     return hipGetLastError();
 }
 
 template <int D, bool HALF, bool PACKED> static hipError_t launch_d(const LongAttnArgs &a, int bm, hipStream_t st) {
     const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
+    // Keys and values that one workgroup reads go past the caches: always with up to
+    // 32 rows in one tile (us past the caches and through them, packed: 24 sequences
+    // of 12000 85 and 96, 40 of 3000 44 and 48, one of 1024 12.6 and 11.5; but trees of
+    // 32 rows in four tiles 141 and 132), of shared tiles where together they are more
+    // than the caches keep.
+    const bool one = tiles == 1, once = one && (double)a.batch * a.kv_heads * a.max_len * D * (PACKED ? 2 : 4) > 192e6;
     hipError_t e;
-    if (bm == 16) e = launch_tile<D, HALF, 1, false, PACKED>(a, tiles, st);
-    else if (bm == 32) e = launch_tile<D, HALF, 2, false, PACKED>(a, tiles, st);
-    else if (bm == 64) e = launch_tile<D, HALF, 1, true, PACKED>(a, tiles, st);
-    else e = launch_tile<D, HALF, 2, true, PACKED>(a, tiles, st);
+    if (PACKED && bm == 16 && !one) e = launch_tile<D, HALF, 1, false, true, false>(a, tiles, st);
+    else if (bm == 16) e = launch_tile<D, HALF, 1, false, PACKED, true>(a, tiles, st);
+    else if (!PACKED && bm == 32) e = launch_tile<D, HALF, 2, false, false, true>(a, tiles, st);
+    else if (bm == 64) e = once ? launch_tile<D, HALF, 1, true, PACKED, true>(a, tiles, st) : launch_tile<D, HALF, 1, true, PACKED, false>(a, tiles, st);
+    else e = once ? launch_tile<D, HALF, 2, true, PACKED, true>(a, tiles, st) : launch_tile<D, HALF, 2, true, PACKED, false>(a, tiles, st);
     if (e != hipSuccess || a.splits == 1) return e;
     const unsigned waves = (unsigned)a.batch * a.max_rows * a.heads;
     long_join_kernel<D, HALF><<<(waves + WAVES - 1) / WAVES, THREADS, 0, st>>>(a.row_start, a.cache_len, a.part_ml, a.part_o, a.heads,

@@ -297,6 +297,8 @@ struct LongAttnArgs : TreeAttnArgs {
     int blocks;                 // of a kv head
     int window, sinks;          // window 0: none
 };
+TreePlan long_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim, bool half,
+                             bool chain, bool packed);
 hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st);
 
 struct VerifyArgs {

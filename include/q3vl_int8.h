@@ -546,7 +546,7 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
  * next token is the first i with w_0 + .. + w_i > sample_u[row] sum w, w_i =
  * max(p_i - c q_i, 0) (p_i where all of these are 0). With draft_probs NULL the
  * next token is drawn from p at once, and its first child that has it stays.
- * All in 64 bits; a p below e^-700 of the row's largest counts as 0.
+ * All in 64 bits.
  *
  * accepted[b]: rows that stay, the first among them (0: the sequence has none);
  * path [batch, max_rows]: their indexes in the sequence, ascending, then -1;

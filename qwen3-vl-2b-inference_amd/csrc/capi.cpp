@@ -1871,7 +1871,9 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
 
 size_t q3vl_verify_drafts_workspace_bytes(size_t rows, size_t V) {
     if (rows == 0 || V == 0 || V > kLogprobMaxV || rows > kLogprobMaxM) return 0;
-    return 2 * align256(rows * 4);
+    const size_t pairs = (size_t)verify_pairs_most((int64_t)rows, (int64_t)V);
+    return align256(pairs * 8) + align256(pairs * 8 * (kVerifyRounds + 1)) + align256(pairs * 4) + 2 * align256(rows * 4) +
+           align256(rows * sizeof(VerifyRow));
 }
 
 int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *draft_probs, size_t ldp,
@@ -1886,9 +1888,9 @@ int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *dr
     if (batch < 0 || max_rows < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape batch=%d max_rows=%d", batch, max_rows);
     if (max_rows > kDraftRows)
         return fail(Q3VL_ERR_UNSUPPORTED, "max_rows=%d: at most %d rows a sequence", max_rows, kDraftRows);
-    const double inv_t = 1.0 / temperature;
-    if (!(temperature > 0.0 && inv_t > 0.0 && inv_t < INFINITY))
-        return fail(Q3VL_ERR_INVALID_ARGUMENT, "temperature=%g: positive and finite, its reciprocal too", temperature);
+    const double per = 1.4426950408889634 / temperature;
+    if (!(temperature > 0.0 && per > 0.0 && per * 3.5e38 < INFINITY))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "temperature=%g: positive and finite, the logits over it too", temperature);
     if (batch == 0) return Q3VL_OK;
     if (rows > kLogprobMaxM || V > kLogprobMaxV || batch > (1 << 22))
         return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu V=%zu batch=%d)", rows, V, batch);
@@ -1897,9 +1899,13 @@ int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *dr
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     if ((uintptr_t)logits % (dtype == Q3VL_DTYPE_FP16 ? 2 : 4)) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned logits");
     if ((uintptr_t)draft_probs % 4) return fail(Q3VL_ERR_INVALID_ARGUMENT, "misaligned draft_probs");
+    const int chunks = rows ? verify_chunks((int64_t)rows, (int64_t)V) : 1;
+    if ((double)rows * chunks > (double)kMaxGrid) return fail(Q3VL_ERR_UNSUPPORTED, "shape too large (rows=%zu V=%zu)", rows, V);
+    const size_t pairs = rows * (size_t)chunks, sum_bytes = align256(pairs * 8), round_bytes = align256(pairs * 8 * (kVerifyRounds + 1));
     char *w = nullptr;
     if (rows) {
-        const int rc = resolve_ws_rows(workspace, workspace_bytes, q3vl_verify_drafts_workspace_bytes(rows, V), (hipStream_t)stream, &w);
+        const int rc = resolve_ws_rows(workspace, workspace_bytes, sum_bytes + round_bytes + align256(pairs * 4) + 2 * align256(rows * 4) + align256(rows * sizeof(VerifyRow)),
+                                       (hipStream_t)stream, &w);
         if (rc) return rc;
     }
     VerifyArgs a{};
@@ -1916,11 +1922,18 @@ int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *dr
     a.rows = (int)rows;
     a.V = (int)V;
     a.max_rows = max_rows;
-    a.inv_t = inv_t;
+    a.per = per;
     a.accepted = accepted;
     a.path = path;
     a.next = next;
-    a.pick = reinterpret_cast<int32_t *>(w);
+    a.chunks = chunks;
+    // (a row of two has one child at most, rejected once)
+    a.rounds = !draft_probs ? 0 : max_rows <= 2 ? 1 : kVerifyRounds;
+    a.chunk_sum = reinterpret_cast<double *>(w);
+    a.round_sum = reinterpret_cast<double *>(w += sum_bytes);
+    a.state = reinterpret_cast<VerifyRow *>(w += round_bytes);
+    a.chunk_top = reinterpret_cast<float *>(w += align256(rows * sizeof(VerifyRow)));
+    a.pick = reinterpret_cast<int32_t *>(w += align256(pairs * 4));
     a.taken = reinterpret_cast<int32_t *>(w + align256(rows * 4));
     Q3VL_HIP(launch_verify_drafts(a, dtype == Q3VL_DTYPE_FP16, (hipStream_t)stream), "draft judging launch");
     return Q3VL_OK;

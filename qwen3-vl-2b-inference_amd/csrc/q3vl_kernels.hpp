@@ -301,6 +301,11 @@ TreePlan long_attention_plan(int64_t rows, int heads, int kv_heads, int batch, i
                              bool chain, bool packed);
 hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st);
 
+struct VerifyRow {  // a row that waits for a round's sums
+    double c;
+    float m;    // its largest logit
+    int child;  // the last one rejected
+};
 struct VerifyArgs {
     const void *logits;
     int64_t ld;
@@ -309,10 +314,19 @@ struct VerifyArgs {
     const int32_t *tokens, *parents, *row_start;
     const float *accept_u, *sample_u;
     int batch, rows, V, max_rows;
-    double inv_t;
+    double per;  // log2 e / temperature
     int32_t *accepted, *path, *next;
+    int chunks;             // of a row
+    int rounds;             // of tests that leave sums (with draft probabilities)
+    float *chunk_top;       // [rows][chunks]
+    double *chunk_sum;      // [rows][chunks]
+    double *round_sum;      // [rounds + 1][rows][chunks]
+    VerifyRow *state;       // [rows]
     int32_t *pick, *taken;  // [rows]
 };
+constexpr int kVerifyRounds = 2;  // most
+int verify_chunks(int64_t rows, int64_t V);
+int64_t verify_pairs_most(int64_t rows, int64_t V);
 hipError_t launch_verify_drafts(const VerifyArgs &a, bool half, hipStream_t st);
 
 }  // namespace q3vl

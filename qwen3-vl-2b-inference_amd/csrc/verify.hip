@@ -11,6 +11,14 @@
 //
 // In 64 bits throughout: the choices are comparisons, and every implementation
 // of their definition should come to the same one.
+//
+// Rows are cut into chunks, one wave each. The first kernel leaves a chunk's
+// maximum m_c and sum of e^((x - m_c) / T). From these a workgroup a row joins m
+// and the whole sum, tests the row's children and, if the row is decided, finds
+// the chunk in which the cumulated sums pass the row's number and the value in
+// it. A row whose child is rejected waits for a round: its chunks' sums of max(p
+// - c q, 0), by all workgroups again, then the next test. So each logit is read
+// once, or once more for each rejection.
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 
@@ -18,180 +26,335 @@ namespace q3vl {
 
 namespace {
 
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr double FAR = -700.0;  // (x - m) / T below which a weight is 0
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int SMALL = 9, LARGE = 11;  // chunks of 2^9 or 2^11 values
 
-struct Scratch {
-    double sum[WAVES];
-    float top[WAVES];
-    int bad[WAVES];
-    int at[WAVES];
-    uint64_t kids[kDraftRows / 64];
-    int child;
+// 2^y for y <= 0: y = n + f, |f| <= 1/2, and 2^f by the polynomial of degree 11
+// that takes its values at the Chebyshev nodes (2e-17 off, relatively).
+__device__ __forceinline__ double exp2_64(double y) {
+    y = fmax(y, -2000.0);  // (0 then: a double's least is 2^-1074)
+    const double n = __builtin_rint(y), f = y - n;
+    constexpr double C[12] = {1.0, 0.69314718055994529, 0.24022650695910158, 0.055504108664821625, 0.0096181291075872564,
+                              0.0013333558146406471, 0.00015403530463724353, 1.5252733841556773e-05, 1.3215432535912375e-06,
+                              1.0178057087733941e-07, 7.0741942972885211e-09, 4.4558179083360645e-10};
+    double r = C[11];
+#pragma unroll
+    for (int k = 10; k >= 0; --k) r = fma(r, f, C[k]);
+    return __builtin_ldexp(r, (int)n);
+}
+// e^((x - m) / T), with per = log2 e / T
+struct Weight {
+    double per, top;
+    __device__ __forceinline__ Weight(float m, double p) : per(p), top(m) {}
+    __device__ __forceinline__ double operator()(float x) const { return exp2_64(((double)x - top) * per); }
 };
+__device__ __forceinline__ double draft_of(float q) { return q > 0.0f ? (double)q : 0.0; }
 
-__device__ __forceinline__ double block_sum(double v, Scratch &sh) {
+__device__ __forceinline__ double wave_sum(double v) {
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.sum[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double s = 0.0;
-    for (int w = 0; w < WAVES; ++w) s += sh.sum[w];
-    return s;
+    return v;
+}
+__device__ __forceinline__ double wave_scan(double v) {  // inclusive
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const double o = __shfl_up(v, k);
+        if (lane >= k) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) v = fmaxf(v, __shfl_xor(v, k));
+    return v;
 }
 
-template <bool HALF> struct Row {
-    const void *x;
-    const float *q;  // or null
-    float m;
-    double inv_t;
-    __device__ __forceinline__ float logit(int i) const {
-        return HALF ? h2f(static_cast<const uint16_t *>(x)[i]) : static_cast<const float *>(x)[i];
+// (rows may begin anywhere)
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t h4_any __attribute__((ext_vector_type(4), aligned(2)));
+
+// Values of a row from `i` on, four and every `step` again; behind its end `rest`.
+template <bool HALF, int PER> __device__ __forceinline__ void load_values(const void *x, int i, int step, int V, float rest, float (&v)[PER]) {
+#pragma unroll
+    for (int k = 0; k < PER; k += 4, i += step) {
+        if (i + 4 <= V) {
+            if constexpr (HALF) {
+                const h4_any r = *reinterpret_cast<const h4_any *>(static_cast<const uint16_t *>(x) + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k + e] = h2f(r[e]);
+            } else {
+                const f4_any r = *reinterpret_cast<const f4_any *>(static_cast<const float *>(x) + i);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k + e] = r[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[k + e] = i + e < V ? (HALF ? h2f(static_cast<const uint16_t *>(x)[i + e]) : static_cast<const float *>(x)[i + e]) : rest;
+        }
     }
-    __device__ __forceinline__ double e(int i) const {  // p times its sum
-        const double d = ((double)logit(i) - (double)m) * inv_t;
-        return d >= FAR ? exp(d) : 0.0;
-    }
-    __device__ __forceinline__ double draft(int i) const {
-        const float v = q[i];
-        return v > 0.0f ? (double)v : 0.0;
-    }
-    // p - c q, times p's sum
-    __device__ __forceinline__ double w(int i, double c) const {
-        double v = e(i);
-        if (c > 0.0) v = fmax(v - c * draft(i), 0.0);
-        return v;
-    }
-};
+}
+template <bool HALF> __device__ __forceinline__ const void *row_of(const VerifyArgs &a, int r) {
+    return HALF ? (const void *)(static_cast<const uint16_t *>(a.logits) + (size_t)r * a.ld)
+                : (const void *)(static_cast<const float *>(a.logits) + (size_t)r * a.ld);
+}
+template <bool HALF> __device__ __forceinline__ float value_of(const void *x, int i) {
+    return HALF ? h2f(static_cast<const uint16_t *>(x)[i]) : static_cast<const float *>(x)[i];
+}
+
+// (a row's chunks by wave: -1 past the last)
+__device__ __forceinline__ int chunk_of(const VerifyArgs &a, int &r) {
+    const int blocks = (a.chunks + WAVES - 1) / WAVES;
+    r = blockIdx.x / blocks;
+    const int c = (blockIdx.x - r * blocks) * WAVES + (threadIdx.x >> 6);
+    return c < a.chunks ? c : -1;
+}
+
+constexpr int OPEN = -2;  // taken[] of a row that waits for a round's sums
 
 }  // namespace
 
-// One workgroup a row: pick[row] the token after it if the path ends there,
-// taken[row] the child that stays (-1: none).
-template <bool HALF> __global__ __launch_bounds__(THREADS) void verify_row_kernel(VerifyArgs a) {
-    __shared__ Scratch sh;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    // the row's sequence
-    int b = 0;
-    {
-        int lo = 0, hi = a.batch;  // the last b with row_start[b] <= r
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (a.row_start[mid] <= r) lo = mid;
-            else hi = mid;
-        }
-        b = lo;
-    }
-    const int start = max(a.row_start[b], 0), end = min(max(a.row_start[b + 1], start), a.rows);
-    const int n = min(end - start, a.max_rows), t = r - start;
-    if (t < 0 || t >= n) return;
-    Row<HALF> row;
-    row.x = HALF ? (const void *)(static_cast<const uint16_t *>(a.logits) + (size_t)r * a.ld)
-                 : (const void *)(static_cast<const float *>(a.logits) + (size_t)r * a.ld);
-    row.q = a.draft ? a.draft + (size_t)r * a.ldp : nullptr;
-    row.inv_t = a.inv_t;
-    float top = -INFINITY;
+// One wave a chunk of a row: its maximum (+inf: a NaN or +inf in it) and the sum
+// of its weights.
+template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verify_sums_kernel(VerifyArgs a) {
+    constexpr int PER = (1 << SHIFT) / 64;
+    const int lane = threadIdx.x & 63;
+    int r;
+    const int c = chunk_of(a, r);
+    if (c < 0) return;
+    float v[PER];
+    load_values<HALF, PER>(row_of<HALF>(a, r), (c << SHIFT) + lane * 4, 256, a.V, -INFINITY, v);
+    float m = -INFINITY;
     bool bad = false;
-    for (int i = tid; i < a.V; i += THREADS) {
-        const float x = row.logit(i);
-        bad = bad || !(x < INFINITY);
-        top = fmaxf(top, x);
-    }
 #pragma unroll
-    for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-    const bool any_bad = __any(bad);
+    for (int k = 0; k < PER; ++k) {
+        bad = bad || !(v[k] < INFINITY);
+        m = fmaxf(m, v[k]);
+    }
+    m = wave_max(m);
+    bad = __any(bad);
+    double s = 0.0;
+    if (m > -INFINITY && !bad) {
+        const Weight w(m, a.per);
+#pragma unroll
+        for (int k = 0; k < PER; ++k) s += w(v[k]);
+    }
+    s = wave_sum(s);
     if (lane == 0) {
-        sh.top[wave] = top;
-        sh.bad[wave] = any_bad;
+        a.chunk_top[(size_t)r * a.chunks + c] = bad ? INFINITY : m;
+        a.chunk_sum[(size_t)r * a.chunks + c] = s;
     }
+}
+
+// A round: of the rows that wait, the chunk's sum of max(e - c q, 0).
+template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verify_round_kernel(VerifyArgs a, int round) {
+    constexpr int PER = (1 << SHIFT) / 64;
+    const int lane = threadIdx.x & 63;
+    int r;
+    const int chunk = chunk_of(a, r);
+    if (chunk < 0 || a.taken[r] != OPEN) return;
+    const VerifyRow s = a.state[r];
+    float v[PER], q[PER];
+    load_values<HALF, PER>(row_of<HALF>(a, r), (chunk << SHIFT) + lane * 4, 256, a.V, -INFINITY, v);
+    load_values<false, PER>(a.draft + (size_t)r * a.ldp, (chunk << SHIFT) + lane * 4, 256, a.V, 0.0f, q);
+    const Weight w(s.m, a.per);
+    double z = 0.0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) z += fmax(w(v[k]) - s.c * draft_of(q[k]), 0.0);
+    z = wave_sum(z);
+    if (lane == 0) a.round_sum[((size_t)round * a.rows + r) * a.chunks + chunk] = z;
+}
+
+// One workgroup a row, behind the sums (round 0) or a round: taken[row], the
+// child that stays (-1: none, OPEN: one was rejected and its sums are not there),
+// and pick[row], the token after the row if the path ends there. In the last
+// step no row stays open: further sums are made here, chunk by chunk.
+template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verify_step_kernel(VerifyArgs a, int round) {
+    constexpr int PER = (1 << SHIFT) / 64, EACH = (1 << SHIFT) / THREADS;
+    __shared__ double sums[WAVES];
+    __shared__ uint64_t kids[kDraftRows / 64];
+    __shared__ int token[kDraftRows];                       // of the children
+    __shared__ float accept[kDraftRows], logit[kDraftRows], draft[kDraftRows];
+    __shared__ int seq, first_at, last_at;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (round > 0 && a.taken[r] != OPEN) return;
+    const void *x = row_of<HALF>(a, r);
+
+    // ---- the row's maximum and sum (each wave for itself, in one order)
+    const float *top = a.chunk_top + (size_t)r * a.chunks;
+    const double *sum = a.chunk_sum + (size_t)r * a.chunks;
+    float m = -INFINITY;
+    for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, top[c]);  // (+inf where the row cannot be judged)
+    m = wave_max(m);
+
+    // ---- its sequence and its children there
+    if (tid == 0) seq = -1;
     __syncthreads();
-    bad = false;
-    for (int w = 0; w < WAVES; ++w) {
-        top = fmaxf(top, sh.top[w]);
-        bad = bad || sh.bad[w];
-    }
-    if (bad || top == -INFINITY) {
+    for (int b = tid; b < a.batch; b += THREADS)
+        if (a.row_start[b] <= r && r < a.row_start[b + 1]) atomicMax(&seq, b);
+    __syncthreads();
+    const int start = seq < 0 ? r : max(a.row_start[seq], 0);
+    const int n = seq < 0 ? 0 : min(min(a.row_start[seq + 1], a.rows) - start, a.max_rows), t = r - start;
+    if (t >= n || !(m > -INFINITY && m < INFINITY)) {
         if (tid == 0) {
             a.pick[r] = -1;
             a.taken[r] = -1;
         }
         return;
     }
-    row.m = top;
-    const uint64_t kid = __ballot(tid < n && tid > t && a.parents[start + min(tid, n - 1)] == t);
-    if (lane == 0) sh.kids[wave] = kid;
-    double s = 0.0;
-    for (int i = tid; i < a.V; i += THREADS) s += row.e(i);
-    const double total = block_sum(s, sh);  // (its barriers stand between kids' write and reads too)
-    double c = 0.0, z = total;              // c and Z, times p's sum
-    int taken = -1;
-    if (row.q) {
-        for (int w = 0; w < WAVES && taken < 0; ++w)
-            for (uint64_t k = sh.kids[w]; k; k &= k - 1) {
+    for (int w = wave; w < kDraftRows / 64; w += WAVES) {
+        const int i = w * 64 + lane;
+        bool kid = i < n && i > t && a.parents[start + i] == t;
+        if (kid) {
+            const int tok = a.tokens[start + i];
+            kid = tok >= 0 && tok < a.V;
+            token[i] = tok;
+            if (kid && a.draft) {
+                accept[i] = a.accept_u[start + i];
+                logit[i] = value_of<HALF>(x, tok);
+                draft[i] = a.draft[(size_t)r * a.ldp + tok];
+            }
+        }
+        const uint64_t bits = __ballot(kid);
+        if (lane == 0) kids[w] = bits;
+    }
+    const Weight weight(m, a.per);
+    double total = 0.0;
+    for (int c = lane; c < a.chunks; c += 64) total = fma(sum[c], weight(top[c]), total);
+    total = wave_sum(total);
+    __syncthreads();
+
+    // ---- the tests
+    int taken = -1, pick = -1;
+    double c = 0.0, z = total;  // times the sum of weights
+    const double *left = nullptr;  // the chunks' sums of max(e - c q, 0) (null: of e)
+    if (a.draft) {
+        int rejected = 0;
+        auto join = [&](const double *p) {
+            double v = 0.0;
+            for (int i = lane; i < a.chunks; i += 64) v += p[i];
+            left = p;
+            return wave_sum(v);
+        };
+        int from = 0;  // the first child not tested yet
+        if (round > 0) {
+            const VerifyRow s = a.state[r];
+            c = s.c;
+            from = s.child + 1;
+            rejected = round;
+            z = join(a.round_sum + ((size_t)(round - 1) * a.rows + r) * a.chunks);
+        }
+        for (int w = from >> 6; w < kDraftRows / 64 && taken < 0; ++w) {
+            uint64_t k = kids[w];
+            if (w == from >> 6) k &= ~0ull << (from & 63);
+            for (; k; k &= k - 1) {
                 const int child = w * 64 + __ffsll((unsigned long long)k) - 1;
-                const int tok = a.tokens[start + child];
-                if (tok < 0 || tok >= a.V) continue;
-                if ((double)a.accept_u[start + child] * row.draft(tok) * z < row.w(tok, c)) {
+                const double q = draft_of(draft[child]), e = weight(logit[child]), rest = rejected ? fmax(e - c * q, 0.0) : e;
+                if ((double)accept[child] * q * z < rest) {
                     taken = child;
                     break;
                 }
                 c += z;
-                s = 0.0;
-                for (int i = tid; i < a.V; i += THREADS) s += row.w(i, c);
-                z = block_sum(s, sh);
+                ++rejected;
+                if (rejected <= a.rounds) {
+                    if (tid == 0) {
+                        a.state[r] = VerifyRow{c, m, child};
+                        a.taken[r] = OPEN;
+                    }
+                    return;
+                }
+                double *own = a.round_sum + ((size_t)a.rounds * a.rows + r) * a.chunks;
+                for (int i = wave; i < a.chunks; i += WAVES) {
+                    float v[PER], p[PER];
+                    load_values<HALF, PER>(x, (i << SHIFT) + lane * 4, 256, a.V, -INFINITY, v);
+                    load_values<false, PER>(a.draft + (size_t)r * a.ldp, (i << SHIFT) + lane * 4, 256, a.V, 0.0f, p);
+                    double s = 0.0;
+#pragma unroll
+                    for (int j = 0; j < PER; ++j) s += fmax(weight(v[j]) - c * draft_of(p[j]), 0.0);
+                    s = wave_sum(s);
+                    if (lane == 0) own[i] = s;
+                }
+                __syncthreads();  // (of this workgroup's own stores too)
+                z = join(own);
+                __syncthreads();
             }
-        if (!(z > 0.0)) {
+        }
+        if (!(z > 0.0)) {  // nothing is left of p: p itself
             c = 0.0;
             z = total;
+            left = nullptr;
         }
     }
-    int pick = -1;
+
+    // ---- the token by the inverse of the cumulated weights
     if (taken < 0) {
-        // the token by the inverse of the cumulated weights, chunk by chunk
         const double want = (double)a.sample_u[r] * z;
-        double before = 0.0;
-        int last = -1;  // the last value with a weight
-        for (int base = 0; base < a.V && pick < 0; base += THREADS) {
-            const int i = base + tid;
-            const double v = i < a.V ? row.w(i, c) : 0.0;
-            double run = v;  // inclusive within the wave
+        double before = 0.0, ahead = 0.0;  // sums of earlier chunks: than the next 64, than the one chosen
+        int chunk = -1, last = 0;
+        double last_ahead = 0.0;
+        for (int base = 0; base < a.chunks && chunk < 0; base += 64) {
+            const int i = base + lane;
+            double v = 0.0;
+            if (i < a.chunks) v = left ? left[i] : sum[i] * weight(top[i]);
+            const double run = wave_scan(v);
+            const uint64_t over = __ballot(v > 0.0 && before + run > want), some = __ballot(v > 0.0);
+            const int at = over ? __ffsll((unsigned long long)over) - 1 : some ? 63 - __clzll((long long)some) : 0;
+            const double prior = before + (at ? __shfl(run, at - 1) : 0.0);
+            if (over) {
+                chunk = base + at;
+                ahead = prior;
+            } else if (some) {
+                last = base + at;
+                last_ahead = prior;
+            }
+            before += __shfl(run, 63);
+        }
+        if (chunk < 0) {  // (the numbers' last bits)
+            chunk = last;
+            ahead = last_ahead;
+        }
+        // EACH values in a row a thread
+        const int first = (chunk << SHIFT) + tid * EACH;
+        double w[EACH], mine = 0.0;
 #pragma unroll
-            for (int k = 1; k < 64; k <<= 1) {
-                const double o = __shfl_up(run, k);
-                if (lane >= k) run += o;
-            }
-            __syncthreads();
-            if (lane == 63) sh.sum[wave] = run;
-            __syncthreads();
-            double ahead = before;
-            for (int w = 0; w < WAVES; ++w) {
-                if (w < wave) ahead += sh.sum[w];
-                before += sh.sum[w];
-            }
-            const uint64_t over = __ballot(v > 0.0 && ahead + run > want), some = __ballot(v > 0.0);
-            __syncthreads();
-            if (lane == 0) {
-                sh.at[wave] = over ? base + wave * 64 + __ffsll((unsigned long long)over) - 1 : -1;
-                sh.bad[wave] = some ? base + wave * 64 + 63 - __clzll((long long)some) : -1;
-            }
-            __syncthreads();
-            for (int w = WAVES - 1; w >= 0; --w) {
-                if (sh.at[w] >= 0) pick = sh.at[w];
-                last = max(last, sh.bad[w]);
+        for (int k = 0; k < EACH; ++k) {
+            const int i = first + k;
+            w[k] = i < a.V ? weight(value_of<HALF>(x, i)) : 0.0;
+            if (c > 0.0 && i < a.V) w[k] = fmax(w[k] - c * draft_of(a.draft[(size_t)r * a.ldp + i]), 0.0);
+            mine += w[k];
+        }
+        const double run = wave_scan(mine);
+        if (lane == 63) sums[wave] = run;
+        if (tid == 0) {
+            first_at = INT_MAX;
+            last_at = -1;
+        }
+        __syncthreads();
+        double at = ahead + (run - mine);
+        for (int v = 0; v < wave; ++v) at += sums[v];
+        int found = INT_MAX, some = -1;
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            at += w[k];
+            if (w[k] > 0.0) {
+                some = first + k;
+                if (at > want && found == INT_MAX) found = first + k;
             }
         }
-        if (pick < 0) pick = last;
-        if (!row.q) {
-            for (int w = 0; w < WAVES && taken < 0; ++w)
-                for (uint64_t k = sh.kids[w]; k; k &= k - 1) {
+        if (found != INT_MAX) atomicMin(&first_at, found);
+        if (some >= 0) atomicMax(&last_at, some);
+        __syncthreads();
+        pick = first_at != INT_MAX ? first_at : last_at;
+        if (!a.draft)  // the first child that has the token
+            for (int w = 0; w < kDraftRows / 64 && taken < 0; ++w)
+                for (uint64_t k = kids[w]; k; k &= k - 1) {
                     const int child = w * 64 + __ffsll((unsigned long long)k) - 1;
-                    if (a.tokens[start + child] == pick) {
+                    if (token[child] == pick) {
                         taken = child;
                         break;
                     }
                 }
-        }
     }
     if (tid == 0) {
         a.pick[r] = pick;
@@ -201,30 +364,59 @@ template <bool HALF> __global__ __launch_bounds__(THREADS) void verify_row_kerne
 
 // One wave a sequence follows its path.
 __global__ __launch_bounds__(64) void verify_path_kernel(VerifyArgs a) {
+    __shared__ int taken[kDraftRows];
     const int b = blockIdx.x, lane = threadIdx.x;
     const int start = min(max(a.row_start[b], 0), a.rows), end = min(max(a.row_start[b + 1], start), a.rows);
     const int n = min(end - start, a.max_rows);
+    for (int i = lane; i < n; i += 64) taken[i] = a.taken[start + i];
+    __syncthreads();
     int32_t *path = a.path + (size_t)b * a.max_rows;
-    int count = 0, at = n > 0 ? 0 : -1, next = -1;
+    int count = 0, at = n > 0 ? 0 : -1, last = -1;
     while (at >= 0) {
         if (lane == 0) path[count] = at;
         ++count;
-        next = a.pick[start + at];
-        const int to = a.taken[start + at];
+        last = at;
+        const int to = taken[at];
         at = to > at && to < n ? to : -1;  // (a row that no sequence claimed holds anything)
     }
     for (int i = count + lane; i < a.max_rows; i += 64) path[i] = -1;
     if (lane == 0) {
         a.accepted[b] = count;
-        a.next[b] = next;
+        a.next[b] = last < 0 ? -1 : a.pick[start + last];
     }
+}
+
+// Chunks of 2^11 values where those of all rows fill the chip (a wave each, 16 a
+// CU), else of 2^9.
+int verify_shift(int64_t rows, int64_t V) { return rows * ((V + 2047) >> 11) >= 4096 ? LARGE : SMALL; }
+int verify_chunks(int64_t rows, int64_t V) {
+    const int s = verify_shift(rows, V);
+    return (int)((V + (1 << s) - 1) >> s);
+}
+// The most (row, chunk) pairs of up to `rows` rows of up to V values: small
+// chunks are taken up to four times 4095 of them.
+int64_t verify_pairs_most(int64_t rows, int64_t V) {
+    const int64_t large = rows * ((V + 2047) >> 11), small = rows * ((V + 511) >> 9);
+    const int64_t s = small < 4 * 4095 ? small : 4 * 4095;
+    return large > s ? large : s;
+}
+
+template <bool HALF, int SHIFT> static hipError_t launch(const VerifyArgs &a, hipStream_t st) {
+    const unsigned grid = (unsigned)a.rows * ((a.chunks + WAVES - 1) / WAVES);
+    verify_sums_kernel<HALF, SHIFT><<<grid, THREADS, 0, st>>>(a);
+    verify_step_kernel<HALF, SHIFT><<<a.rows, THREADS, 0, st>>>(a, 0);
+    for (int round = 0; round < a.rounds; ++round) {
+        verify_round_kernel<HALF, SHIFT><<<grid, THREADS, 0, st>>>(a, round);
+        verify_step_kernel<HALF, SHIFT><<<a.rows, THREADS, 0, st>>>(a, round + 1);
+    }
+    return hipGetLastError();
 }
 
 hipError_t launch_verify_drafts(const VerifyArgs &a, bool half, hipStream_t st) {
     if (a.rows) {
-        if (half) verify_row_kernel<true><<<a.rows, THREADS, 0, st>>>(a);
-        else verify_row_kernel<false><<<a.rows, THREADS, 0, st>>>(a);
-        const hipError_t e = hipGetLastError();
+        const bool large = verify_shift(a.rows, a.V) == LARGE;
+        const hipError_t e = half ? (large ? launch<true, LARGE>(a, st) : launch<true, SMALL>(a, st))
+                                  : (large ? launch<false, LARGE>(a, st) : launch<false, SMALL>(a, st));
         if (e != hipSuccess) return e;
     }
     verify_path_kernel<<<a.batch, 64, 0, st>>>(a);

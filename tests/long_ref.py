@@ -110,8 +110,7 @@ def verify(x, tokens, parents, row_start, accept_u, sample_u, max_rows, draft=No
             if np.isnan(row).any() or not np.isfinite(row.max()):
                 break
             with np.errstate(under="ignore"):
-                d = (row - row.max()) * (1.0 / temperature)
-                p = np.where(d >= -700, np.exp(np.maximum(d, -700)), 0)
+                p = np.exp((row - row.max()) / temperature)
             p /= p.sum()
             kids = [t for t in range(at + 1, n) if parents[s + t] == at]
             go = -1

@@ -1690,6 +1690,13 @@ static int check_blocks(const q3vl_kv_blocks *p, const q3vl_kv_cache *c) {
     return Q3VL_OK;
 }
 
+// Sequences or heads that share rows cannot be written one by one.
+static int check_own_rows(const q3vl_kv_cache *c) {
+    if ((c->batch > 1 && !c->seq_stride) || (c->kv_heads > 1 && !c->head_stride))
+        return fail(Q3VL_ERR_INVALID_ARGUMENT, "sequences or heads of the cache share their rows");
+    return Q3VL_OK;
+}
+
 // Whether `per` workgroups for each (sequence, kv head) are a launch.
 static bool blocks_fit(const q3vl_kv_cache *c, int64_t per) {
     return per <= kMaxGrid && per * c->kv_heads <= kMaxGrid && per * c->kv_heads <= kMaxGrid / c->batch;
@@ -1698,7 +1705,7 @@ static bool blocks_fit(const q3vl_kv_cache *c, int64_t per) {
 int q3vl_kv_pack(const q3vl_kv_cache *cache, const q3vl_kv_blocks *blocks, const int32_t *cache_len,
                  const int32_t *packed_len, q3vl_stream stream) {
     int rc = check_cache(cache);
-    if (rc || (rc = check_blocks(blocks, cache))) return rc;
+    if (rc || (rc = check_blocks(blocks, cache)) || (rc = check_own_rows(cache))) return rc;
     if (!cache_len || !packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "null pointer");
     if (!blocks_fit(cache, cache->max_seq / 32))
         return fail(Q3VL_ERR_UNSUPPORTED, "cache too large: batch=%d kv_heads=%d max_seq=%d", cache->batch, cache->kv_heads, cache->max_seq);
@@ -1736,7 +1743,7 @@ int q3vl_kv_advance(const q3vl_kv_cache *cache, const q3vl_kv_blocks *blocks, in
 int q3vl_kv_unpack(const q3vl_kv_blocks *blocks, const int32_t *packed_len, const int32_t *first,
                    const q3vl_kv_cache *cache, int count, q3vl_stream stream) {
     int rc = check_cache(cache);
-    if (rc || (rc = check_blocks(blocks, cache))) return rc;
+    if (rc || (rc = check_blocks(blocks, cache)) || (rc = check_own_rows(cache))) return rc;
     if (count < 0 || count > cache->max_seq)
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "count=%d: 0 to the cache's max_seq=%d", count, cache->max_seq);
     if (count == 0) return Q3VL_OK;
@@ -1767,6 +1774,8 @@ static int check_long_attention(size_t rows, int heads, int max_rows, int max_le
                                 const q3vl_kv_blocks *p) {
     int rc = check_tree_attention(rows, heads, max_rows, max_len, c);
     if (rc || (p && (rc = check_blocks(p, c)))) return rc;
+    if (p && (int64_t)c->max_seq + (int64_t)p->blocks * 32 > 0x7fffff00)
+        return fail(Q3VL_ERR_UNSUPPORTED, "too many positions: %d packed and %d", p->blocks * 32, c->max_seq);
     if (window < 0 || sinks < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "window=%d sinks=%d", window, sinks);
     if (sinks && !window) return fail(Q3VL_ERR_INVALID_ARGUMENT, "sinks=%d without a window", sinks);
     return Q3VL_OK;
@@ -1888,7 +1897,7 @@ int q3vl_verify_drafts(const void *logits, size_t ld, int dtype, const float *dr
     if (batch < 0 || max_rows < 0) return fail(Q3VL_ERR_INVALID_ARGUMENT, "bad shape batch=%d max_rows=%d", batch, max_rows);
     if (max_rows > kDraftRows)
         return fail(Q3VL_ERR_UNSUPPORTED, "max_rows=%d: at most %d rows a sequence", max_rows, kDraftRows);
-    const double per = 1.4426950408889634 / temperature;
+    const double per = 32.0 * 1.4426950408889634 / temperature;
     if (!(temperature > 0.0 && per > 0.0 && per * 3.5e38 < INFINITY))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "temperature=%g: positive and finite, the logits over it too", temperature);
     if (batch == 0) return Q3VL_OK;

@@ -387,14 +387,14 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
     };
 
     // ---- what a row's window holds: positions from lo[] on, and below `sinks`
-    int lo[NR], lo_most = INT_MIN;  // (lo_most: of this wave's rows)
+    int lo[NR], lo_most = 0;  // (lo_most: of this wave's rows)
     const bool windowed = a.window != 0;
     if (windowed) {
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) lo[nr] = (int)max(window_from(a, s, tok[nr]), (int64_t)INT_MIN);
+        for (int nr = 0; nr < NR; ++nr) lo[nr] = (int)max(window_from(a, s, tok[nr]), (int64_t)0);
         const int last = min((r0 + (SHARED ? (wid + 1) * 16 * NR : T::BM) - 1) / group, n - 1);
         const int64_t most = (int64_t)before + (a.mask ? min((int64_t)0, (int64_t)s.n - a.window) : (int64_t)last + 1 - a.window);
-        lo_most = (int)max(most, (int64_t)INT_MIN);
+        lo_most = (int)max(most, (int64_t)0);
     }
     // whether all of this wave's rows see positions j .. j + 31, as far as the window goes
     auto inside = [&](int j) { return !windowed || j >= lo_most || j + 32 <= a.sinks; };

@@ -314,7 +314,7 @@ struct VerifyArgs {
     const int32_t *tokens, *parents, *row_start;
     const float *accept_u, *sample_u;
     int batch, rows, V, max_rows;
-    double per;  // log2 e / temperature
+    double per;  // 32 log2 e / temperature
     int32_t *accepted, *path, *next;
     int chunks;             // of a row
     int rounds;             // of tests that leave sums (with draft probabilities)

@@ -29,24 +29,38 @@ namespace {
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int SMALL = 9, LARGE = 11;  // chunks of 2^9 or 2^11 values
 
-// 2^y for y <= 0: y = n + f, |f| <= 1/2, and 2^f by the polynomial of degree 11
-// that takes its values at the Chebyshev nodes (2e-17 off, relatively).
-__device__ __forceinline__ double exp2_64(double y) {
-    y = fmax(y, -2000.0);  // (0 then: a double's least is 2^-1074)
-    const double n = __builtin_rint(y), f = y - n;
-    constexpr double C[12] = {1.0, 0.69314718055994529, 0.24022650695910158, 0.055504108664821625, 0.0096181291075872564,
-                              0.0013333558146406471, 0.00015403530463724353, 1.5252733841556773e-05, 1.3215432535912375e-06,
-                              1.0178057087733941e-07, 7.0741942972885211e-09, 4.4558179083360645e-10};
-    double r = C[11];
-#pragma unroll
-    for (int k = 10; k >= 0; --k) r = fma(r, f, C[k]);
-    return __builtin_ldexp(r, (int)n);
+// 2^(z / 32) for z <= 0: z = n + f, |f| <= 1/2, 2^(n / 32) from a table of the 32
+// fractions, and 2^(f / 32) by the polynomial of degree 5 that takes its values at
+// the Chebyshev nodes (1.4e-16 off, relatively). Without the table the degree is
+// 11: 164 rows' sums 26.0 us for 24.0.
+__constant__ double kFractions[32] = {
+    1.0, 1.0218971486541166, 1.0442737824274138, 1.0671404006768237, 1.0905077326652577, 1.1143867425958924, 1.1387886347566916,
+    1.1637248587775775, 1.189207115002721, 1.215247359980469, 1.241857812073484, 1.2690509571917332, 1.2968395546510096,
+    1.3252366431597413, 1.3542555469368927, 1.383909881963832, 1.4142135623730951, 1.4451808069770467, 1.4768261459394993,
+    1.5091644275934228, 1.5422108254079407, 1.5759808451078865, 1.6104903319492543, 1.6457554781539649, 1.681792830507429,
+    1.7186192981224779, 1.7562521603732995, 1.7947090750031072, 1.8340080864093424, 1.8741676341103, 1.9152065613971474,
+    1.9571441241754002};
+__device__ __forceinline__ void fill_table(double *table) {  // (a barrier follows)
+    if (threadIdx.x < 32) table[threadIdx.x] = kFractions[threadIdx.x];
 }
-// e^((x - m) / T), with per = log2 e / T
+__device__ __forceinline__ double exp2_64(double z, const double *table) {
+    z = fmax(z, -64000.0);  // (0 then: a double's least is 2^-1074)
+    const double n = __builtin_rint(z), f = z - n;
+    const int i = (int)n;
+    double r = 3.9737266313166245e-11;
+    r = fma(r, f, 9.1726164981598514e-09);
+    r = fma(r, f, 1.6938509724215757e-06);
+    r = fma(r, f, 0.00023459619819720339);
+    r = fma(r, f, 0.02166084939249829);
+    r = fma(r, f, 1.0);
+    return __builtin_ldexp(r * table[i & 31], i >> 5);
+}
+// e^((x - m) / T), with per = 32 log2 e / T
 struct Weight {
     double per, top;
-    __device__ __forceinline__ Weight(float m, double p) : per(p), top(m) {}
-    __device__ __forceinline__ double operator()(float x) const { return exp2_64(((double)x - top) * per); }
+    const double *table;
+    __device__ __forceinline__ Weight(float m, double p, const double *t) : per(p), top(m), table(t) {}
+    __device__ __forceinline__ double operator()(float x) const { return exp2_64(((double)x - top) * per, table); }
 };
 __device__ __forceinline__ double draft_of(float q) { return q > 0.0f ? (double)q : 0.0; }
 
@@ -103,6 +117,16 @@ template <bool HALF> __device__ __forceinline__ float value_of(const void *x, in
     return HALF ? h2f(static_cast<const uint16_t *>(x)[i]) : static_cast<const float *>(x)[i];
 }
 
+// EACH values of a row from `i` on; behind its end `rest`.
+template <bool HALF, int EACH> __device__ __forceinline__ void load_few(const void *x, int i, int V, float rest, float (&v)[EACH]) {
+    if constexpr (EACH % 4 == 0) {
+        load_values<HALF, EACH>(x, i, 4, V, rest, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) v[k] = i + k < V ? value_of<HALF>(x, i + k) : rest;
+    }
+}
+
 // (a row's chunks by wave: -1 past the last)
 __device__ __forceinline__ int chunk_of(const VerifyArgs &a, int &r) {
     const int blocks = (a.chunks + WAVES - 1) / WAVES;
@@ -119,12 +143,16 @@ constexpr int OPEN = -2;  // taken[] of a row that waits for a round's sums
 // of its weights.
 template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verify_sums_kernel(VerifyArgs a) {
     constexpr int PER = (1 << SHIFT) / 64;
+    __shared__ double table[32];
     const int lane = threadIdx.x & 63;
     int r;
     const int c = chunk_of(a, r);
-    if (c < 0) return;
     float v[PER];
-    load_values<HALF, PER>(row_of<HALF>(a, r), (c << SHIFT) + lane * 4, 256, a.V, -INFINITY, v);
+    // (a wave past the last chunk reads nothing: from 0 on, of a row of none)
+    load_values<HALF, PER>(row_of<HALF>(a, r), (max(c, 0) << SHIFT) + lane * 4, 256, c < 0 ? 0 : a.V, -INFINITY, v);
+    fill_table(table);
+    __syncthreads();
+    if (c < 0) return;
     float m = -INFINITY;
     bool bad = false;
 #pragma unroll
@@ -136,7 +164,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
     bad = __any(bad);
     double s = 0.0;
     if (m > -INFINITY && !bad) {
-        const Weight w(m, a.per);
+        const Weight w(m, a.per, table);
 #pragma unroll
         for (int k = 0; k < PER; ++k) s += w(v[k]);
     }
@@ -150,15 +178,19 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
 // A round: of the rows that wait, the chunk's sum of max(e - c q, 0).
 template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verify_round_kernel(VerifyArgs a, int round) {
     constexpr int PER = (1 << SHIFT) / 64;
+    __shared__ double table[32];
     const int lane = threadIdx.x & 63;
     int r;
     const int chunk = chunk_of(a, r);
-    if (chunk < 0 || a.taken[r] != OPEN) return;
+    if (a.taken[r] != OPEN) return;  // (the whole workgroup)
+    fill_table(table);
+    __syncthreads();
+    if (chunk < 0) return;
     const VerifyRow s = a.state[r];
     float v[PER], q[PER];
     load_values<HALF, PER>(row_of<HALF>(a, r), (chunk << SHIFT) + lane * 4, 256, a.V, -INFINITY, v);
     load_values<false, PER>(a.draft + (size_t)r * a.ldp, (chunk << SHIFT) + lane * 4, 256, a.V, 0.0f, q);
-    const Weight w(s.m, a.per);
+    const Weight w(s.m, a.per, table);
     double z = 0.0;
 #pragma unroll
     for (int k = 0; k < PER; ++k) z += fmax(w(v[k]) - s.c * draft_of(q[k]), 0.0);
@@ -172,7 +204,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
 // step no row stays open: further sums are made here, chunk by chunk.
 template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verify_step_kernel(VerifyArgs a, int round) {
     constexpr int PER = (1 << SHIFT) / 64, EACH = (1 << SHIFT) / THREADS;
-    __shared__ double sums[WAVES];
+    __shared__ double sums[WAVES], table[32];
     __shared__ uint64_t kids[kDraftRows / 64];
     __shared__ int token[kDraftRows];                       // of the children
     __shared__ float accept[kDraftRows], logit[kDraftRows], draft[kDraftRows];
@@ -181,21 +213,40 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
     if (round > 0 && a.taken[r] != OPEN) return;
     const void *x = row_of<HALF>(a, r);
 
-    // ---- the row's maximum and sum (each wave for itself, in one order)
+    // what does not depend on anything: loads under way together
     const float *top = a.chunk_top + (size_t)r * a.chunks;
     const double *sum = a.chunk_sum + (size_t)r * a.chunks;
-    float m = -INFINITY;
-    for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, top[c]);  // (+inf where the row cannot be judged)
-    m = wave_max(m);
+    constexpr int HELD = 5;  // chunks that a lane keeps (a row of up to 320; others are read again)
+    float tops[HELD];
+    double held[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int c = lane + 64 * k;
+        tops[k] = c < a.chunks ? top[c] : -INFINITY;
+        held[k] = c < a.chunks ? sum[c] : 0.0;
+    }
+    const double number = (double)a.sample_u[r];
+    int found_seq = -1;
+    for (int b = tid; b < a.batch; b += THREADS)
+        if (a.row_start[b] <= r && r < a.row_start[b + 1]) found_seq = b;
+    fill_table(table);
+    if (tid == 0) {
+        seq = -1;
+        first_at = INT_MAX;
+        last_at = -1;
+    }
+    __syncthreads();
+    if (found_seq >= 0) atomicMax(&seq, found_seq);
+    __syncthreads();
 
     // ---- its sequence and its children there
-    if (tid == 0) seq = -1;
-    __syncthreads();
-    for (int b = tid; b < a.batch; b += THREADS)
-        if (a.row_start[b] <= r && r < a.row_start[b + 1]) atomicMax(&seq, b);
-    __syncthreads();
     const int start = seq < 0 ? r : max(a.row_start[seq], 0);
     const int n = seq < 0 ? 0 : min(min(a.row_start[seq + 1], a.rows) - start, a.max_rows), t = r - start;
+    float m = -INFINITY;  // (+inf where the row cannot be judged)
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) m = fmaxf(m, tops[k]);
+    for (int c = lane + 64 * HELD; c < a.chunks; c += 64) m = fmaxf(m, top[c]);
+    m = wave_max(m);
     if (t >= n || !(m > -INFINITY && m < INFINITY)) {
         if (tid == 0) {
             a.pick[r] = -1;
@@ -205,23 +256,34 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
     }
     for (int w = wave; w < kDraftRows / 64; w += WAVES) {
         const int i = w * 64 + lane;
-        bool kid = i < n && i > t && a.parents[start + i] == t;
-        if (kid) {
-            const int tok = a.tokens[start + i];
-            kid = tok >= 0 && tok < a.V;
-            token[i] = tok;
-            if (kid && a.draft) {
-                accept[i] = a.accept_u[start + i];
-                logit[i] = value_of<HALF>(x, tok);
-                draft[i] = a.draft[(size_t)r * a.ldp + tok];
+        bool kid = false;
+        if (w * 64 < n) {
+            const int at = start + min(i, n - 1), tok = a.tokens[at];
+            const float u = a.draft ? a.accept_u[at] : 0.0f;
+            kid = i < n && i > t && a.parents[at] == t && tok >= 0 && tok < a.V;
+            if (kid) {
+                token[i] = tok;
+                if (a.draft) {
+                    accept[i] = u;
+                    logit[i] = value_of<HALF>(x, tok);
+                    draft[i] = a.draft[(size_t)r * a.ldp + tok];
+                }
             }
         }
         const uint64_t bits = __ballot(kid);
         if (lane == 0) kids[w] = bits;
     }
-    const Weight weight(m, a.per);
+
+    // ---- the sum of its weights (each wave for itself, in one order)
+    const Weight weight(m, a.per, table);
     double total = 0.0;
-    for (int c = lane; c < a.chunks; c += 64) total = fma(sum[c], weight(top[c]), total);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        if (64 * k >= a.chunks) break;
+        held[k] *= weight(tops[k]);
+        total += held[k];
+    }
+    for (int c = lane + 64 * HELD; c < a.chunks; c += 64) total += sum[c] * weight(top[c]);
     total = wave_sum(total);
     __syncthreads();
 
@@ -289,14 +351,11 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
 
     // ---- the token by the inverse of the cumulated weights
     if (taken < 0) {
-        const double want = (double)a.sample_u[r] * z;
+        const double want = number * z;
         double before = 0.0, ahead = 0.0;  // sums of earlier chunks: than the next 64, than the one chosen
         int chunk = -1, last = 0;
         double last_ahead = 0.0;
-        for (int base = 0; base < a.chunks && chunk < 0; base += 64) {
-            const int i = base + lane;
-            double v = 0.0;
-            if (i < a.chunks) v = left ? left[i] : sum[i] * weight(top[i]);
+        auto look = [&](int base, double v) {  // at 64 chunks' sums
             const double run = wave_scan(v);
             const uint64_t over = __ballot(v > 0.0 && before + run > want), some = __ballot(v > 0.0);
             const int at = over ? __ffsll((unsigned long long)over) - 1 : some ? 63 - __clzll((long long)some) : 0;
@@ -309,6 +368,15 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
                 last_ahead = prior;
             }
             before += __shfl(run, 63);
+        };
+        if (!left) {
+#pragma unroll
+            for (int k = 0; k < HELD; ++k)
+                if (chunk < 0 && 64 * k < a.chunks) look(64 * k, held[k]);
+        }
+        for (int base = left ? 0 : 64 * HELD; base < a.chunks && chunk < 0; base += 64) {
+            const int i = base + lane;
+            look(base, i < a.chunks ? (left ? left[i] : sum[i] * weight(top[i])) : 0.0);
         }
         if (chunk < 0) {  // (the numbers' last bits)
             chunk = last;
@@ -316,20 +384,18 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
         }
         // EACH values in a row a thread
         const int first = (chunk << SHIFT) + tid * EACH;
+        float v[EACH], p[EACH];
+        load_few<HALF, EACH>(x, first, a.V, -INFINITY, v);
+        if (c > 0.0) load_few<false, EACH>(a.draft + (size_t)r * a.ldp, first, a.V, 0.0f, p);
         double w[EACH], mine = 0.0;
 #pragma unroll
         for (int k = 0; k < EACH; ++k) {
-            const int i = first + k;
-            w[k] = i < a.V ? weight(value_of<HALF>(x, i)) : 0.0;
-            if (c > 0.0 && i < a.V) w[k] = fmax(w[k] - c * draft_of(a.draft[(size_t)r * a.ldp + i]), 0.0);
+            w[k] = weight(v[k]);
+            if (c > 0.0) w[k] = fmax(w[k] - c * draft_of(p[k]), 0.0);
             mine += w[k];
         }
         const double run = wave_scan(mine);
         if (lane == 63) sums[wave] = run;
-        if (tid == 0) {
-            first_at = INT_MAX;
-            last_at = -1;
-        }
         __syncthreads();
         double at = ahead + (run - mine);
         for (int v = 0; v < wave; ++v) at += sums[v];

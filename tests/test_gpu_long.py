@@ -372,6 +372,14 @@ def test_unseen_infinities(half, T):
     assert np.isnan(got[0, :128]).all()
 
 
+@pytest.mark.parametrize("T", [1, 40])
+def test_windows_of_any_size(T):
+    """The largest windows and first parts there are: everything is seen."""
+    for window, sinks in ((2 ** 31 - 1, 0), (2 ** 31 - 1, 2 ** 31 - 1), (100, 2 ** 31 - 1)):
+        B = Long(T, [T, 1], [40, 3], [320, 64], 4, 2, 64, False, T > 1, window=window, sinks=sinks)
+        B.check(B.run())
+
+
 def test_windows_leave_infinities_unseen():
     """NaN in fp16 rows that a window passes over, beside ones it holds."""
     for T in (1, 4, 70):

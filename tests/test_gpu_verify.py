@@ -68,6 +68,14 @@ def test_sizes(V, tree, probs):
         Drafts(V + half, rows, V, tree, probs, half, pad=2).check(temperature=0.8 if half else 1.0)
 
 
+@pytest.mark.parametrize("probs", [False, True])
+@pytest.mark.parametrize("V,rows", [(400_001, [4, 2]), (700_003, [7, 7])], ids=str)
+def test_more_chunks_than_a_lane_keeps(V, rows, probs):
+    """Rows of more chunks than the sums held in registers, small and large ones;
+    flat ones, so that tokens come from all over them."""
+    Drafts(V, rows, V, True, probs, spread=0.3, near=1.5).check()
+
+
 @pytest.mark.parametrize("tree,probs", KINDS, ids=["chain", "chain probs", "tree", "tree probs"])
 def test_paths_of_all_lengths(tree, probs):
     """Many sequences whose drafts are good: paths end everywhere."""

@@ -52,6 +52,14 @@ def test_pack_refusals(fn, over, code, text):
     refused(pack(fn=fn, **over), code, text)
 
 
+def test_caches_that_share_rows_are_not_written():
+    for over in (dict(seq_stride=0), dict(head_stride=0)):
+        refused(pack(cache_over=over), BAD, "share their rows")
+        refused(unpack(cache_over=over), BAD, "share their rows")
+    assert pack(cache_over=dict(seq_stride=0, batch=1), blocks_over=dict(batch=1), cache_len=None) == BAD
+    assert "null" in q.last_error()
+
+
 def test_pack_sizes_and_one_array():
     refused(pack(cache_over=dict(batch=1 << 20, max_seq=1 << 20), blocks_over=dict(batch=1 << 20)), UNS, "too large")
     refused(pack(fn="q3vl_kv_advance", packed_len=P), BAD, "one array")
@@ -104,6 +112,7 @@ def attn(cache_over={}, blocks_over={}, **over):
     (dict(q=None), BAD, "null"),
     (dict(row_start=None), BAD, "null"),
     (dict(rows=1 << 30), UNS, "too large"),
+    (dict(cache_over=dict(max_seq=2 ** 31 - 1000), blocks_over=dict(blocks=1 << 24)), UNS, "too many positions"),
 ])
 def test_long_attention_refusals(over, code, text):
     refused(attn(**over), code, text)

@@ -183,6 +183,40 @@ __device__ void long_row(const LongAttnArgs &a, const LongSeq &s, int b, int t, 
 }  // namespace
 
 // ------------------------------------------------------------ the kernel
+// Scores, softmax and values of 32 positions a step as in tree_attention_kernel,
+// which tells the layout: S^T = K Q^T and O^T = V^T P^T by v_mfma_f32_16x16x32_f16,
+// a query row in a lane, p held as 2^(s sc + bias). fp16 rows come as they do there.
+// What differs:
+//
+// Packed blocks. int8 are exact in fp16, so a block's integers are operands as they
+// are, and its scales are factors: the keys' of the score (sc ks), the values' of
+// the probability, p vs. vs goes relative to U, a power of two that the largest
+// scale so far fits, so that p vs stays within fp16; O is in units of U until the
+// packed positions are done. l sums p itself, in fp32 and in the lane: a key with
+// much weight and tiny values must count in it. So nothing is held coarser than
+// tree_attention holds it (of p vs nothing finer than 2^-31 of the largest p times
+// the largest scale).
+//
+// Few rows: a wave takes a block of every four, 16 bytes a lane and load, straight
+// from memory into operand registers (the block's order is theirs) and widens them
+// there; a block's registers are filled again as soon as they are read, the next
+// block is on its way meanwhile. No LDS, no barrier. Bound by the reads: one token
+// each of 24 sequences of up to 12000, 472 MB, 81 us, 5.8 TB/s, 32 of 16384 all
+// alike 6.5 (a plain read here: 6.46); the rest is sequences of different length.
+// Of the busy cycles the matrix cores work in 16 of 100 and other vector
+// instructions run in 42.
+//
+// Many rows: the four waves each widen a quarter of the next 64 positions into LDS,
+// in the operands' order, read ahead by a turn (each wave widening all of them for
+// itself: three trees of 61 rows over 16000 128 us for 63). Trees 63 us, 1000 rows
+// behind 8000 in fp16 91; matrix cores 33 and 34 of 100, other vector instructions
+// 35 and 44, two waves a SIMD.
+//
+// A window. The turns that no row of the workgroup sees are left out: the ones of
+// the first positions come first, then from the earliest window's start on. Within
+// the others a lane masks what its row does not see, where some row does not see
+// all. One token of 16 sequences through 4096 positions 45 us, 6.0 TB/s; a prompt
+// of 4000 through 1024 in fp16 48 us.
 template <int D, int NR, bool SHARED, bool PACKED> struct LongTile {
     static constexpr int RB = 2 * D;                           // bytes of an fp16 row
     static constexpr int NS = SHARED ? 2 : PACKED ? 128 / D : 256 / D;  // stages of fp16 rows

@@ -18,7 +18,14 @@
 // the chunk in which the cumulated sums pass the row's number and the value in
 // it. A row whose child is rejected waits for a round: its chunks' sums of max(p
 // - c q, 0), by all workgroups again, then the next test. So each logit is read
-// once, or once more for each rejection.
+// once, or once more for each rejection. Two rounds are launched; a row that they
+// leave open goes on by itself, a workgroup for all its chunks.
+//
+// us at 151936 values, fp32: the sums of 83 rows 15.8, of 164 23.7 (4.2 TB/s: 64-bit
+// conversions and products, 69 of 100 busy cycles in vector instructions), a step
+// 12 (its chain of loads: lengths, parents and tokens, logits, the chunk), a round
+// of which most rows have no part 13, the path 3. Each step of all tests in one
+// workgroup a row took 545 for the 83.
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 

@@ -71,24 +71,36 @@ struct Weight {
 };
 __device__ __forceinline__ double draft_of(float q) { return q > 0.0f ? (double)q : 0.0; }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
-    return v;
+// A lane's value from the lane `ctrl` says, 0 where there is none or `rows` (of 16
+// lanes, a bit each) leaves it out: data-parallel moves, an eighth of the latency
+// of an exchange through LDS.
+template <int ctrl, int rows> __device__ __forceinline__ double moved(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, ctrl, rows, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), ctrl, rows, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 __device__ __forceinline__ double wave_scan(double v) {  // inclusive
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const double o = __shfl_up(v, k);
-        if (lane >= k) v += o;
-    }
+    v += moved<0x111, 0xF>(v);  // from 1, 2, 4, 8 lanes before in the row
+    v += moved<0x112, 0xF>(v);
+    v += moved<0x114, 0xF>(v);
+    v += moved<0x118, 0xF>(v);
+    v += moved<0x142, 0xA>(v);  // lane 15 of the row before, to rows 1 and 3
+    v += moved<0x143, 0xC>(v);  // lane 31, to rows 2 and 3
     return v;
 }
+__device__ __forceinline__ double lane_value(double v, int lane) {  // (lane uniform)
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum(double v) { return lane_value(wave_scan(v), 63); }
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) v = fmaxf(v, __shfl_xor(v, k));
-    return v;
+    v = row16_max(v);
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
 // (rows may begin anywhere)
@@ -366,7 +378,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
             const double run = wave_scan(v);
             const uint64_t over = __ballot(v > 0.0 && before + run > want), some = __ballot(v > 0.0);
             const int at = over ? __ffsll((unsigned long long)over) - 1 : some ? 63 - __clzll((long long)some) : 0;
-            const double prior = before + (at ? __shfl(run, at - 1) : 0.0);
+            const double prior = before + (at ? lane_value(run, at - 1) : 0.0);
             if (over) {
                 chunk = base + at;
                 ahead = prior;
@@ -374,7 +386,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
                 last = base + at;
                 last_ahead = prior;
             }
-            before += __shfl(run, 63);
+            before += lane_value(run, 63);
         };
         if (!left) {
 #pragma unroll

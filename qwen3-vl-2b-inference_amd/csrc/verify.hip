@@ -21,11 +21,11 @@
 // once, or once more for each rejection. Two rounds are launched; a row that they
 // leave open goes on by itself, a workgroup for all its chunks.
 //
-// us at 151936 values, fp32: the sums of 83 rows 15.8, of 164 23.7 (4.2 TB/s: 64-bit
+// us at 151936 values, fp32: the sums of 83 rows 15.9, of 164 24.3 (4.1 TB/s: 64-bit
 // conversions and products, 69 of 100 busy cycles in vector instructions), a step
-// 12 (its chain of loads: lengths, parents and tokens, logits, the chunk), a round
-// of which most rows have no part 13, the path 3. Each step of all tests in one
-// workgroup a row took 545 for the 83.
+// 6.6 (its chain of loads: lengths, parents and tokens, logits, the chunk), a round
+// of which two rows in five have a part 12.9, the path 3 to 4. All tests and the
+// choice in one workgroup a row took 545 for the 83.
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"
 
@@ -227,7 +227,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
     __shared__ uint64_t kids[kDraftRows / 64];
     __shared__ int token[kDraftRows];                       // of the children
     __shared__ float accept[kDraftRows], logit[kDraftRows], draft[kDraftRows];
-    __shared__ int seq, first_at, last_at;
+    __shared__ int seq, first_at[WAVES], last_at[WAVES];
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (round > 0 && a.taken[r] != OPEN) return;
     const void *x = row_of<HALF>(a, r);
@@ -249,11 +249,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
     for (int b = tid; b < a.batch; b += THREADS)
         if (a.row_start[b] <= r && r < a.row_start[b + 1]) found_seq = b;
     fill_table(table);
-    if (tid == 0) {
-        seq = -1;
-        first_at = INT_MAX;
-        last_at = -1;
-    }
+    if (tid == 0) seq = -1;
     __syncthreads();
     if (found_seq >= 0) atomicMax(&seq, found_seq);
     __syncthreads();
@@ -273,20 +269,18 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
         }
         return;
     }
-    for (int w = wave; w < kDraftRows / 64; w += WAVES) {
+    const int words = (n + 63) >> 6;
+    for (int w = wave; w < words; w += WAVES) {
         const int i = w * 64 + lane;
-        bool kid = false;
-        if (w * 64 < n) {
-            const int at = start + min(i, n - 1), tok = a.tokens[at];
-            const float u = a.draft ? a.accept_u[at] : 0.0f;
-            kid = i < n && i > t && a.parents[at] == t && tok >= 0 && tok < a.V;
-            if (kid) {
-                token[i] = tok;
-                if (a.draft) {
-                    accept[i] = u;
-                    logit[i] = value_of<HALF>(x, tok);
-                    draft[i] = a.draft[(size_t)r * a.ldp + tok];
-                }
+        const int at = start + min(i, n - 1), tok = a.tokens[at];
+        const float u = a.draft ? a.accept_u[at] : 0.0f;
+        const bool kid = i < n && i > t && a.parents[at] == t && tok >= 0 && tok < a.V;
+        if (kid) {
+            token[i] = tok;
+            if (a.draft) {
+                accept[i] = u;
+                logit[i] = value_of<HALF>(x, tok);
+                draft[i] = a.draft[(size_t)r * a.ldp + tok];
             }
         }
         const uint64_t bits = __ballot(kid);
@@ -326,7 +320,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
             rejected = round;
             z = join(a.round_sum + ((size_t)(round - 1) * a.rows + r) * a.chunks);
         }
-        for (int w = from >> 6; w < kDraftRows / 64 && taken < 0; ++w) {
+        for (int w = from >> 6; w < words && taken < 0; ++w) {
             uint64_t k = kids[w];
             if (w == from >> 6) k &= ~0ull << (from & 63);
             for (; k; k &= k - 1) {
@@ -427,12 +421,25 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
                 if (at > want && found == INT_MAX) found = first + k;
             }
         }
-        if (found != INT_MAX) atomicMin(&first_at, found);
-        if (some >= 0) atomicMax(&last_at, some);
+        // (the values ascend with the lanes and waves)
+        const uint64_t over = __ballot(found != INT_MAX), any = __ballot(some >= 0);
+        if (lane == 0) {
+            first_at[wave] = INT_MAX;
+            last_at[wave] = -1;
+        }
+        if (over && lane == __ffsll((unsigned long long)over) - 1) first_at[wave] = found;
+        if (any && lane == 63 - __clzll((long long)any)) last_at[wave] = some;
         __syncthreads();
-        pick = first_at != INT_MAX ? first_at : last_at;
+        int last_value = -1;
+        pick = INT_MAX;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            pick = min(pick, first_at[w]);
+            last_value = max(last_value, last_at[w]);
+        }
+        if (pick == INT_MAX) pick = last_value;
         if (!a.draft)  // the first child that has the token
-            for (int w = 0; w < kDraftRows / 64 && taken < 0; ++w)
+            for (int w = 0; w < words && taken < 0; ++w)
                 for (uint64_t k = kids[w]; k; k &= k - 1) {
                     const int child = w * 64 + __ffsll((unsigned long long)k) - 1;
                     if (token[child] == pick) {

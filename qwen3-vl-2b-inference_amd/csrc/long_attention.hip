@@ -190,7 +190,7 @@ __device__ void long_row(const LongAttnArgs &a, const LongSeq &s, int b, int t, 
 //
 // Packed blocks. int8 are exact in fp16, so a block's integers are operands as they
 // are, and its scales are factors: the keys' of the score (sc ks), the values' of
-// the probability, p vs. vs goes relative to U, a power of two that the largest
+// the probability, p vs. vs goes relative to U, a power of two that the largest (of either sign)
 // scale so far fits, so that p vs stays within fp16; O is in units of U until the
 // packed positions are done. l sums p itself, in fp32 and in the lane: a key with
 // much weight and tiny values must count in it. So nothing is held coarser than
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
     // largest scale of values so far fits.
     float U = 0.0f, to_units = 0.0f;
     auto new_units = [&](float vs) {
-        if (vs > U) {  // (uniform)
+        if (fabsf(vs) > U) {  // (uniform)
             const int e = __builtin_amdgcn_frexp_expf(vs);
             const float r = U > 0.0f ? ldexpf(U, -e) : 0.0f;
             U = ldexpf(1.0f, e);

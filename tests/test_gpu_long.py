@@ -183,7 +183,7 @@ class Long:
         scale = self.D ** -0.5 if scale is None else scale
         for b, n in enumerate(self.rows):
             k, v, p = self.positions(b)
-            vmax = 127 * float(np.nanmax(self.vs[b, :, :p // 32])) if p else 0.0
+            vmax = 127 * float(np.nanmax(np.abs(self.vs[b, :, :p // 32]))) if p else 0.0
             for t in range(n):
                 r = int(self.st[b]) + t
                 if only is not None and not only(b, t):
@@ -311,6 +311,47 @@ def test_zero_blocks():
     B.ks[:, :, 1], B.vs[:, :, 2] = 0, 0
     B.kn[:, :, 1], B.vn[:, :, 2] = 0, 0
     B.check(B.run())
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 70)])
+@pytest.mark.parametrize("T", [1, 6, 80])
+def test_scales_of_any_sign(T, window, sinks):
+    """Blocks that a caller wrote by its own rule: negative scales, and zeros where
+    a window begins and its first part ends."""
+    B = Long(T + window, [T, 2], [4, 9], [320, 96], 4, 2, 64, False, T > 1, window=window, sinks=sinks)
+    B.ks[:, :, 1::2] *= -1
+    B.vs[:, 0] *= -1
+    B.vs[:, 1, ::3] *= -1
+    B.ks[:, :, 2] = B.ks[:, 1, 5] = B.vs[:, 1, 5] = 0
+    B.check(B.run())
+
+
+@pytest.mark.parametrize("T", [1, 80])
+def test_blocks_past_32_bits(T):
+    """Blocks whose bytes lie more than 2^32 behind the first: seen through a
+    window, packed to and read back."""
+    D, n = 64, (1 << 20) + 3
+    B = Long(T, [1, T], [3, 10], [64, 192], 4, 1, D, False, False, window=100, sinks=5)
+    small = B.tensors()["packed"]
+    k, v = (torch.empty((2, 1, n, 32 * D), dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros((2, 1, n), device="cuda") for _ in range(2))
+    assert k[1, 0, -5].data_ptr() - k.data_ptr() > 2 ** 32 - 2 ** 15 and k[1, 0, -1].data_ptr() - k.data_ptr() >= 2 ** 32
+    for to, x in ((k, small.k), (v, small.v), (ks, small.k_scale), (vs, small.v_scale)):
+        to[0, 0, :2], to[1, 0, 0], to[1, 0, -5:] = x[0, 0, :2], x[1, 0, 0], x[1, 0, 1:6]
+    big = qa.PackedKV(k, v, ks, vs)
+    B.check(B.run(packed=big, packed_len=i32([64, 32 * n])))
+
+    s = Store(T, 2, 1, D, 70, 3)
+    kv, _, cache, few = s.device()
+    qa.kv_pack(cache, few, i32([0, 64]), i32([0, 32]))
+    qa.kv_pack(qa.KVCache(dev(s.k), dev(s.v)), big, i32([0, 64]), i32([0, 32 * (n - 2)]))
+    for got, want in ((k, few.k), (v, few.v), (ks, few.k_scale), (vs, few.v_scale)):
+        assert torch.equal(got[1, 0, -2:], want[1, 0, 1:])
+    back = [[torch.zeros_like(x) for x in kv] for _ in range(2)]
+    qa.kv_unpack(few, i32([0, 96]), qa.KVCache(*back[0]), first=i32([0, 37]), count=70)
+    qa.kv_unpack(big, i32([0, 32 * n]), qa.KVCache(*back[1]), first=i32([0, 32 * (n - 3) + 37]), count=70)
+    for got, want in zip(back[1], back[0]):
+        assert want[1, :, :59].any() and torch.equal(got, want)
 
 
 @pytest.mark.parametrize("qscale", [1e-30, 300.0])

@@ -1050,10 +1050,11 @@ static hipError_t launch_tile(const LongAttnArgs &a, int tiles, hipStream_t st) 
 template <int D, bool HALF, bool PACKED> static hipError_t launch_d(const LongAttnArgs &a, int bm, hipStream_t st) {
     const int tiles = (int)(((int64_t)a.max_rows * (a.heads / a.kv_heads) + bm - 1) / bm);
     // Keys and values that one workgroup reads go past the caches: always with up to
-    // 32 rows in one tile (us past the caches and through them, packed: 24 sequences
-    // of 12000 85 and 96, 40 of 3000 44 and 48, one of 1024 12.6 and 11.5; but trees of
-    // 32 rows in four tiles 141 and 132), of shared tiles where together they are more
-    // than the caches keep.
+    // 32 rows in one tile (us past the caches and through them, packed, three calls'
+    // blocks in turn: one token of 16 sequences of 8000 41.9 and 47.0, of 8 27.0 and
+    // 29.3, of one 13.4 and 14.2; one of 1024 13.1 both; but trees of 32 rows in four
+    // tiles 141 and 132), of shared tiles where together they are more than the caches
+    // keep.
     const bool one = tiles == 1, once = one && (double)a.batch * a.kv_heads * a.max_len * D * (PACKED ? 2 : 4) > 192e6;
     hipError_t e;
     if (PACKED && bm == 16 && !one) e = launch_tile<D, HALF, 1, false, true, false>(a, tiles, st);

@@ -83,6 +83,21 @@ def test_paths_of_all_lengths(tree, probs):
     assert len(set(want[0].tolist())) >= (4 if tree else 8)
 
 
+@pytest.mark.parametrize("probs", [False, True])
+def test_many_sequences(probs):
+    """More sequences than a workgroup has threads, some of none."""
+    Drafts(12, [1, 3, 0, 2, 5] * 130, 70, True, probs, pad=3).check()
+
+
+@pytest.mark.parametrize("temperature", [1e-30, 1e-3, 7.5, 1e30])
+def test_temperatures(temperature):
+    """The largest logit alone, and all that are not ruled out alike."""
+    for probs in (False, True):
+        d = Drafts(13, [5] * 20, 600, True, probs)
+        d.x[:, 1::3] = -np.inf
+        d.check(temperature=temperature)
+
+
 def test_many_children():
     """Rows with many children, tokens that come twice among them, all rejected
     now and then."""

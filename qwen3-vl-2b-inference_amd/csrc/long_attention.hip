@@ -950,7 +950,7 @@ __global__ __launch_bounds__(THREADS) void long_join_kernel(const int32_t *row_s
     a.max_rows = max_rows_p;
     constexpr int LANES = D / 4, SIDE = 64 / LANES;
     const int lane = threadIdx.x & 63, d = lane % LANES * 4, side = lane / LANES;
-    const int x = blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const int x = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hd = x % a.heads, bt = x / a.heads, t = bt % a.max_rows, b = bt / a.max_rows;
     if (b >= a.batch) return;
     const LongSeq s = long_sequence(a, b);
@@ -963,32 +963,47 @@ __global__ __launch_bounds__(THREADS) void long_join_kernel(const int32_t *row_s
             m = part_ml_p[(part + lane) * 2];
             lw = part_ml_p[(part + lane) * 2 + 1];
         }
-        float top = m;
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);  // (nothing seen there: o = l = 0)
-        lw *= f;
-#pragma unroll
-        for (int k = 1; k < 64; k <<= 1) lw += __shfl_xor(lw, k);
         const float *p = part_o_p + part * D + d;
-        for (int k = 0; k < a.splits; k += 4 * SIDE) {
-            float4_t v[4];
+        float4_t v[4];
+        auto load = [&](int k) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int at = k + u * SIDE + side;
                 v[u] = at < a.splits ? *reinterpret_cast<const float4_t *>(p + (size_t)at * D) : float4_t{0, 0, 0, 0};
             }
+        };
+        load(0);
+        const float top = column_max(row16_max(m));
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);  // (nothing seen there: o = l = 0)
+        lw *= f;
+        lw += dpp_f(lw, dpp_xor1);
+        lw += dpp_f(lw, dpp_xor2);
+        lw += dpp_f(lw, dpp_half_mirror);
+        lw += dpp_f(lw, dpp_mirror);
+        lw = column_sum(lw);
+        for (int k = 0; k < a.splits; k += 4 * SIDE) {
+            if (k) load(k);
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const float fk = __shfl(f, min(k + u * SIDE + side, 63));
+                float fk = 0.0f;
+#pragma unroll
+                for (int z = 0; z < SIDE; ++z) {
+                    const float fz = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), min(k + u * SIDE + z, 63)));
+                    fk = side == z ? fz : fk;
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] = fmaf(v[u][e], fk, o[e]);
             }
         }
 #pragma unroll
-        for (int k = LANES; k < 64; k <<= 1)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], k);
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (SIDE == 4) {
+                o[e] = column_sum(o[e]);
+            } else {
+                auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(o[e]), __float_as_uint(o[e]), false, false);
+                o[e] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+            }
+        }
         const float inv = top == -INFINITY ? 0.0f : 1.0f / lw;
         o *= inv;
     } else {
@@ -997,8 +1012,10 @@ __global__ __launch_bounds__(THREADS) void long_join_kernel(const int32_t *row_s
     }
     if (side) return;
     const int64_t at = r * a.ldo + (int64_t)hd * D + d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) put<HALF>(a.out, at + e, o[e]);
+    if constexpr (HALF)
+        *reinterpret_cast<half4_bits *>(static_cast<uint16_t *>(a.out) + at) = half4_bits{f2h(o[0]), f2h(o[1]), f2h(o[2]), f2h(o[3])};
+    else
+        *reinterpret_cast<float4_any *>(static_cast<float *>(a.out) + at) = o;
 }
 
 // Rows of a workgroup and splits.

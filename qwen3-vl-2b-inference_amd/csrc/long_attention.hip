@@ -371,6 +371,16 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
 #pragma unroll
         for (int k = 0; k < PER; ++k) nv[k] = __builtin_amdgcn_raw_buffer_load_b128(rv, (wid * PER + k) * 1024 + lane * 16, 0, NT_BIT);
     };
+    // ... their scales, a turn ahead too (keys', then values'; of the last block twice)
+    float scale[4];
+    auto fetch_scales = [&](int u) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const size_t at = head_blocks + min(u * 2 + k, held - 1);
+            scale[k] = a.k_scale[at];
+            scale[2 + k] = a.v_scale[at];
+        }
+    };
     auto widen_tile = [&](int lds) {
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -557,13 +567,13 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                 for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= r;
         }
     };
-    auto packed_softmax = [&](float ks, float vs, int j) {
-        if (inside(j)) {
+    auto packed_softmax = [&](float ks, float vs, int j, bool there = true) {
+        if (there && inside(j)) {
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) any[nr] = true;
         } else {
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) masked(nr, window_bits(nr, j));
+            for (int nr = 0; nr < NR; ++nr) masked(nr, there ? windowed ? window_bits(nr, j) : 0xFFFFFFFFu : 0u);
         }
         softmax(ks, vs * to_units, kPacked);
     };
@@ -666,6 +676,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
         if constexpr (PACKED) {
             if (u0 < tp) {
                 fetch_tile(turns.at(u0));
+                fetch_scales(turns.at(u0));
                 widen_tile(0);
                 if (u0 + 1 < tp) fetch_tile(turns.at(u0 + 1));
             }
@@ -683,33 +694,56 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                 } else if (t + 1 < u1) {
                     load_tile(turns.at(t + 1), T::STAGE - lds);
                 }
-                const int end = min(held - u * 2, 2);
+                const bool two = u * 2 + 1 < held;  // (else the second block's bytes are zeros, and no row sees it)
+                const float k0 = scale[0], k1 = two ? scale[1] : 1.0f, v0 = scale[2], v1 = scale[3];
+                if (t + 1 < tp) fetch_scales(turns.at(t + 1));
+                const unsigned char *at = smem + lds + lane * 16;
+                auto keys = [&](half8_t (&f)[KS], const unsigned char *p, int kb) {
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) f[i] = *reinterpret_cast<const half8_t *>(p + (kb * KS + i) * 1024);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                auto vals = [&](half8_t (&f)[NT / 2], const unsigned char *p, int part) {
+#pragma unroll
+                    for (int i = 0; i < NT / 2; ++i) f[i] = *reinterpret_cast<const half8_t *>(p + 64 * T::RB + (part * (NT / 2) + i) * 1024);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                // (us a call, scales loaded where they are needed and a loop over the blocks: trees
+                // in fp32 69, a prompt in fp16 100. Scales a turn ahead: 61 and 101; both blocks
+                // in a row, the second's keys read under the first's last products: 68 and 94.)
+                if constexpr (HALF) {
+                    keys(ka, at, 0);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const unsigned char *p = at + k * 64 * D;
+                        keys(kb, p, 1);
+                        scores(ka, 0);
+                        scores(kb, 1);
+                        vals(va, p, 0);
+                        new_units(k ? v1 : v0);
+                        packed_softmax(k ? k1 : k0, k ? v1 : v0, (u * 2 + k) * BLOCK, k == 0 || two);
+                        vals(vb, p, 1);
+                        values(va, 0);
+                        if (k == 0) keys(ka, p + 64 * D, 0);
+                        values(vb, 1);
+                    }
+                } else {
+                    const int end = two ? 2 : 1;
 #pragma unroll 1
-                for (int k = 0; k < end; ++k) {
-                    const int blk = u * 2 + k;
-                    const float ks = a.k_scale[head_blocks + blk], vs = a.v_scale[head_blocks + blk];
-                    const unsigned char *p = smem + lds + k * 64 * D + lane * 16;
-                    auto keys = [&](half8_t (&f)[KS], int kb) {
-#pragma unroll
-                        for (int i = 0; i < KS; ++i) f[i] = *reinterpret_cast<const half8_t *>(p + (kb * KS + i) * 1024);
-                        __builtin_amdgcn_sched_barrier(0);
-                    };
-                    auto vals = [&](half8_t (&f)[NT / 2], int part) {
-#pragma unroll
-                        for (int i = 0; i < NT / 2; ++i)
-                            f[i] = *reinterpret_cast<const half8_t *>(p + 64 * T::RB + (part * (NT / 2) + i) * 1024);
-                        __builtin_amdgcn_sched_barrier(0);
-                    };
-                    keys(ka, 0);
-                    keys(kb, 1);
-                    new_units(vs);
-                    scores(ka, 0);
-                    scores(kb, 1);
-                    vals(va, 0);
-                    packed_softmax(ks, vs, blk * BLOCK);
-                    vals(vb, 1);
-                    values(va, 0);
-                    values(vb, 1);
+                    for (int k = 0; k < end; ++k) {
+                        const unsigned char *p = at + k * 64 * D;
+                        const float ks = k ? k1 : k0, vs = k ? v1 : v0;
+                        keys(ka, p, 0);
+                        keys(kb, p, 1);
+                        scores(ka, 0);
+                        scores(kb, 1);
+                        vals(va, p, 0);
+                        new_units(vs);
+                        packed_softmax(ks, vs, (u * 2 + k) * BLOCK, true);
+                        vals(vb, p, 1);
+                        values(va, 0);
+                        values(vb, 1);
+                    }
                 }
             }
             if (U > 0.0f) leave_units();

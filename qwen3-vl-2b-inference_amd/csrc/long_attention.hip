@@ -208,9 +208,9 @@ __device__ void long_row(const LongAttnArgs &a, const LongSeq &s, int b, int t, 
 //
 // Many rows: the four waves each widen a quarter of the next 64 positions into LDS,
 // in the operands' order, read ahead by a turn (each wave widening all of them for
-// itself: three trees of 61 rows over 16000 128 us for 63). Trees 63 us, 1000 rows
-// behind 8000 in fp16 91; matrix cores 33 and 34 of 100, other vector instructions
-// 35 and 44, two waves a SIMD.
+// itself: three trees of 61 rows over 16000 128 us for 63). Trees 59 us, 1000 rows
+// behind 8000 in fp16 87; matrix cores 36 and 37 of 100, other vector instructions
+// 39 and 47, two waves a SIMD.
 //
 // A window. The turns that no row of the workgroup sees are left out: the ones of
 // the first positions come first, then from the earliest window's start on. Within

@@ -21,10 +21,10 @@
 // once, or once more for each rejection. Two rounds are launched; a row that they
 // leave open goes on by itself, a workgroup for all its chunks.
 //
-// us at 151936 values, fp32: the sums of 83 rows 15.9, of 164 24.3 (4.1 TB/s: 64-bit
-// conversions and products, 69 of 100 busy cycles in vector instructions), a step
-// 6.6 (its chain of loads: lengths, parents and tokens, logits, the chunk), a round
-// of which two rows in five have a part 12.9, the path 3 to 4. All tests and the
+// us at 151936 values, fp32: the sums of 83 rows 15.5, of 164 24 (4.2 TB/s: 64-bit
+// conversions and products, 71 of 100 busy cycles in vector instructions), a step
+// 6 to 8 (its chain of loads: lengths, parents and tokens, logits, the chunk), a round
+// of which two rows in five have a part 12, the path 3 to 4. All tests and the
 // choice in one workgroup a row took 545 for the 83.
 #include "q3vl_device.hpp"
 #include "q3vl_kernels.hpp"

@@ -333,6 +333,7 @@ template <bool HALF, int SHIFT> __global__ __launch_bounds__(THREADS) void verif
                 c += z;
                 ++rejected;
                 if (rejected <= a.rounds) {
+                    __syncthreads();  // (every wave has read what the round before left)
                     if (tid == 0) {
                         a.state[r] = VerifyRow{c, m, child};
                         a.taken[r] = OPEN;

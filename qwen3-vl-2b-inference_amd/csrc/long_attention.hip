@@ -16,6 +16,10 @@ namespace {
 
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 
+// Weights p |vs| of packed positions: set to 2^BASE .. 2^(BASE + 2), they may grow
+// by 2^MORE before they are set anew, and stay under 2^15.
+constexpr float MORE = 7.0f;
+
 // What a block knows of its sequence.
 struct LongSeq {
     int start, n;  // its rows of q
@@ -190,12 +194,13 @@ __device__ void long_row(const LongAttnArgs &a, const LongSeq &s, int b, int t, 
 //
 // Packed blocks. int8 are exact in fp16, so a block's integers are operands as they
 // are, and its scales are factors: the keys' of the score (sc ks), the values' of
-// the probability, p vs. vs goes relative to U, a power of two that the largest (of either sign)
-// scale so far fits, so that p vs stays within fp16; O is in units of U until the
-// packed positions are done. l sums p itself, in fp32 and in the lane: a key with
-// much weight and tiny values must count in it. So nothing is held coarser than
-// tree_attention holds it (of p vs nothing finer than 2^-31 of the largest p times
-// the largest scale).
+// the probability, p vs. These weights have a reference of their own: each row's are
+// in units of a power of two that puts the largest p |vs| which the row has seen so
+// far at 2^BASE or a little more, whatever the scales of blocks that it does not see
+// or that weigh nothing in it; O is in those units until the packed positions are
+// done. l sums p itself, in fp32 and in the lane: a key with much weight and tiny
+// values must count in it. So no p vs is held finer than 2^-31 of the row's largest
+// p |vs|, as no p of a fp16 row finer than 2^-31 of its largest.
 //
 // Few rows: a wave takes a block of every four, 16 bytes a lane and load, straight
 // from memory into operand registers (the block's order is theirs) and widens them
@@ -455,16 +460,18 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
     for (int ks = 0; ks < KS; ++ks) kaddr[ks] = i * T::RB + ((ks * 4 + g) ^ swizzle<D>(i)) * 16;
     const int vr = 4 * g + (i >> 2);  // row of a 16-position tile this lane's transposing read starts from
     const int vaddr = vr * T::RB + (((i & 3) >> 1) ^ swizzle<D>(vr)) * 16 + (i & 1) * 8;
-    float M[NR], bias[NR], limit[NR], room[NR];  // limit: the score from which M is set anew, M + room
+    float M[NR], bias[NR], limit[NR];  // limit: the score from which M is set anew
     float4_t O[NT][NR], L[NR];  // L: the sum of p, in each register and lane of the column,
     float lsum[NR];             // and of packed positions, this lane's share
     bool any[NR];
+    float most[NR];  // packed positions: log2 of p |vs| from which O's units are set anew, and
+    int units[NR];   // those units, a power of two
     auto clear_rows = [&] {
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
-            M[nr] = limit[nr] = -INFINITY;
-            room[nr] = GROW / sc[nr];
+            M[nr] = limit[nr] = most[nr] = -INFINITY;
             bias[nr] = lsum[nr] = 0.0f;
+            units[nr] = 0;
             any[nr] = false;
             L[nr] = float4_t{0, 0, 0, 0};
 #pragma unroll
@@ -502,12 +509,16 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
     auto softmax = [&](float ks, float vs, auto packed) {
         float top[NR];  // of this lane's positions
         bool grow = false;
+        const float by = (float)(__float_as_uint(vs) >> 23 & 255);  // |vs| is in [2^(by - 127), 2^(by - 126)), or less for by = 0
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
             top[nr] = S[0][nr][0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) top[nr] = fmaxf(top[nr], S[e >> 2][nr][e & 3]);
-            if constexpr (packed) top[nr] *= ks;
+            if constexpr (packed) {
+                top[nr] *= ks;
+                grow = grow || fmaf(top[nr], sc[nr], by) > most[nr];
+            }
             grow = grow || top[nr] > limit[nr];
         }
         if (__any(grow)) {
@@ -516,13 +527,22 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                 const float m = fmaxf(M[nr], column_max(top[nr]));
                 const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], BASE);
                 const float f = M[nr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(nb - bias[nr]);
+                float fo = f;
+                if constexpr (packed) {  // the largest weight to [2^BASE, 2^(BASE + 2))
+                    const float w = fmaxf(most[nr] - MORE, column_max(fmaf(top[nr], sc[nr], by)));
+                    const float u = floorf(w + nb - (BASE + 127.0f));
+                    const int to = m == -INFINITY ? 0 : (int)fminf(fmaxf(u, -999.0f), 999.0f);
+                    fo = ldexpf(f, units[nr] - to);
+                    units[nr] = to;
+                    most[nr] = w + MORE;
+                }
                 M[nr] = m;
-                limit[nr] = m + room[nr];
+                limit[nr] = m + GROW / sc[nr];
                 bias[nr] = nb;
                 L[nr] *= f;
                 if constexpr (PACKED) lsum[nr] *= f;
 #pragma unroll
-                for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= f;
+                for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= fo;
             }
         }
 #pragma unroll
@@ -532,11 +552,12 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(S[e >> 2][nr][e & 3], c, bias[nr]));
             if constexpr (packed) {
+                const float v = ldexpf(vs, -units[nr]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) lsum[nr] += p[e];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    p[e] *= vs;
+                    p[e] *= v;
                     // (the product as it is rounded here: fused into the conversion below, the
                     // first term would now and then be another than the one the rest is of)
                     asm("" : "+v"(p[e]));
@@ -552,21 +573,6 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
     constexpr std::integral_constant<bool, true> kPacked{};
     constexpr std::integral_constant<bool, false> kRows{};
 
-    // Values of packed positions come out in units of U, a power of two that the
-    // largest scale of values so far fits.
-    float U = 0.0f, to_units = 0.0f;
-    auto new_units = [&](float vs) {
-        if (fabsf(vs) > U) {  // (uniform)
-            const int e = __builtin_amdgcn_frexp_expf(vs);
-            const float r = U > 0.0f ? ldexpf(U, -e) : 0.0f;
-            U = ldexpf(1.0f, e);
-            to_units = ldexpf(1.0f, -e);
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= r;
-        }
-    };
     auto packed_softmax = [&](float ks, float vs, int j, bool there = true) {
         if (there && inside(j)) {
 #pragma unroll
@@ -575,13 +581,12 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) masked(nr, there ? windowed ? window_bits(nr, j) : 0xFFFFFFFFu : 0u);
         }
-        softmax(ks, vs * to_units, kPacked);
+        softmax(ks, vs, kPacked);
     };
     // 32 packed positions from j on, out of registers; more_k and more_v: the keys'
     // and the values' registers are free
     auto packed_step = [&](const PackedBlock<D> &f, int j, auto more_k, auto more_v) {
         const float ks = f.ks, vs = f.vs;
-        new_units(vs);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
             zero_scores(kb);
@@ -606,7 +611,9 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= U;
+            for (int dt = 0; dt < NT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) O[dt][nr][e] = ldexpf(O[dt][nr][e], units[nr]);
     };
 
     // 32 fp16 rows from row j on, K and V at LDS offsets. Operand reads, half a
@@ -720,7 +727,6 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                         scores(ka, 0);
                         scores(kb, 1);
                         vals(va, p, 0);
-                        new_units(k ? v1 : v0);
                         packed_softmax(k ? k1 : k0, k ? v1 : v0, (u * 2 + k) * BLOCK, k == 0 || two);
                         vals(vb, p, 1);
                         values(va, 0);
@@ -738,7 +744,6 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                         scores(ka, 0);
                         scores(kb, 1);
                         vals(va, p, 0);
-                        new_units(vs);
                         packed_softmax(ks, vs, (u * 2 + k) * BLOCK, true);
                         vals(vb, p, 1);
                         values(va, 0);
@@ -746,7 +751,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                     }
                 }
             }
-            if (U > 0.0f) leave_units();
+            if (u0 < tp) leave_units();
         }
         for (int t = tp; t < u1; ++t, lds = T::STAGE - lds) {
             const int j = (turns.at(t) - turns.packed) * UNIT;
@@ -830,7 +835,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                 step(f[0], t);
                 if (t + 1 < tp) step(f[1], t + 1);
             }
-            if (U > 0.0f) leave_units();
+            if (u0 < tp) leave_units();
         } else {
             queries();
             clear_rows();

@@ -537,7 +537,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                     most[nr] = w + MORE;
                 }
                 M[nr] = m;
-                limit[nr] = m + GROW / sc[nr];
+                limit[nr] = m == -INFINITY ? m : m + GROW / sc[nr];  // (the quotient is infinite for the smallest queries)
                 bias[nr] = nb;
                 L[nr] *= f;
                 if constexpr (PACKED) lsum[nr] *= f;

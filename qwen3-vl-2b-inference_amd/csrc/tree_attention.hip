@@ -442,7 +442,7 @@ __global__ __launch_bounds__(THREADS, SHARED ? 2 : 1) void tree_attention_kernel
                 const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], BASE);
                 const float f = M[nr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(nb - bias[nr]);
                 M[nr] = m;
-                limit[nr] = m + room[nr];
+                limit[nr] = m == -INFINITY ? m : m + room[nr];  // (room is infinite for the smallest queries)
                 bias[nr] = nb;
                 L[nr] *= f;
 #pragma unroll

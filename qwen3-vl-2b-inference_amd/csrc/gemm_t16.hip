@@ -373,10 +373,13 @@ __global__ __launch_bounds__(64 * T::NW, MINB) void gemm_t16_kernel(
         for (int y = 0; y < FE; ++y)
             out[i][(x0 + y) / 4][(x0 + y) % 4] = fmaf(tt[y], ws[(x0 + y) / 4][us * GU + g], out[i][(x0 + y) / 4][(x0 + y) % 4]);
     };
-    // dword d of B * UC * 4 of raw, widened into bf[bs]
-    auto widen = [&](int bs, int d) __attribute__((always_inline)) {
+    // dword d of B * UC * 4 of raw, widened into bf[bs] (ahead: a fold stands
+    // between it and the next MFMA)
+    auto widen = [&](int bs, int d, bool ahead) __attribute__((always_inline)) {
         const int j = d / (UC * 4), u = d / 4 % UC, w = d % 4;
-        widen4(raw[j][u][w], bf[bs][j][2 * u + w / 2][2 * (w & 1)], bf[bs][j][2 * u + w / 2][2 * (w & 1) + 1]);
+        uint32_t &lo = bf[bs][j][2 * u + w / 2][2 * (w & 1)], &hi = bf[bs][j][2 * u + w / 2][2 * (w & 1) + 1];
+        if (ahead) widen4_ahead(raw[j][u][w], lo, hi);
+        else widen4(raw[j][u][w], lo, hi);
     };
     constexpr int ND = B * UC * 4;           // dwords to widen per unit
     constexpr int NSUB = (A - 1) * NM;       // sub-steps that widen (the next unit's first MFMA follows)
@@ -418,7 +421,7 @@ __global__ __launch_bounds__(64 * T::NW, MINB) void gemm_t16_kernel(
                     const int sub = i * NM + k;
 #pragma unroll
                     for (int x = 0; x < ND; ++x)
-                        if (x * NSUB / ND == sub) widen((us + 1) & 1, x);
+                        if (x * NSUB / ND == sub) widen((us + 1) & 1, x, true);
                 }
                 __builtin_amdgcn_sched_barrier(0);
                 fold(i, us, k, tt, ws);
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(64 * T::NW, MINB) void gemm_t16_kernel(
         for (int x = 0; x < PD; ++x) read_fr(x, x / A >= SU ? 1 : 0, x / A % SU, x % A);
         read_raw(0, 0);
 #pragma unroll
-        for (int x = 0; x < ND; ++x) widen(0, x);
+        for (int x = 0; x < ND; ++x) widen(0, x, false);
         if (UB == 1) {
             __builtin_amdgcn_sched_barrier(0);
             load_b(0, min(NB, lastb));
@@ -528,7 +531,7 @@ __global__ __launch_bounds__(64 * T::NW, MINB) void gemm_t16_kernel(
         lds_barrier();
         read_as(0, 0, 0);
 #pragma unroll
-        for (int x = 0; x < ND; ++x) widen(0, x);
+        for (int x = 0; x < ND; ++x) widen(0, x, false);
 #pragma unroll
         for (int i = 0; i < A; ++i) {
             read_fr(0, 0, 0, i);

@@ -24,9 +24,8 @@ template <int D> __host__ __device__ __forceinline__ constexpr int value_at(int 
 }
 
 // Eight int8 as fp16, exactly: a byte u under the byte 0x64 is the half 1024 + u,
-// so x ^ 0x80 gives 1152 + x. (widen4's conversions in asm are not for operands
-// that a matrix instruction has just read: written over too early there, two of
-// eight products came out wrong.)
+// so x ^ 0x80 gives 1152 + x. (No asm as in widen8: the compiler moves these
+// instructions between the products and knows their waits.)
 Q3VL_INLINE half8_t widen8_plain(uint32_t x, uint32_t y) {
     typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
     const half2_t off = {(_Float16)-1152.0f, (_Float16)-1152.0f};

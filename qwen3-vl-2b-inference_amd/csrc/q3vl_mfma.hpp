@@ -70,18 +70,28 @@ Q3VL_INLINE float quant_team(const float4 (&cv)[GS / 16], Store store) {
 // source select) and writing one half of the destination, exact for every
 // int8. The two destinations alternate, so no instruction reads the half that
 // the one right before it wrote.
+//
+// A matrix instruction may read a vector instruction's result after two wait
+// states. The compiler keeps them for its own instructions, not for these, so
+// the asm ends with them. widen4_ahead leaves them out, for results that other
+// vector instructions follow (tests/test_mfma_waits.py reads the built code).
+#define Q3VL_WIDEN(half, unused, lo, hi, x, b0, b2)                                                      \
+    "v_cvt_f16_i16_sdwa " lo ", sext(" x ") dst_sel:" half " dst_unused:" unused " src0_sel:" b0 "\n\t" \
+    "v_cvt_f16_i16_sdwa " hi ", sext(" x ") dst_sel:" half " dst_unused:" unused " src0_sel:" b2 "\n\t"
+#define Q3VL_WIDEN_LOW(lo, hi, x) Q3VL_WIDEN("WORD_0", "UNUSED_PAD", lo, hi, x, "BYTE_0", "BYTE_2")
+#define Q3VL_WIDEN_HIGH(lo, hi, x) Q3VL_WIDEN("WORD_1", "UNUSED_PRESERVE", lo, hi, x, "BYTE_1", "BYTE_3")
+Q3VL_INLINE void widen4_ahead(uint32_t x, uint32_t &lo, uint32_t &hi) {
+    asm(Q3VL_WIDEN_LOW("%0", "%1", "%2") Q3VL_WIDEN_HIGH("%0", "%1", "%2") : "=&v"(lo), "=&v"(hi) : "v"(x));
+}
 Q3VL_INLINE void widen4(uint32_t x, uint32_t &lo, uint32_t &hi) {
-    asm("v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_0\n\t"
-        "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:BYTE_2\n\t"
-        "v_cvt_f16_i16_sdwa %0, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_1\n\t"
-        "v_cvt_f16_i16_sdwa %1, sext(%2) dst_sel:WORD_1 dst_unused:UNUSED_PRESERVE src0_sel:BYTE_3"
-        : "=&v"(lo), "=&v"(hi)
-        : "v"(x));
+    asm(Q3VL_WIDEN_LOW("%0", "%1", "%2") Q3VL_WIDEN_HIGH("%0", "%1", "%2") "s_nop 1" : "=&v"(lo), "=&v"(hi) : "v"(x));
 }
 Q3VL_INLINE half8_t widen8(uint32_t x, uint32_t y) {
     uint32_t a, b, c, d;
-    widen4(x, a, b);
-    widen4(y, c, d);
+    asm(Q3VL_WIDEN_LOW("%0", "%1", "%4") Q3VL_WIDEN_LOW("%2", "%3", "%5")
+        Q3VL_WIDEN_HIGH("%0", "%1", "%4") Q3VL_WIDEN_HIGH("%2", "%3", "%5") "s_nop 1"
+        : "=&v"(a), "=&v"(b), "=&v"(c), "=&v"(d)
+        : "v"(x), "v"(y));
     return __builtin_bit_cast(half8_t, (u32x4){a, b, c, d});
 }
 

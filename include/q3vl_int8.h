@@ -514,9 +514,10 @@ int q3vl_kv_unpack(const q3vl_kv_blocks *blocks, const int32_t *packed_len, cons
  * blocks and packed_len NULL: none), then those of `cache`, and through a
  * window: of the positions that a row would see, in their order, it sees the
  * first `sinks` and the last `window` (window 0: all). A window over a mask is
- * at least max_rows. Arguments, types and results are otherwise
- * q3vl_tree_attention's; max_len counts packed positions too, and 0 stands for
- * all that the cache and the blocks can hold. A sequence also gives NaN where packed_len[b] is not a
+ * at least max_rows, or `rows` where they are fewer, and no row's mask has more
+ * bits. Arguments, types and results are otherwise q3vl_tree_attention's;
+ * max_len counts packed positions too, and 0 stands for all that the cache and
+ * the blocks can hold. A sequence also gives NaN where packed_len[b] is not a
  * multiple of 32 in [0, 32 * blocks->blocks]. A row that sees a position of a
  * block with a NaN scale gives NaN. */
 size_t q3vl_long_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,

@@ -1825,8 +1825,9 @@ int q3vl_long_attention(const void *q, size_t ldq, void *out, size_t ldo, int dt
     if (out == q && ldo != ldq && rows > 1) return fail(Q3VL_ERR_INVALID_ARGUMENT, "out over q needs q's stride");
     if (mask_words < 0 || (mask && mask_words < 1) || mask_words > (1 << 24))
         return fail(Q3VL_ERR_INVALID_ARGUMENT, "mask_words=%d", mask_words);
-    if (window && mask && window < max_rows)
-        return fail(Q3VL_ERR_UNSUPPORTED, "window=%d over masks of up to %d rows: at least as many are served", window, max_rows);
+    const int most_rows = (size_t)max_rows < rows ? max_rows : (int)rows;  // (no sequence has more)
+    if (window && mask && window < most_rows)
+        return fail(Q3VL_ERR_UNSUPPORTED, "window=%d over masks of up to %d rows: at least as many are served", window, most_rows);
     if (!blocks != !packed_len) return fail(Q3VL_ERR_INVALID_ARGUMENT, "blocks and packed_len come together");
     const float scale_log2e = (float)((double)scale * 1.4426950408889634);
     if (!(scale_log2e > -INFINITY && scale_log2e < INFINITY))

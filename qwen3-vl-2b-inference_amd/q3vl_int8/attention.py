@@ -462,8 +462,8 @@ def long_attention(q, cache, row_start, cache_len, max_rows, packed=None, packed
     """tree_attention over the packed_len[b] positions of `packed` and, behind
     them, those of the cache; through a window where one is given: of what a row
     would see it sees the first `sinks` positions and the last `window` (with a
-    mask at least max_rows). packed None: the cache alone. max_len counts packed
-    positions too. The rest as tree_attention. workspace:
+    mask at least max_rows, or q's rows where they are fewer). packed None: the
+    cache alone. max_len counts packed positions too. The rest as tree_attention. workspace:
     alloc_long_attention_workspace with the same packed, max_rows, max_len,
     window and sinks."""
     torch, dev = _device()

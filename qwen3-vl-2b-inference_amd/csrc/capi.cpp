@@ -1781,17 +1781,27 @@ static int check_long_attention(size_t rows, int heads, int max_rows, int max_le
     return Q3VL_OK;
 }
 
+// Rows as the plan counts them: each up to 64, from there on eight steps an
+// octave. So a workspace for the most bytes of any fewer rows is found at few of
+// them (a plan of more rows may split less, and need less).
+static size_t row_step(size_t rows) {
+    size_t step = rows <= 64 ? 1 : 8;
+    while (step > 1 && rows > 16 * step) step *= 2;
+    return step;
+}
+
 // A call's tile and splits, and its workspace bytes. Through a window a
 // workgroup's rows see its positions, the first ones and their own.
 static TreePlan plan_long_attention(size_t rows, int heads, int max_rows, int max_len, int window, int sinks, const q3vl_kv_cache *c,
                                     const q3vl_kv_blocks *p, bool half, bool chain, size_t *bytes, int *most = nullptr) {
-    if ((size_t)max_rows > rows) max_rows = (int)rows;
+    const size_t step = row_step(rows), counted = (rows + step - 1) / step * step;
+    if ((size_t)max_rows > counted) max_rows = (int)counted;
     const int64_t room = (int64_t)c->max_seq + (p ? (int64_t)p->blocks * 32 : 0);
     int64_t len = max_len && max_len < room ? max_len : room;
     if (window && (int64_t)window + sinks + max_rows < len) len = (int64_t)window + sinks + max_rows;
     if (len > INT32_MAX - 256) len = INT32_MAX - 256;
     if (most) *most = (int)len;
-    const TreePlan t = long_attention_plan((int64_t)rows, heads, c->kv_heads, c->batch, max_rows, (int)len, c->head_dim, half, chain, p);
+    const TreePlan t = long_attention_plan((int64_t)counted, heads, c->kv_heads, c->batch, max_rows, (int)len, c->head_dim, half, chain, p);
     const size_t parts = rows * (size_t)heads * (size_t)t.splits;
     *bytes = t.splits > 1 ? align256(parts * (size_t)c->head_dim * 4) + align256(parts * 8) : 0;
     return t;
@@ -1802,10 +1812,15 @@ size_t q3vl_long_attention_workspace_bytes(size_t rows, int heads, int max_rows,
                                            const q3vl_kv_blocks *blocks) {
     if (check_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks)) return 0;
     size_t most = 0;
-    for (int i = 0; i < 4; ++i) {  // types, chains and trees
-        size_t bytes = 0;
-        plan_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks, i & 1, i >> 1, &bytes);
-        most = bytes > most ? bytes : most;
+    const size_t each = (size_t)heads * kLongSplits * (cache->head_dim * 4 + 8);  // (a row's bytes at most)
+    while (rows > 0 && rows * each + 512 > most) {
+        for (int i = 0; i < 4; ++i) {  // types, chains and trees
+            size_t bytes = 0;
+            plan_long_attention(rows, heads, max_rows, max_len, window, sinks, cache, blocks, i & 1, i >> 1, &bytes);
+            most = bytes > most ? bytes : most;
+        }
+        const size_t step = row_step(rows);
+        rows = (rows + step - 1) / step * step - step;  // (the most rows that are counted as fewer)
     }
     return most;
 }

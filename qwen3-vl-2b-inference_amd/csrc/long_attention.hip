@@ -1089,7 +1089,7 @@ TreePlan long_attention_plan(int64_t rows, int heads, int kv_heads, int batch, i
         break;
     }
     k = k < most ? k : most;
-    return {16, (int)(k < 1 ? 1 : k < 32 ? k : 32)};
+    return {16, (int)(k < 1 ? 1 : k < kLongSplits ? k : kLongSplits)};
 }
 
 template <int D, bool HALF, int NR, bool SHARED, bool PACKED, bool ONCE>

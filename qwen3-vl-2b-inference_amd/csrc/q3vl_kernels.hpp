@@ -299,6 +299,7 @@ struct LongAttnArgs : TreeAttnArgs {
 };
 TreePlan long_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim, bool half,
                              bool chain, bool packed);
+constexpr int kLongSplits = 32;  // most
 hipError_t launch_long_attention(const LongAttnArgs &a, int head_dim, bool half, int block_rows, hipStream_t st);
 
 struct VerifyRow {  // a row that waits for a round's sums

@@ -706,6 +706,7 @@ template <int D, bool HALF> __global__ __launch_bounds__(THREADS) void tree_join
 namespace {
 
 constexpr int kSplits = 32;  // most (a lane of the joining wave each; 64 gained nothing and cost up to half more)
+static_assert(kSplits <= kLongSplits, "long_attention_plan's most");
 constexpr int64_t kBlocks = (1 << 24) - 1;  // of 256 threads in a launch
 
 }  // namespace

@@ -452,7 +452,7 @@ def long_attention_workspace_bytes(cache, rows, heads, max_rows, max_len=None, p
 
 
 def alloc_long_attention_workspace(cache, rows, heads, max_rows, max_len=None, packed=None, window=0, sinks=0):
-    """Device workspace for long_attention at these sizes."""
+    """Device workspace for long_attention at these sizes, and of fewer rows."""
     n = long_attention_workspace_bytes(cache, rows, heads, max_rows, max_len, packed, window, sinks)
     return _torch().empty(max(n, 256), dtype=_torch().uint8, device=cache.device)
 
@@ -463,9 +463,9 @@ def long_attention(q, cache, row_start, cache_len, max_rows, packed=None, packed
     them, those of the cache; through a window where one is given: of what a row
     would see it sees the first `sinks` positions and the last `window` (with a
     mask at least max_rows, or q's rows where they are fewer). packed None: the
-    cache alone. max_len counts packed positions too. The rest as tree_attention. workspace:
-    alloc_long_attention_workspace with the same packed, max_rows, max_len,
-    window and sinks."""
+    cache alone. max_len counts packed positions too. The rest as
+    tree_attention. workspace: alloc_long_attention_workspace with no fewer rows
+    and the same packed, max_rows, max_len, window and sinks."""
     torch, dev = _device()
     ldq = _rows(q, (torch.float32, torch.float16), "q", dev)
     c = cache.c

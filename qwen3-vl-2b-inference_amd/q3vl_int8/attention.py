@@ -150,6 +150,14 @@ def _mask_words(mask, rows, dev):
     return words
 
 
+def _wide(**numbers):
+    """Refuses what a C int does not hold: ctypes would take its low bits. (Calls
+    ask first whether a number is negative or wide.)"""
+    for name, v in numbers.items():
+        if not -1 << 31 <= v < 1 << 31:
+            raise ValueError(f"{name}={v}: below 2^31")
+
+
 def _workspace(t, dev):
     """(address, bytes) of a call's workspace; none: the library's own."""
     if t is None:
@@ -443,10 +451,14 @@ def kv_unpack(packed, packed_len, cache, first=None, count=None, stream=None):
         _vec(first, torch.int32, c.batch, "first", dev)
     if count is None:
         count = min(32 * packed.c.blocks, c.max_seq)
+    if count >> 31:
+        _wide(count=count)
     _check(_L().q3vl_kv_unpack(packed.ref, packed_len.data_ptr(), _ptr(first), cache.ref, count, _raw_stream(stream, torch, dev)))
 
 
 def long_attention_workspace_bytes(cache, rows, heads, max_rows, max_len=None, packed=None, window=0, sinks=0) -> int:
+    if (max_rows | (max_len or 0) | window | sinks) >> 31:
+        _wide(max_rows=max_rows, max_len=max_len or 0, window=window, sinks=sinks)
     return _L().q3vl_long_attention_workspace_bytes(rows, heads, max_rows, max_len or 0, window, sinks, cache.ref,
                                                     None if packed is None else packed.ref)
 
@@ -473,6 +485,8 @@ def long_attention(q, cache, row_start, cache_len, max_rows, packed=None, packed
     rows, qn = q.shape
     if qn % D:
         raise ValueError("q's rows must be whole heads of the cache's head_dim")
+    if (max_rows | (max_len or 0) | window | sinks) >> 31:
+        _wide(max_rows=max_rows, max_len=max_len or 0, window=window, sinks=sinks)
     if cache.dev != dev:
         raise ValueError("cache must be on the current device")
     if (packed is None) != (packed_len is None):
@@ -543,6 +557,7 @@ def verify_drafts(logits, tokens, parents, row_start, accept_u, sample_u, max_ro
     _vec(sample_u, f32, rows, "sample_u", dev)
     if max_rows < 0:
         raise ValueError("max_rows must not be negative")
+    _wide(max_rows=max_rows)
     accepted, path, nxt = _empty(tokens, stream, batch), _empty(tokens, stream, batch, max_rows), _empty(tokens, stream, batch)
     wp, wb = _workspace(workspace, dev)
     rc = (_verify_fn or _L().q3vl_verify_drafts)(

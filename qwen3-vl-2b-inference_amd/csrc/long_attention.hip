@@ -460,11 +460,12 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
     for (int ks = 0; ks < KS; ++ks) kaddr[ks] = i * T::RB + ((ks * 4 + g) ^ swizzle<D>(i)) * 16;
     const int vr = 4 * g + (i >> 2);  // row of a 16-position tile this lane's transposing read starts from
     const int vaddr = vr * T::RB + (((i & 3) >> 1) ^ swizzle<D>(vr)) * 16 + (i & 1) * 8;
-    float M[NR], bias[NR], limit[NR];  // limit: the score from which M is set anew
+    float M[NR], bias[NR];
+    float limit[NR];  // of fp16 rows: the score from which M is set anew
     float4_t O[NT][NR], L[NR];  // L: the sum of p, in each register and lane of the column,
     float lsum[NR];             // and of packed positions, this lane's share
     bool any[NR];
-    float most[NR];  // packed positions: log2 of p |vs| from which O's units are set anew, and
+    float most[NR];  // of packed positions: log2 of p |vs|, and 126, from which O's units are set anew
     int units[NR];   // those units, a power of two
     auto clear_rows = [&] {
 #pragma unroll
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
             bias[nr] = lsum[nr] = 0.0f;
             units[nr] = 0;
             any[nr] = false;
-            L[nr] = float4_t{0, 0, 0, 0};
+            if constexpr (!PACKED) L[nr] = float4_t{0, 0, 0, 0};
 #pragma unroll
             for (int dt = 0; dt < NT; ++dt) O[dt][nr] = float4_t{0, 0, 0, 0};
         }
@@ -517,29 +518,30 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
             for (int e = 1; e < 8; ++e) top[nr] = fmaxf(top[nr], S[e >> 2][nr][e & 3]);
             if constexpr (packed) {
                 top[nr] *= ks;
-                grow = grow || fmaf(top[nr], sc[nr], by) > most[nr];
+                grow = grow || fmaf(top[nr], sc[nr], bias[nr]) > fminf(BASE + GROW, most[nr] - by);
+            } else {
+                grow = grow || top[nr] > limit[nr];
             }
-            grow = grow || top[nr] > limit[nr];
         }
         if (__any(grow)) {
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-                const float m = fmaxf(M[nr], column_max(top[nr]));
+                const float t = column_max(top[nr]), m = fmaxf(M[nr], t);
                 const float nb = m == -INFINITY ? 0.0f : fmaf(-m, sc[nr], BASE);
                 const float f = M[nr] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(nb - bias[nr]);
                 float fo = f;
-                if constexpr (packed) {  // the largest weight to [2^BASE, 2^(BASE + 2))
-                    const float w = fmaxf(most[nr] - MORE, column_max(fmaf(top[nr], sc[nr], by)));
-                    const float u = floorf(w + nb - (BASE + 127.0f));
-                    const int to = m == -INFINITY ? 0 : (int)fminf(fmaxf(u, -999.0f), 999.0f);
+                if constexpr (packed) {  // the largest weight to [2^BASE, 2^(BASE + 2)), or up to that from below
+                    const float w = fmaxf(M[nr] == -INFINITY ? M[nr] : most[nr] - MORE + (nb - bias[nr]), fmaf(t, sc[nr], nb) + by);
+                    const int to = (int)fminf(fmaxf(floorf(w - (BASE + 127.0f)), -999.0f), 999.0f);
                     fo = ldexpf(f, units[nr] - to);
                     units[nr] = to;
-                    most[nr] = w + MORE;
+                    most[nr] = m == -INFINITY ? m : (float)to + (BASE + 127.0f + MORE);
+                } else {
+                    limit[nr] = m == -INFINITY ? m : m + GROW / sc[nr];  // (the quotient is infinite for the smallest queries)
+                    L[nr] *= f;
                 }
                 M[nr] = m;
-                limit[nr] = m == -INFINITY ? m : m + GROW / sc[nr];  // (the quotient is infinite for the smallest queries)
                 bias[nr] = nb;
-                L[nr] *= f;
                 if constexpr (PACKED) lsum[nr] *= f;
 #pragma unroll
                 for (int dt = 0; dt < NT; ++dt) O[dt][nr] *= fo;
@@ -607,13 +609,16 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
         }
         more_v();
     };
-    auto leave_units = [&] {  // O in the values' own units
+    auto leave_packed = [&] {  // to fp16 rows: O in the values' own units
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr)
+        for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
             for (int dt = 0; dt < NT; ++dt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) O[dt][nr][e] = ldexpf(O[dt][nr][e], units[nr]);
+            L[nr] = float4_t{0, 0, 0, 0};
+            limit[nr] = M[nr] == -INFINITY ? M[nr] : M[nr] + GROW / sc[nr];
+        }
     };
 
     // 32 fp16 rows from row j on, K and V at LDS offsets. Operand reads, half a
@@ -751,7 +756,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                     }
                 }
             }
-            if (u0 < tp) leave_units();
+            leave_packed();
         }
         for (int t = tp; t < u1; ++t, lds = T::STAGE - lds) {
             const int j = (turns.at(t) - turns.packed) * UNIT;
@@ -835,7 +840,7 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                 step(f[0], t);
                 if (t + 1 < tp) step(f[1], t + 1);
             }
-            if (u0 < tp) leave_units();
+            leave_packed();
         } else {
             queries();
             clear_rows();
@@ -1067,12 +1072,12 @@ __global__ __launch_bounds__(THREADS) void long_join_kernel(const int32_t *row_s
 // 119 in shared tiles of 64; of 20 rows 94 and 131 shared; of 32 139 and 140; of
 // 40 146 and 146, 6 of 40 53 and 51.
 // As many splits as fill whole rounds of 512 workgroups to nine tenths (the rule's
-// choice first): one token of 4 sequences of 16000 24.9 at 16, 27.6 at 8; of 8 of
-// 12000 32.6 at 8, 39.3 at 4; of 12 47.1 at 5, 58.2 at 2; of 24 86.9 at 5, 95.6 at
-// 2, 85.3 at 8; of 40 of 3000 43.7 at 3, 46.4 at 1. Below 512 positions a split one
-// round of 256: one token of 8 of 3000 17.2 at 4, 17.9 at 8; of 2 of 8000 15.0 at
-// 16, 16.8 at 32; 6 trees of 20 over 1000 15.1 at 1, 16.7 at 4. (All of one length:
-// 32 of 8192 90.8 at 2, 87.6 at 1, which the host cannot tell apart.)
+// choice first): one token of 4 sequences of 16000 25.2 at 15, 24.9 at 16, 26.9 at
+// 8; of 8 of 12000 31.7 at 8, 34.9 at 4; of 12 47.0 at 5, 55.4 at 2; of 24 84.7 at
+// 5, 90.6 at 2, 83.8 at 8; of 40 of 3000 43.7 at 3, 44.6 at 1. Below 512 positions
+// a split one round of 256: one token of 8 of 3000 16.9 at 4, 17.8 at 8; of 2 of
+// 8000 14.9 at 16, 16.5 at 32; 6 trees of 20 over 1000 15.1 at 1, 16.2 at 4. (All of
+// one length: 32 of 8192 90.8 at 2, 87.6 at 1, which the host cannot tell apart.)
 //
 // Else as tree_attention_plan says, whose kernels these are.
 TreePlan long_attention_plan(int64_t rows, int heads, int kv_heads, int batch, int max_rows, int max_len, int head_dim, bool half,

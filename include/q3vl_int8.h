@@ -519,9 +519,11 @@ int q3vl_kv_unpack(const q3vl_kv_blocks *blocks, const int32_t *packed_len, cons
  * max_len counts packed positions too, and 0 stands for all that the cache and
  * the blocks can hold. A sequence also gives NaN where packed_len[b] is not a
  * multiple of 32 in [0, 32 * blocks->blocks]. A row that sees a position of a
- * block with a NaN scale gives NaN. Workspace: the bytes for as many rows, and
- * the same heads, max_rows, max_len, window, sinks, cache and blocks, serve any
- * call of no more rows, of any type and mask. */
+ * block with a NaN scale gives NaN. Of packed positions no probability times its
+ * block's value scale is held finer than 2^-31 of the largest such product that
+ * the row sees, whatever other blocks' scales are. Workspace: the bytes for as
+ * many rows, and the same heads, max_rows, max_len, window, sinks, cache and
+ * blocks, serve any call of no more rows, of any type and mask. */
 size_t q3vl_long_attention_workspace_bytes(size_t rows, int heads, int max_rows, int max_len,
                                            int window, int sinks, const q3vl_kv_cache *cache,
                                            const q3vl_kv_blocks *blocks);

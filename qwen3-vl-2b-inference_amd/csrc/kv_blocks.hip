@@ -38,8 +38,10 @@ template <int GAP> __device__ __forceinline__ int spread(int at) { return at + a
 // rows that this one alone reads, before it writes them.
 //
 // Bound by latency at a step's size (192 blocks 5.4 us); a prompt of 4099 rows, 25
-// MB in and out, 8.8 us (with the block's bytes unspread in LDS, values a byte at a
-// time, and the compiler's division 10.6).
+// MB in and out, 8.4 us (with the block's bytes unspread in LDS, values a byte at a
+// time, and the compiler's division 10.6). The grid is what the cache can hold, not
+// what it does: 24 sequences with one whole block among them, 8 heads, us a call 5.0
+// at 64 rows a sequence, 5.2 at 512, 14.0 at 4160, 26.5 at 8192.
 template <int D> __global__ __launch_bounds__(THREADS) void kv_pack_kernel(KvPackArgs a, int most) {
     constexpr int HALF = THREADS / 2, PIECES = BLOCK * D / 8 / HALF;  // pieces of 8 values a thread
     __shared__ __align__(16) unsigned char tile[2][BLOCK * D / 256 * (256 + KGAP)];

@@ -213,15 +213,17 @@ __device__ void long_row(const LongAttnArgs &a, const LongSeq &s, int b, int t, 
 //
 // Many rows: the four waves each widen a quarter of the next 64 positions into LDS,
 // in the operands' order, read ahead by a turn (each wave widening all of them for
-// itself: three trees of 61 rows over 16000 128 us for 63). Trees 59 us, 1000 rows
-// behind 8000 in fp16 87; matrix cores 36 and 37 of 100, other vector instructions
-// 39 and 47, two waves a SIMD.
+// itself: three trees of 61 rows over 16000 128 us for 63). Trees 60 us, 1000 rows
+// behind 8000 in fp16 89; matrix cores 36 of 100, other vector instructions 40 and
+// 49, two waves a SIMD. (One unit for all rows of a wave, which loses bits: 59 and
+// 87.) In fp32 and heads of 128 the tiles of 128 rows take all 256 registers, with 6
+// spilled over blocks and 8 without.
 //
 // A window. The turns that no row of the workgroup sees are left out: the ones of
 // the first positions come first, then from the earliest window's start on. Within
 // the others a lane masks what its row does not see, where some row does not see
 // all. One token of 16 sequences through 4096 positions 45 us, 6.0 TB/s; a prompt
-// of 4000 through 1024 in fp16 48 us.
+// of 4000 through 1024 in fp16 49 us.
 template <int D, int NR, bool SHARED, bool PACKED> struct LongTile {
     static constexpr int RB = 2 * D;                           // bytes of an fp16 row
     static constexpr int NS = SHARED ? 2 : PACKED ? 128 / D : 256 / D;  // stages of fp16 rows
@@ -720,9 +722,10 @@ __global__ __launch_bounds__(THREADS, SHARED || PACKED ? 2 : 1) void long_attent
                     for (int i = 0; i < NT / 2; ++i) f[i] = *reinterpret_cast<const half8_t *>(p + 64 * T::RB + (part * (NT / 2) + i) * 1024);
                     __builtin_amdgcn_sched_barrier(0);
                 };
-                // (us a call, scales loaded where they are needed and a loop over the blocks: trees
-                // in fp32 69, a prompt in fp16 100. Scales a turn ahead: 61 and 101; both blocks
-                // in a row, the second's keys read under the first's last products: 68 and 94.)
+                // (us a call when all rows shared their units, scales loaded where they are needed
+                // and a loop over the blocks: trees in fp32 69, a prompt in fp16 100. Scales a turn
+                // ahead: 61 and 101; both blocks in a row, the second's keys read under the first's
+                // last products: 68 and 94.)
                 if constexpr (HALF) {
                     keys(ka, at, 0);
 #pragma unroll

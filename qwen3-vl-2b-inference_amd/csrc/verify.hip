@@ -19,7 +19,11 @@
 // it. A row whose child is rejected waits for a round: its chunks' sums of max(p
 // - c q, 0), by all workgroups again, then the next test. So each logit is read
 // once, or once more for each rejection. Two rounds are launched; a row that they
-// leave open goes on by itself, a workgroup for all its chunks.
+// leave open goes on by itself, a workgroup for all its chunks, which costs most
+// where trees have many children a row. us a call with 1, 2, 4 and 6 rounds, values
+// as below: 16 chains of 8 rows 43, 47, 55, 63; 8 trees of 16 rows 102, 53, 60, 68; 3
+// trees of 61 rows, with up to nine children, 212, 171, 113, 103 (with 2, the last
+// step alone 126).
 //
 // us at 151936 values, fp32: the sums of 83 rows 15.5, of 164 24 (4.2 TB/s: 64-bit
 // conversions and products, 71 of 100 busy cycles in vector instructions), a step

@@ -13,7 +13,7 @@ from test_rows_capi import cache
 
 torch = pytest.importorskip("torch")
 
-ROWS = sorted({*range(1, 150), *(1 << i for i in range(18)), *(3 << i for i in range(16)), 511, 513, 1000, 1001, 4097, 100000})
+ROWS = sorted({*range(1, 150), *(1 << i for i in range(18)), *(5 << i for i in range(15)), 511, 513, 1000, 1001, 4097, 100000})
 
 
 @pytest.mark.parametrize("packed", [True, False], ids=["packed", "fp16 rows"])
